@@ -283,7 +283,7 @@ def _append(s):
 
 def _evict(s):
     """Keeps `budget` slots of each head: those of the first `sinks` and the last `recent` positions, then the
-    largest scores (ties: the lowest slot).  Kept slots below the new length stay; the others move, in order,
+    largest scores (NaN last, ties: the lowest slot).  Kept slots below the new length stay; the others move, in order,
     into the places that became free."""
     scores, positions, table = s["scores"], s["positions"], s["table"]
     pages, hkv, ps, _ = s["k"].shape
@@ -292,7 +292,7 @@ def _evict(s):
     lens = s["lens"][:, None, None]
     new = lens.clamp(max=s["budget"])
     kept_always = (positions < s["sinks"]) | (positions >= s["seen"][:, None, None] - s["recent"])
-    key = torch.nan_to_num(scores.double(), nan=-1e300, posinf=1e300, neginf=-1e300)
+    key = torch.nan_to_num(scores.double(), nan=-2e300, posinf=1e300, neginf=-1e300)
     key = torch.where(slot < lens, torch.where(kept_always, 2e300, key), -math.inf)
     rank = key.argsort(dim=-1, descending=True, stable=True).argsort(-1)
     keep = rank < new
