@@ -15,9 +15,9 @@
  *     tallax_last_error().
  *   - dtype codes: TALLAX_F32 = 0, TALLAX_BF16 = 1, TALLAX_I32 = 2.
  *
- * Each entry point replaces one jit-wrapped Pallas call of the reference
- * (oliverdutton/tallax); the reference interface is cited above each
- * declaration as file:line.
+ * Entry points that replace a jit-wrapped Pallas call of the reference
+ * (oliverdutton/tallax) cite its interface above their declaration as
+ * file:line; the others say that they have no counterpart there.
  */
 #ifndef TALLAX_HIP_H_
 #define TALLAX_HIP_H_
@@ -300,6 +300,115 @@ int tallax_sort_rows_ws(const void* key, int key_dtype, int64_t rows, int64_t co
  * ---------------------------------------------------------------------- */
 int tallax_softmax_topk_cumsum(const float* logits, int64_t rows, int64_t cols, int k, float p, float* out_probs,
                                int32_t* out_idx, float* out_cumsum, int32_t* out_cutoff, tallax_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * A paged key-value cache.  NO COUNTERPART IN THE REFERENCE (it samples from
+ * logits; the cache is what the model before the sampler reads).
+ * k, v: pools of `pages` pages, each [kv_heads, page_size, dim] of dtype f32 or
+ * bf16.  Strides are in elements, for a page, a head and a slot; the dim
+ * elements of a slot are contiguous, and base addresses and strides are
+ * multiples of 16 bytes (any order of heads and slots inside a page fits).
+ * dim: a multiple of 8 up to 256.
+ * block_table [batch, table_width] int32: slot s of sequence b lies in page
+ * block_table[b][s / page_size] at place s % page_size.  An entry outside
+ * [0, pages) is no page: its slots are neither written nor seen.  Only entries
+ * of slots below the sequence's length are looked at.
+ * Pages that several sequences share may be read, but not appended to or evicted from.
+ * ---------------------------------------------------------------------- */
+typedef struct tallax_kv_cache {
+  void* k;
+  void* v;
+  int32_t dtype;
+  int32_t dim;
+  int64_t pages, kv_heads, page_size;
+  int64_t k_stride_page, k_stride_head, k_stride_slot;
+  int64_t v_stride_page, v_stride_head, v_stride_slot;
+  const int32_t* block_table;
+  int64_t batch, table_width;
+} tallax_kv_cache;
+
+/* ------------------------------------------------------------------------
+ * Writes k_new, v_new [batch, tokens, kv_heads, dim] (dense, the cache's
+ * dtype) into slots lens[b] .. lens[b] + counts[b] - 1 of each sequence
+ * (counts [batch] int32, null: all of `tokens`; clamped to [0, tokens]).
+ * Slots past the table's capacity or in no page are dropped.  scores,
+ * positions [batch, kv_heads, table_width * page_size] (both or neither): the
+ * written slots get score 0 and position seen[b] + t.  out_lens [batch] =
+ * min(lens + counts, capacity), a buffer other than lens.
+ * ---------------------------------------------------------------------- */
+int tallax_kv_append(const tallax_kv_cache* cache, const int32_t* lens, const int32_t* counts, const void* k_new,
+                     const void* v_new, int64_t tokens, float* scores, int32_t* positions, const int32_t* seen,
+                     int32_t* out_lens, tallax_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of the newest tokens over the cache.  q, out [batch, queries,
+ * heads, dim] (q with element strides for its first three axes, out dense);
+ * head h reads kv head h / (heads / kv_heads).  Query t < counts[b] (counts
+ * null: queries) of sequence b sees slots j < lens[b] - counts[b] + t + 1;
+ * queries t >= counts[b] see none.
+ *   x_j = scale * q.k_j, lse = log sum_j exp(x_j), w_j = exp(x_j - lse),
+ *   out = sum_j w_j v_j.
+ * A query that sees no slot, or whose every x_j is -inf, has out 0 and lse
+ * -inf.  out_lse [batch, queries, heads] f32 (optional).  scores, out_scores
+ * [batch, kv_heads, table_width * page_size] f32 (both or neither, may be the
+ * same buffer): out_scores = scores + the sum of w_j over the queries and the heads of
+ * a kv head; other slots are copied.  lens above max_len are taken as max_len
+ * (max_len: a bound on lens that the host knows, at most the capacity).
+ * Workspace: tallax_kv_decode_workspace_size bytes.
+ * ---------------------------------------------------------------------- */
+size_t tallax_kv_decode_workspace_size(const tallax_kv_cache* cache, int64_t queries, int64_t heads, int64_t max_len,
+                                       int with_scores);
+int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stride_batch, int64_t q_stride_query,
+                     int64_t q_stride_head, int64_t queries, int64_t heads, double scale, const int32_t* lens,
+                     const int32_t* counts, int64_t max_len, const float* scores, void* out, float* out_lse,
+                     float* out_scores, void* workspace, size_t workspace_bytes, tallax_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Eviction by accumulated attention weight: keeps new_len = min(lens[b],
+ * budget) slots of every head.  Slots whose position is below `sinks` or at
+ * least seen[b] - recent come first, then larger scores (NaN last), ties to
+ * the lowest slot.  Kept slots below new_len stay where they are; the other
+ * kept slots move, in ascending order, into the places that became free below
+ * new_len, also in ascending order.  K and V are moved in place (their sources
+ * lie at or above new_len and are not written); scores and positions [batch,
+ * kv_heads, table_width * page_size] are written to out_scores and
+ * out_positions, distinct buffers, with 0 and -1 from new_len on.  out_lens
+ * [batch] = new_len.  Slots in no page take part in the choice but are not
+ * moved.  Workspace: tallax_kv_evict_workspace_size bytes.
+ * ---------------------------------------------------------------------- */
+size_t tallax_kv_evict_workspace_size(const tallax_kv_cache* cache, int64_t budget);
+int tallax_kv_evict(const tallax_kv_cache* cache, const int32_t* lens, const float* scores, const int32_t* positions,
+                    const int32_t* seen, int64_t budget, int64_t recent, int64_t sinks, int32_t* out_lens,
+                    float* out_scores, int32_t* out_positions, void* workspace, size_t workspace_bytes,
+                    tallax_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Verification of drafted tokens.  NO COUNTERPART IN THE REFERENCE (it draws
+ * one token a row; this draws as many as the target agrees with).
+ * draft [batch, drafted] int32, target logits [batch, drafted + 1, vocab]
+ * f32/bf16 (row i is what the target says after i drafted tokens), counts
+ * [batch] int32 or null (how many of the drafts a sequence has, clamped to
+ * [0, drafted]), temperature [batch] f32, draft_probs [batch, drafted, vocab]
+ * f32/bf16 or null (null: each draft was certain, q = 1 at it), uniforms
+ * [batch, drafted] f32 in [0, 1), noise [batch, vocab] f32 > 0 (standard
+ * exponential).  With p_i = softmax(logits_i / temperature), q_i the draft's
+ * probabilities:
+ *   draft x_i is accepted while uniforms_i * q_i(x_i) < p_i(x_i);
+ *   after n accepted ones the next token is argmax_v r(v) / noise(v) (ties to
+ *   the lowest v), r = max(p_n - q_n, 0) where draft n was refused, r = p_n
+ *   where all were accepted or p_n - q_n is nowhere positive.
+ * A row with temperature < 1e-5 is greedy: p is 1 at the largest logit (lowest
+ * index), and the next token is that one.  NaN logits count as -inf; +inf
+ * logits share the whole weight.  A draft outside [0, vocab) is refused.
+ * out_tokens [batch, drafted + 1] int32: the accepted drafts, the next token,
+ * then -1; out_accepted [batch] int32 = n.  A row with no admissible logit
+ * gives the token -1.  Workspace: tallax_verify_workspace_size bytes.
+ * ---------------------------------------------------------------------- */
+size_t tallax_verify_workspace_size(int64_t batch, int64_t drafted, int64_t vocab, int logits_dtype);
+int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch, int64_t drafted,
+                  int64_t vocab, const int32_t* counts, const float* temperature, const void* draft_probs,
+                  int probs_dtype, const float* uniforms, const float* noise, int32_t* out_tokens,
+                  int32_t* out_accepted, void* workspace, size_t workspace_bytes, tallax_stream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -24,6 +24,17 @@ OK, INVALID_ARGUMENT, UNSUPPORTED, HIP_ERROR, WORKSPACE_TOO_SMALL = 0, 1, 2, 3, 
 _c_i64, _c_i32, _c_int, _c_sz, _c_p, _c_d = (
     ctypes.c_int64, ctypes.c_int32, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_double)
 
+
+class KvCache(ctypes.Structure):
+    """tallax_kv_cache of include/tallax_hip.h."""
+    _fields_ = [("k", _c_p), ("v", _c_p), ("dtype", _c_i32), ("dim", _c_i32), ("pages", _c_i64),
+                ("kv_heads", _c_i64), ("page_size", _c_i64), ("k_stride_page", _c_i64), ("k_stride_head", _c_i64),
+                ("k_stride_slot", _c_i64), ("v_stride_page", _c_i64), ("v_stride_head", _c_i64),
+                ("v_stride_slot", _c_i64), ("block_table", _c_p), ("batch", _c_i64), ("table_width", _c_i64)]
+
+
+_c_kv = ctypes.POINTER(KvCache)
+
 _SIGNATURES = {
     "tallax_last_error": ([], ctypes.c_char_p),
     "tallax_abi_version": ([], _c_int),
@@ -57,6 +68,16 @@ _SIGNATURES = {
                               _c_int, _c_d, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p], _c_int),
     "tallax_softmax_topk_cumsum": ([_c_p, _c_i64, _c_i64, _c_int, ctypes.c_float, _c_p, _c_p, _c_p, _c_p, _c_p],
                                    _c_int),
+    "tallax_kv_append": ([_c_kv, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p], _c_int),
+    "tallax_kv_decode_workspace_size": ([_c_kv, _c_i64, _c_i64, _c_i64, _c_int], _c_sz),
+    "tallax_kv_decode": ([_c_kv, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_d, _c_p, _c_p, _c_i64, _c_p, _c_p,
+                          _c_p, _c_p, _c_p, _c_sz, _c_p], _c_int),
+    "tallax_kv_evict_workspace_size": ([_c_kv, _c_i64], _c_sz),
+    "tallax_kv_evict": ([_c_kv, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p],
+                        _c_int),
+    "tallax_verify_workspace_size": ([_c_i64, _c_i64, _c_i64, _c_int], _c_sz),
+    "tallax_verify": ([_c_p, _c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_int, _c_p, _c_p, _c_p, _c_p,
+                       _c_p, _c_sz, _c_p], _c_int),
     # test hooks (include/tallax_hip_testing.h)
     "tallax_testing_expf_logf": ([_c_p, _c_p, _c_p, _c_i64, _c_p], _c_int),
     "tallax_testing_gumbel": ([ctypes.c_uint32, ctypes.c_uint32, _c_p, _c_p, _c_p, _c_i64, _c_p], _c_int),

@@ -33,6 +33,9 @@ SOURCES = [
     "binned.hip",
     "softmax_topk.hip",
     "sample_wide.hip",
+    "kv_cache.hip",
+    "kv_attention.hip",
+    "verify.hip",
     "testing.hip",
 ]
 

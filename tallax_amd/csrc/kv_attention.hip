@@ -1,0 +1,648 @@
+// Attention of the newest tokens over a paged key-value cache.
+//
+// One workgroup of four waves takes one kv head of one sequence, up to 16 * MT
+// of its query rows (row = query * group + head in the group) and one chunk of
+// the length; a wave takes every fourth tile of the chunk and keeps its own
+// running maximum, sum and output, joined in LDS at the chunk's end.  Chunks
+// are joined by a second kernel.
+//
+// Both products have the tokens of a tile as a matrix dimension and are laid
+// out so that nothing is exchanged between lanes and nothing goes through LDS:
+//   S^T = K Q^T   operand A: lane (n, g) holds 16 bytes of token n's key,
+//                 B: of row n's query; the result has row n's scores of tokens
+//                 4g .. 4g + 3 in lane (n, g)   (n = lane % 16, g = lane / 16);
+//   O^T = V^T P^T operand B: those scores as they lie; operand A: the values of
+//                 the same tokens, which lane (n, g) has loaded whole (dim / 16
+//                 of each token, so 16 lanes read a token's value in one
+//                 piece) and transposes in its own registers.  Product j of
+//                 dim / 16 then has output d = n * dim / 16 + j.
+// bfloat16 takes the 16x16x32 products on tiles of 32 tokens, float32 the
+// 16x16x4 ones on tiles of 16.
+#include <math.h>
+
+#include "tx_common.h"
+#include "tx_kv.h"
+
+namespace tx {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+constexpr int kAttnThreads = 256;
+constexpr int kAttnWaves = 4;
+
+struct AttnArgs {
+  KvView c;
+  const char* q;
+  int64_t q_batch, q_query, q_head;  // strides in bytes
+  const int32_t* lens;
+  const int32_t* counts;
+  char* out;
+  float* lse;
+  int queries, heads, kv_heads, group;  // group = heads / kv_heads
+  int rows;                             // queries * group
+  int max_len, chunk, chunks;
+  int row_groups;                       // workgroups that share a kv head's rows
+  float scale2;                         // scale * log2 e
+  float2* part_ml;                      // [batch * kv_heads][chunks][rows]: maximum (base 2), sum
+  float* part_o;                        // [batch * kv_heads][chunks][rows][dim]
+  float* raw;                           // [batch * kv_heads][rows][raw_ld]: scores (base 2), or null
+  int raw_ld;
+  const float* scores;
+  float* out_scores;
+};
+
+// What a sequence's rows see: row of query t sees slots below limit(t).
+struct Seen {
+  int len, cnt, first;  // first + t = limit of query t
+  __device__ __forceinline__ Seen(const AttnArgs& a, int b) {
+    const int l = max(a.lens[b], 0);
+    cnt = a.queries;
+    if (a.counts) cnt = min(max(a.counts[b], 0), a.queries);
+    first = l - cnt + 1;
+    len = min(l, a.max_len);
+  }
+  __device__ __forceinline__ int limit(int t) const { return t < cnt ? min(first + t, len) : 0; }
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // round to nearest even
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  bf16x2_t r;
+  r[0] = (__bf16)lo;
+  r[1] = (__bf16)hi;
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+__device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
+  return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+}
+
+template <bool F32, int DP>
+struct Tile {
+  static constexpr int kTokens = F32 ? 16 : 32;
+  static constexpr int kKeyVecs = F32 ? DP / 16 : DP / 32;     // 16-byte vectors of a key per lane and 16 tokens
+  static constexpr int kValueTokens = F32 ? 4 : 8;             // tokens whose values a lane holds
+  static constexpr int kValueWords = F32 ? DP / 16 : DP / 32;  // 32-bit words of each
+  static constexpr int kAcc = DP / 16;                         // products (and f32x4 accumulators) per 16 rows
+};
+
+template <bool F32, int DP>
+using ValueWords = uint32_t[Tile<F32, DP>::kValueWords];
+
+template <bool F32, int DP, int MT>
+struct Work {
+  using T = Tile<F32, DP>;
+  uint4 q[MT][T::kKeyVecs];
+  f32x4 acc[MT][T::kAcc];
+  float m[MT], l[MT];
+};
+
+// x of a tile's 16-token part u for 16 rows: S^T in the accumulator layout
+template <bool F32, int DP>
+__device__ __forceinline__ f32x4 scores_of(const uint4 (&k)[Tile<F32, DP>::kKeyVecs],
+                                           const uint4 (&q)[Tile<F32, DP>::kKeyVecs]) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < Tile<F32, DP>::kKeyVecs; ++i) {
+    if constexpr (F32) {
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x), __uint_as_float(q[i].x), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].y), __uint_as_float(q[i].y), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].z), __uint_as_float(q[i].z), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].w), __uint_as_float(q[i].w), s, 0, 0, 0);
+    } else {
+      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[i]),
+                                                  __builtin_bit_cast(bf16x8_t, q[i]), s, 0, 0, 0);
+    }
+  }
+  return s;
+}
+
+// O^T += V^T P^T for 16 rows.  v[j]: this lane's part of its j-th token's value.
+template <bool F32, int DP>
+__device__ __forceinline__ void add_values(const uint32_t (&v)[Tile<F32, DP>::kValueTokens][Tile<F32, DP>::kValueWords],
+                                           const float* p, f32x4 (&acc)[Tile<F32, DP>::kAcc]) {
+  if constexpr (F32) {
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j]), p[r], acc[j], 0, 0, 0);
+  } else {
+    uint4 pk;
+    pk.x = pack_bf16(p[0], p[1]);
+    pk.y = pack_bf16(p[2], p[3]);
+    pk.z = pack_bf16(p[4], p[5]);
+    pk.w = pack_bf16(p[6], p[7]);
+    const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, pk);
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) {
+      const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+      uint4 t;  // element j of the eight tokens
+      t.x = __builtin_amdgcn_perm(v[1][j / 2], v[0][j / 2], sel);
+      t.y = __builtin_amdgcn_perm(v[3][j / 2], v[2][j / 2], sel);
+      t.z = __builtin_amdgcn_perm(v[5][j / 2], v[4][j / 2], sel);
+      t.w = __builtin_amdgcn_perm(v[7][j / 2], v[6][j / 2], sel);
+      acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, t), pb, acc[j], 0, 0, 0);
+    }
+  }
+}
+
+// d of accumulator j, register r, lane group g.  bfloat16: a lane holds DP / 16
+// neighbouring elements of a value; float32: four of each 64.
+template <bool F32, int DP>
+__device__ __forceinline__ int out_dim(int j, int r, int g) {
+  return F32 ? 64 * (j / 4) + 4 * (4 * g + r) + (j & 3) : (DP / 16) * (4 * g + r) + j;
+}
+
+template <bool F32, int DP>
+__device__ __forceinline__ void load_value(ValueWords<F32, DP>& w, const char* p, int n, int dim) {
+  if constexpr (F32) {
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (64 * c + 4 * n < dim) x = *(const uint4*)(p + (64 * c + 4 * n) * 4);
+      w[4 * c] = x.x;
+      w[4 * c + 1] = x.y;
+      w[4 * c + 2] = x.z;
+      w[4 * c + 3] = x.w;
+    }
+  } else if constexpr (DP == 64) {
+    uint2 x = make_uint2(0, 0);
+    if (4 * n < dim) x = *(const uint2*)(p + 8 * n);
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int c = 0; c < DP / 128; ++c) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      const int d = (DP / 16) * n + 8 * c;
+      if (d < dim) x = *(const uint4*)(p + 2 * d);
+      w[4 * c] = x.x;
+      w[4 * c + 1] = x.y;
+      w[4 * c + 2] = x.z;
+      w[4 * c + 3] = x.w;
+    }
+  }
+}
+
+template <bool F32, int DP, int MT>
+__global__ __launch_bounds__(kAttnThreads) void kv_decode_kernel(AttnArgs a) {
+  using T = Tile<F32, DP>;
+  constexpr int ES = F32 ? 4 : 2;
+  constexpr int PARTS = T::kTokens / 16;  // 16-token parts of a tile
+  extern __shared__ float lds[];          // [kAttnWaves][16][DP + 4], then m, l of the waves
+
+  const int rg = blockIdx.x % a.row_groups;
+  const int unit = blockIdx.x / a.row_groups;  // sequence * kv_heads + kv head
+  const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
+  const int wave = threadIdx.x / kWave, lane = lane_id(), n = lane & 15, g = lane >> 4;
+  const Seen seen(a, b);
+  const int start = blockIdx.y * a.chunk;
+  if (start >= seen.len && a.chunks > 1) return;
+  const int end = min(start + a.chunk, seen.len);
+  const int row0 = rg * 16 * MT;
+
+  Work<F32, DP, MT> w;
+  int limit[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = row0 + 16 * mt + n;
+    const int t = row / a.group;
+    limit[mt] = row < a.rows ? seen.limit(t) : 0;
+    const char* qp = a.q + b * a.q_batch + t * a.q_query + (int64_t)(kvh * a.group + row - t * a.group) * a.q_head;
+#pragma unroll
+    for (int i = 0; i < T::kKeyVecs; ++i) {
+      const int d = F32 ? 16 * i + 4 * g : 32 * i + 8 * g;
+      w.q[mt][i] = make_uint4(0, 0, 0, 0);
+      if (row < a.rows && d < a.c.dim) w.q[mt][i] = *(const uint4*)(qp + d * ES);
+    }
+    w.m[mt] = -INFINITY;
+    w.l[mt] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < T::kAcc; ++j) w.acc[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const char* kbase = a.c.k + kvh * a.c.k_head;
+  const char* vbase = a.c.v + kvh * a.c.v_head;
+  const int32_t* table = a.c.table + (int64_t)b * a.c.width;
+  // below this every row of a query that counts sees every slot
+  const int open = min(seen.first, end);
+
+  for (int t0 = start + wave * T::kTokens; t0 < end; t0 += kAttnWaves * T::kTokens) {
+    const int mine = t0 + (lane & (T::kTokens - 1));
+    const int page = mine < end ? page_id(a.c, table, mine) : -1;
+    const bool plain = t0 + T::kTokens <= open && __ballot(page < 0) == 0;
+
+    uint4 key[PARTS][T::kKeyVecs];
+    uint32_t val[T::kValueTokens][T::kValueWords];
+    bool gone[PARTS][4];  // this lane's tokens 4g .. 4g + 3 of each part lie past the end or in no page
+#pragma unroll
+    for (int u = 0; u < PARTS; ++u) {
+      const int tok = t0 + 16 * u + n;
+      const int p = __builtin_amdgcn_ds_bpermute((16 * u + n) << 2, page);
+      const int off = tok - (int)page_of(a.c.div, (uint32_t)tok) * a.c.div.size;
+      const char* kp = kbase + p * a.c.k_page + off * a.c.k_slot;
+#pragma unroll
+      for (int i = 0; i < T::kKeyVecs; ++i) {
+        const int d = F32 ? 16 * i + 4 * g : 32 * i + 8 * g;
+        key[u][i] = make_uint4(0, 0, 0, 0);
+        if (p >= 0 && d < a.c.dim) key[u][i] = *(const uint4*)(kp + d * ES);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < T::kValueTokens; ++j) {
+      const int in = 16 * (j / 4) + 4 * g + (j & 3);
+      const int tok = t0 + in;
+      const int p = __builtin_amdgcn_ds_bpermute(in << 2, page);
+      const int off = tok - (int)page_of(a.c.div, (uint32_t)tok) * a.c.div.size;
+      gone[j / 4][j & 3] = p < 0;
+#pragma unroll
+      for (int i = 0; i < T::kValueWords; ++i) val[j][i] = 0;
+      if (p >= 0) load_value<F32, DP>(val[j], vbase + p * a.c.v_page + off * a.c.v_slot, n, a.c.dim);
+    }
+    // A value that is not finite would reach rows that do not see its token
+    // through 0 * inf; such a tile is added one query at a time.
+    bool strange = false;
+    if (!plain && seen.cnt > 1) {
+#pragma unroll
+      for (int j = 0; j < T::kValueTokens; ++j)
+#pragma unroll
+        for (int i = 0; i < T::kValueWords; ++i)
+          strange = strange || (F32 ? (val[j][i] & 0x7f800000u) == 0x7f800000u : bf16_pair_not_finite(val[j][i]));
+      strange = __ballot(strange) != 0;
+    }
+
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float x[4 * PARTS];
+#pragma unroll
+      for (int u = 0; u < PARTS; ++u) {
+        const f32x4 s = scores_of<F32, DP>(key[u], w.q[mt]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[4 * u + r] = s[r] * a.scale2;
+      }
+      if (!plain) {
+#pragma unroll
+        for (int u = 0; u < PARTS; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (gone[u][r] || t0 + 16 * u + 4 * g + r >= limit[mt]) x[4 * u + r] = -INFINITY;
+      }
+      if (a.raw) {
+        const int row = row0 + 16 * mt + n;
+        if (row < a.rows) {
+          float* rp = a.raw + ((int64_t)unit * a.rows + row) * a.raw_ld + t0 + 4 * g;
+#pragma unroll
+          for (int u = 0; u < PARTS; ++u)
+            *(float4*)(rp + 16 * u) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+        }
+      }
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < 4 * PARTS; ++i) top = fmaxf(top, x[i]);
+      top = fmaxf(top, lane_xor_f(top, 16));
+      top = fmaxf(top, lane_xor_f(top, 32));
+      const float m = fmaxf(w.m[mt], top);
+      const float base = m == -INFINITY ? 0.0f : m;  // nothing seen yet: every weight is exp2(-inf) = 0
+      const float shrink = __builtin_amdgcn_exp2f(w.m[mt] - base);
+      w.m[mt] = m;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4 * PARTS; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] - base);
+        sum += x[i];
+      }
+      w.l[mt] = w.l[mt] * shrink + sum;
+#pragma unroll
+      for (int j = 0; j < T::kAcc; ++j) w.acc[mt][j] *= shrink;
+      if (!strange) {
+        add_values<F32, DP>(val, x, w.acc[mt]);
+      } else {
+        const int t_of = (row0 + 16 * mt + n) / a.group;
+        for (int t = 0; t < seen.cnt; ++t) {
+          const int lim = seen.limit(t);
+          uint32_t v[T::kValueTokens][T::kValueWords];
+#pragma unroll
+          for (int j = 0; j < T::kValueTokens; ++j)
+#pragma unroll
+            for (int i = 0; i < T::kValueWords; ++i)
+              v[j][i] = t0 + 16 * (j / 4) + 4 * g + (j & 3) < lim ? val[j][i] : 0u;
+          f32x4 acc[T::kAcc];
+#pragma unroll
+          for (int j = 0; j < T::kAcc; ++j) acc[j] = w.acc[mt][j];
+          add_values<F32, DP>(v, x, acc);
+          if (t_of == t)
+#pragma unroll
+            for (int j = 0; j < T::kAcc; ++j) w.acc[mt][j] = acc[j];
+        }
+      }
+    }
+  }
+
+  // join the four waves
+  float* ml = lds + kAttnWaves * 16 * (DP + 4);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    float l = w.l[mt];
+    l += lane_xor_f(l, 16);
+    l += lane_xor_f(l, 32);
+    if (limit[mt] <= 0) {  // a row that sees nothing
+      w.m[mt] = -INFINITY;
+      l = 0.0f;
+    }
+    if (g == 0) {
+      ml[(wave * 16 + n) * 2] = w.m[mt];
+      ml[(wave * 16 + n) * 2 + 1] = l;
+    }
+    __syncthreads();
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kAttnWaves; ++i) m = fmaxf(m, ml[(i * 16 + n) * 2]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    const float mine = __builtin_amdgcn_exp2f(w.m[mt] - base);
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAttnWaves; ++i)
+      l += ml[(i * 16 + n) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(i * 16 + n) * 2] - base);
+    float* mo = lds + (wave * 16 + n) * (DP + 4);
+#pragma unroll
+    for (int j = 0; j < T::kAcc; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        mo[out_dim<F32, DP>(j, r, g)] = w.m[mt] == -INFINITY ? 0.0f : w.acc[mt][j][r] * mine;
+    if (wave == 0 && g == 0) {  // for the threads that write the rows
+      ml[kAttnWaves * 32 + 2 * n] = m;
+      ml[kAttnWaves * 32 + 2 * n + 1] = l;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (DP / 4); i += kAttnThreads) {
+      const int rn = i / (DP / 4), d = (i - rn * (DP / 4)) * 4;
+      const int row = row0 + 16 * mt + rn;
+      if (row >= a.rows || d >= a.c.dim) continue;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kAttnWaves; ++k) {
+        const float4 x = *(const float4*)(lds + (k * 16 + rn) * (DP + 4) + d);
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
+      }
+      const float rm = ml[kAttnWaves * 32 + 2 * rn], rl = ml[kAttnWaves * 32 + 2 * rn + 1];
+      if (a.chunks > 1) {
+        const int64_t at = ((int64_t)unit * a.chunks + blockIdx.y) * a.rows + row;
+        *(float4*)(a.part_o + at * a.c.dim + d) = o;
+        if (d == 0) a.part_ml[at] = make_float2(rm, rl);
+      } else {
+        const float inv = rl == 0.0f ? 0.0f : 1.0f / rl;
+        const int t = row / a.group;
+        const int64_t head = ((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group);
+        const bool none = rl == 0.0f;
+        o.x = none ? 0.f : o.x * inv, o.y = none ? 0.f : o.y * inv, o.z = none ? 0.f : o.z * inv,
+        o.w = none ? 0.f : o.w * inv;
+        if constexpr (F32)
+          *(float4*)(a.out + (head * a.c.dim + d) * 4) = o;
+        else
+          *(uint2*)(a.out + (head * a.c.dim + d) * 2) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+        if (d == 0) {
+          if (a.lse) a.lse[head] = none ? -INFINITY : (rm + __builtin_amdgcn_logf(rl)) * kLn2;
+          if (a.raw) a.part_ml[(int64_t)unit * a.rows + row] = make_float2(rm, rl);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the chunks: blocks with blockIdx.y == 0 the outputs of a sequence's kv
+// head, the others the sums of 1024 slots' weights over its rows.
+__global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32, int join_out) {
+  extern __shared__ float row_ml[];  // [rows]: base, then [rows]: 1 / sum, or lse in base 2 for the weights
+  const int unit = blockIdx.x, b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, tid = threadIdx.x;
+  const Seen seen(a, b);
+  const int nch = a.chunks > 1 ? (seen.len + a.chunk - 1) / a.chunk : 1;
+  const bool weights = (int)blockIdx.y >= join_out;
+  const float2* ml = a.part_ml + (int64_t)unit * a.chunks * a.rows;
+  for (int row = tid; row < a.rows; row += 256) {
+    float m = -INFINITY, l = 0.0f;
+    for (int c = 0; c < nch; ++c) m = fmaxf(m, ml[(int64_t)c * a.rows + row].x);
+    const float base = m == -INFINITY ? 0.0f : m;
+    for (int c = 0; c < nch; ++c) {
+      const float2 x = ml[(int64_t)c * a.rows + row];
+      l += x.y * __builtin_amdgcn_exp2f(x.x - base);
+    }
+    row_ml[2 * row] = base;
+    row_ml[2 * row + 1] = l == 0.0f ? 0.0f : 1.0f / l;
+    if (!weights && a.lse) {
+      const int t = row / a.group;
+      a.lse[((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group)] =
+          l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+  }
+  __syncthreads();
+  if (!weights) {
+    const int dv = a.c.dim / 4;
+    for (int i = tid; i < a.rows * dv; i += 256) {
+      const int row = i / dv, d = (i - row * dv) * 4;
+      const float base = row_ml[2 * row], inv = row_ml[2 * row + 1];
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < nch; ++c) {
+        const int64_t at = ((int64_t)unit * a.chunks + c) * a.rows + row;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[at].x - base);
+        const float4 x = *(const float4*)(a.part_o + at * a.c.dim + d);
+        o.x += x.x * f;
+        o.y += x.y * f;
+        o.z += x.z * f;
+        o.w += x.w * f;
+      }
+      if (inv == 0.0f) {
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+      }
+      const int t = row / a.group;
+      const int64_t head = ((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group);
+      if (f32)
+        *(float4*)(a.out + (head * a.c.dim + d) * 4) = o;
+      else
+        *(uint2*)(a.out + (head * a.c.dim + d) * 2) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+    }
+    return;
+  }
+  const int slot0 = ((int)blockIdx.y - join_out) * 1024 + tid * 4;
+  for (int k = 0; k < 4; ++k) {
+    const int slot = slot0 + k;
+    if (slot >= a.c.capacity) break;
+    float s = 0.0f;
+    if (slot < seen.len) {
+      for (int row = 0; row < a.rows; ++row) {
+        if (seen.limit(row / a.group) <= 0) continue;
+        const float x = a.raw[((int64_t)unit * a.rows + row) * a.raw_ld + slot];
+        s += __builtin_amdgcn_exp2f(x - row_ml[2 * row]) * row_ml[2 * row + 1];
+      }
+    }
+    const int64_t at = (int64_t)unit * a.c.capacity + slot;
+    a.out_scores[at] = a.scores[at] + s;
+  }
+}
+
+struct AttnPlan {
+  int mt, row_groups, chunk, chunks, max_len, rows, raw_ld;
+  size_t ml_bytes, o_bytes, raw_bytes;
+};
+
+static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int dim, int dtype, int64_t max_len,
+                           bool with_scores, AttnPlan* p) {
+  const int tiles = (int)((rows + 15) / 16), most = dtype == TALLAX_F32 ? 2 : 4;
+  p->mt = tiles <= 1 ? 1 : tiles <= 2 ? 2 : most;
+  p->row_groups = (tiles + p->mt - 1) / p->mt;
+  p->rows = (int)rows;
+  p->max_len = (int)max_len;
+  const int64_t units = batch * kv_heads * p->row_groups;
+  int64_t chunk = (max_len * units / 2048 + 127) / 128 * 128;
+  if (chunk < 256) chunk = 256;
+  p->chunk = (int)chunk;
+  p->chunks = max_len <= chunk ? 1 : (int)((max_len + chunk - 1) / chunk);
+  p->raw_ld = (int)((max_len + 31) / 32 * 32);
+  const int64_t kv = batch * kv_heads;
+  p->ml_bytes = align_up((size_t)(kv * p->chunks * rows) * sizeof(float2), 256);
+  p->o_bytes = p->chunks > 1 ? align_up((size_t)(kv * p->chunks * rows) * dim * 4, 256) : 0;
+  p->raw_bytes = with_scores ? align_up((size_t)(kv * rows) * p->raw_ld * 4, 256) : 0;
+  if (p->chunks == 1 && !with_scores) p->ml_bytes = 0;
+}
+
+template <bool F32, int DP, int MT>
+static int launch_decode_mt(const AttnArgs& a, const AttnPlan& p, int64_t units, hipStream_t s) {
+  const int bytes = (kAttnWaves * 16 * (DP + 4) + (kAttnWaves + 1) * 32) * 4;
+  if (bytes > 65536) {
+    const hipError_t e = set_dynamic_lds_limit((const void*)kv_decode_kernel<F32, DP, MT>, bytes, s);
+    if (e != hipSuccess) {
+      set_error("kv_decode: %s", hipGetErrorString(e));
+      return kHipError;
+    }
+  }
+  kv_decode_kernel<F32, DP, MT>
+      <<<dim3((unsigned)(units * p.row_groups), (unsigned)p.chunks), kAttnThreads, bytes, s>>>(a);
+  return launch_status("kv_decode");
+}
+
+template <bool F32, int DP>
+static int launch_decode(const AttnArgs& a, const AttnPlan& p, int64_t units, hipStream_t s) {
+  if (p.mt == 1) return launch_decode_mt<F32, DP, 1>(a, p, units, s);
+  if (p.mt == 2) return launch_decode_mt<F32, DP, 2>(a, p, units, s);
+  if constexpr (!F32) return launch_decode_mt<F32, DP, 4>(a, p, units, s);
+  return kInvalidArgument;
+}
+
+}  // namespace tx
+
+using namespace tx;
+
+extern "C" {
+
+size_t tallax_kv_decode_workspace_size(const tallax_kv_cache* cache, int64_t queries, int64_t heads, int64_t max_len,
+                                       int with_scores) {
+  KvView v;
+  if (make_kv_view(cache, "kv_decode", &v) != kOk || queries < 1 || heads < 1 || heads % cache->kv_heads) return 0;
+  if (max_len > v.capacity || max_len < 0) max_len = v.capacity;
+  AttnPlan p;
+  plan_attention(cache->batch, cache->kv_heads, queries * (heads / cache->kv_heads), v.dim, cache->dtype, max_len,
+                 with_scores != 0, &p);
+  return p.ml_bytes + p.o_bytes + p.raw_bytes;
+}
+
+int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stride_batch, int64_t q_stride_query,
+                     int64_t q_stride_head, int64_t queries, int64_t heads, double scale, const int32_t* lens,
+                     const int32_t* counts, int64_t max_len, const float* scores, void* out, float* out_lse,
+                     float* out_scores, void* workspace, size_t workspace_bytes, tallax_stream_t stream) {
+  AttnArgs a;
+  int st = make_kv_view(cache, "kv_decode", &a.c);
+  if (st != kOk) return st;
+  if (queries < 1 || queries > 1024 || heads < 1 || heads % cache->kv_heads) {
+    set_error("kv_decode: %lld queries (1 to 1024), %lld heads over %lld kv heads (a multiple)", (long long)queries,
+              (long long)heads, (long long)cache->kv_heads);
+    return kInvalidArgument;
+  }
+  const int64_t group = heads / cache->kv_heads, rows = queries * group;
+  if (rows > 4096) {
+    set_error("kv_decode: %lld queries x %lld heads of a kv head: at most 4096 rows", (long long)queries,
+              (long long)group);
+    return kUnsupported;
+  }
+  if (!(scale == scale) || scale - scale != 0.0) {
+    set_error("kv_decode: scale must be finite");
+    return kInvalidArgument;
+  }
+  if (cache->batch == 0) return kOk;
+  if (!q || !lens || !out || (!scores != !out_scores)) {
+    set_error("kv_decode: null pointer, or scores without out_scores");
+    return kInvalidArgument;
+  }
+  const int64_t es = cache->dtype == TALLAX_F32 ? 4 : 2;
+  if (((uintptr_t)q | (uintptr_t)out) & 15 || q_stride_batch * es % 16 || q_stride_query * es % 16 ||
+      q_stride_head * es % 16 || q_stride_batch < 0 || q_stride_query < 0 || q_stride_head < 0) {
+    set_error("kv_decode: q, its strides and out must be multiples of 16 bytes");
+    return kUnsupported;
+  }
+  if (max_len < 0 || max_len > a.c.capacity) {
+    set_error("kv_decode: max_len %lld must be in [0, %d], the slots of a table row", (long long)max_len,
+              a.c.capacity);
+    return kInvalidArgument;
+  }
+  AttnPlan p;
+  plan_attention(cache->batch, cache->kv_heads, rows, a.c.dim, cache->dtype, max_len, scores != nullptr, &p);
+  const size_t need = p.ml_bytes + p.o_bytes + p.raw_bytes;
+  if (need && (!workspace || workspace_bytes < need)) {
+    set_error("kv_decode: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    return kWorkspaceTooSmall;
+  }
+  a.q = (const char*)q;
+  a.q_batch = q_stride_batch * es;
+  a.q_query = q_stride_query * es;
+  a.q_head = q_stride_head * es;
+  a.lens = lens;
+  a.counts = counts;
+  a.out = (char*)out;
+  a.lse = out_lse;
+  a.queries = (int)queries;
+  a.heads = (int)heads;
+  a.kv_heads = (int)cache->kv_heads;
+  a.group = (int)group;
+  a.rows = p.rows;
+  a.max_len = p.max_len;
+  a.chunk = p.chunk;
+  a.chunks = p.chunks;
+  a.row_groups = p.row_groups;
+  a.scale2 = (float)(scale * 1.4426950408889634);
+  char* ws = (char*)workspace;
+  a.part_ml = (float2*)ws;
+  a.part_o = (float*)(ws + p.ml_bytes);
+  a.raw = scores ? (float*)(ws + p.ml_bytes + p.o_bytes) : nullptr;
+  a.raw_ld = p.raw_ld;
+  a.scores = scores;
+  a.out_scores = out_scores;
+  const int64_t units = cache->batch * cache->kv_heads;
+  if (units * p.row_groups > INT32_MAX || p.chunks > 65535) {
+    set_error("kv_decode: too many workgroups");
+    return kUnsupported;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  const bool f32 = cache->dtype == TALLAX_F32;
+  if (a.c.dim <= 64)
+    st = f32 ? launch_decode<true, 64>(a, p, units, s) : launch_decode<false, 64>(a, p, units, s);
+  else if (a.c.dim <= 128)
+    st = f32 ? launch_decode<true, 128>(a, p, units, s) : launch_decode<false, 128>(a, p, units, s);
+  else
+    st = f32 ? launch_decode<true, 256>(a, p, units, s) : launch_decode<false, 256>(a, p, units, s);
+  if (st != kOk) return st;
+  const int join_out = p.chunks > 1;
+  const int blocks = join_out + (scores ? (a.c.capacity + 1023) / 1024 : 0);
+  if (blocks == 0) return kOk;
+  kv_decode_join_kernel<<<dim3((unsigned)units, (unsigned)blocks), 256, (size_t)p.rows * 8, s>>>(a, f32, join_out);
+  return launch_status("kv_decode");
+}
+
+}  // extern "C"
