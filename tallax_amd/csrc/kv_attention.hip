@@ -59,11 +59,10 @@ struct AttnArgs {
 struct Seen {
   int len, cnt, first;  // first + t = limit of query t
   __device__ __forceinline__ Seen(const AttnArgs& a, int b) {
-    const int l = max(a.lens[b], 0);
+    len = min(max(a.lens[b], 0), a.max_len);
     cnt = a.queries;
     if (a.counts) cnt = min(max(a.counts[b], 0), a.queries);
-    first = l - cnt + 1;
-    len = min(l, a.max_len);
+    first = len - cnt + 1;
   }
   __device__ __forceinline__ int limit(int t) const { return t < cnt ? min(first + t, len) : 0; }
 };

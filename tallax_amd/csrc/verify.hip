@@ -312,8 +312,9 @@ __device__ __forceinline__ RacePart race_chunk(const VerifyArgs& a, int b, const
     const float p = scale.weight(logit_at<DT>(logits, v) - d.row.max) * inv_sum;
     const float q = !with_q ? 0.0f : a.probs ? (float)prob_of_draft(a, qrow, v) : v == certain ? 1.0f : 0.0f;
     const float e = noise[v];
-    // p is off by at most 2^-20 of itself (exp2 and four roundings), the quotient by 2^-22 more
-    const float slack = p * 0x1p-19f;
+    // p is off by at most 2^-17 of itself (its exponent is as low as -150 and rounded to half of 2^-16; exp2
+    // and four roundings add little) and by what lies below the normal numbers, the quotient by 2^-22 more
+    const float slack = p * 0x1p-16f + 0x1p-120f;
     hi[k] = (p - q + slack) / e * (1.0f + 0x1p-20f);
     low = fmaxf(low, (p - q - slack) / e * (1.0f - 0x1p-20f));
   }

@@ -441,3 +441,14 @@ def test_empty_batches_and_tables(gpu):
         assert kvcache.append(k, v, table, lens, n, n).tolist() == [0] * batch
         assert kvcache.evict(k, v, table, lens, scores, positions, lens, budget=3)[0].tolist() == [0] * batch
     assert float(k.float().abs().max()) == 0
+
+
+def test_decode_max_len_cuts_several_queries(gpu):
+    """A length above max_len is taken as max_len for every query of a draft, not for the last alone."""
+    q, k, v, table, lens, counts, scores = _inputs(14, "bf16", 3, 4, 8, 2, 64, 16, [300, 90, 101], [4, 2, 3])
+    cut = torch.clamp(lens, max=100)
+    want = R.attention(q, k, v, table, cut, 0.125, counts, scores)
+    out, lse, new = _decode(gpu, q, k, v, table, lens, counts, scores, max_len=100)
+    _check(out, want[0], want[3][0], "out")
+    _check(lse, want[1], want[3][1], "lse")
+    _check(new, want[2], want[3][2], "scores")

@@ -185,3 +185,26 @@ def test_refusals(gpu):
                            torch.zeros((1, 64), device=gpu), torch.ones((1, 8), device=gpu))
     empty = speculative.verify(draft[:0], logits[:0], u[:0], noise[:0])
     assert empty[0].shape == (0, 4) and empty[1].shape == (0,)
+
+
+def test_small_probabilities_race_closely(gpu):
+    """Two tokens of probability 2^-66 to 2^-148 whose noise makes them the largest, a few 1e-6 apart: a 32-bit
+    exponent is rounded by as much there, and below 2^-126 a 32-bit probability by more."""
+    rng = np.random.default_rng(9)
+    batch, vocab = 3000, 32
+    rows = np.arange(batch)
+    logits = np.full((batch, 1, vocab), -np.inf, np.float32)
+    at = np.stack([rng.permutation(vocab)[:3] for _ in range(batch)]).T
+    a = rng.uniform(-102, -46, batch)
+    logits[rows, 0, at[0]], logits[rows, 0, at[1]], logits[rows, 0, at[2]] = 0, a, a + rng.uniform(-0.7, 0.7, batch)
+    p = np.exp(logits[:, 0].astype(np.float64))
+    p /= p.sum(-1, keepdims=True)
+    noise = rng.exponential(size=(batch, vocab)).astype(np.float32) + np.float32(1e-12)
+    noise[rows, at[0]] = 2.0 ** 60
+    noise[rows, at[1]] = p[rows, at[1]] * 2.0 ** 30
+    apart = 1 + rng.uniform(1.2e-6, 6e-6, batch) * rng.choice([-1, 1], batch)
+    s = p[rows, at[1]] / noise[rows, at[1]].astype(np.float64) * apart
+    noise[rows, at[2]] = p[rows, at[2]] / s
+    none = np.zeros((batch, 0), np.int32)
+    want = _run(gpu, "f32", None, none, logits, none.astype(np.float32), noise, None, np.ones(batch, np.float32))
+    assert 1000 < (want[0][:, 0] == at[1]).sum() < 2000 and ((want[0][:, 0] == at[1]) | (want[0][:, 0] == at[2])).all()
