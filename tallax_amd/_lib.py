@@ -201,6 +201,25 @@ def require_cuda(*ts: torch.Tensor) -> None:
         raise ValueError(f"operands on different devices: { {t.device for t in ts} }")
 
 
+def _load_serving():
+    """The module behind kvcache and speculative: the same library, called without ctypes."""
+    if not (_LIB_PATH.parent / "serving_ext.so").exists():
+        raise ImportError(
+            f"tallax_amd extension not built: {_LIB_PATH.parent / 'serving_ext.so'} is missing. "
+            "Run `python -c 'import __graft_entry__ as g; g.build()'` (hipcc, gfx950).")
+    from ._build import serving_ext
+
+    def per_row(value, rows, device):
+        from .sampling import _per_row
+        return _per_row(value, rows, torch.float32, device)
+
+    serving_ext.setup(TallaxError, torch.OutOfMemoryError, workspace_arg, per_row)
+    return serving_ext
+
+
+SERVING = _load_serving()
+
+
 def select_plan(rows: int, cols: int, dtype: int, k: int = 128, sample: bool = True) -> dict:
     """Work split of the selection kernels for a [rows, cols] input (host only).
     A row is one whole-row workgroup (1024 threads, one segment), 2-4

@@ -247,6 +247,11 @@ __global__ __launch_bounds__(256) void kv_evict_move_kernel(EvictArgs a, int vec
   }
 }
 
+// No sequence can be longer than the table's capacity.
+static int64_t clamp_budget(int64_t budget, int64_t capacity) {
+  return budget > capacity ? (capacity > 0 ? capacity : 1) : budget;
+}
+
 }  // namespace tx
 
 using namespace tx;
@@ -292,7 +297,8 @@ int tallax_kv_append(const tallax_kv_cache* cache, const int32_t* lens, const in
 }
 
 size_t tallax_kv_evict_workspace_size(const tallax_kv_cache* cache, int64_t budget) {
-  if (!cache || budget < 0 || cache->batch < 0 || cache->kv_heads < 0) return 0;
+  if (!cache || budget < 0 || cache->batch < 0 || cache->kv_heads < 0 || cache->table_width < 0) return 0;
+  budget = clamp_budget(budget, cache->table_width * cache->page_size);
   return (size_t)(cache->batch * cache->kv_heads) * (1 + 2 * (size_t)budget) * 4;
 }
 
@@ -314,7 +320,7 @@ int tallax_kv_evict(const tallax_kv_cache* cache, const int32_t* lens, const flo
     set_error("kv_evict: null pointer, or an output that is its input");
     return kInvalidArgument;
   }
-  if (budget > a.c.capacity) budget = a.c.capacity > 0 ? a.c.capacity : 1;  // nothing can be longer
+  budget = clamp_budget(budget, a.c.capacity);
   const size_t bytes = tallax_kv_evict_workspace_size(cache, budget);
   if (!workspace || workspace_bytes < bytes) {
     set_error("kv_evict: workspace of %zu bytes, %zu needed", workspace_bytes, bytes);

@@ -12,7 +12,6 @@ from typing import Any
 import torch
 
 from . import _lib
-from .sampling import _per_row
 
 
 def verify(draft_tokens: torch.Tensor, target_logits: torch.Tensor, uniforms: torch.Tensor, noise: torch.Tensor, *,
@@ -38,46 +37,7 @@ def verify(draft_tokens: torch.Tensor, target_logits: torch.Tensor, uniforms: to
     Returns (tokens [batch, drafted + 1] int32: the accepted drafts, the next
     token, then -1; accepted [batch] int32).
     """
-    _lib.require_cuda(target_logits, draft_tokens, uniforms, noise)
-    if target_logits.ndim != 3 or target_logits.shape[1] < 1 or target_logits.shape[2] < 1:
-        raise ValueError(f"target_logits must be [batch, drafted + 1, vocab], got {tuple(target_logits.shape)}")
-    batch, rows, vocab = target_logits.shape
-    drafted = rows - 1
-    for name, t, shape, dtype in (("draft_tokens", draft_tokens, (batch, drafted), torch.int32),
-                                  ("uniforms", uniforms, (batch, drafted), torch.float32),
-                                  ("noise", noise, (batch, vocab), torch.float32)):
-        if t.shape != shape or t.dtype is not dtype:
-            raise ValueError(f"{name} must be a {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    dt = _lib.dtype_code(target_logits)
-    if dt == _lib.I32:
-        raise NotImplementedError("verify needs float logits")
-    qdt = _lib.F32
-    if draft_probs is not None:
-        _lib.require_cuda(target_logits, draft_probs)
-        if draft_probs.shape != (batch, drafted, vocab):
-            raise ValueError(f"draft_probs must be of shape {(batch, drafted, vocab)}, got {tuple(draft_probs.shape)}")
-        qdt = _lib.dtype_code(draft_probs)
-        if qdt == _lib.I32:
-            raise NotImplementedError("verify needs float draft probabilities")
-        draft_probs = draft_probs.contiguous()
-    dev = target_logits.device
-    if counts is not None:
-        _lib.require_cuda(target_logits, counts)
-        if counts.shape != (batch,) or counts.dtype is not torch.int32:
-            raise ValueError(f"counts must be an int32 tensor of shape ({batch},)")
-        counts = counts.contiguous()
-    temp = _per_row(temperature, batch, torch.float32, dev)
-    logits, draft = target_logits.contiguous(), draft_tokens.contiguous()
-    uniforms, noise = uniforms.contiguous(), noise.contiguous()
-    tokens = torch.empty((batch, rows), dtype=torch.int32, device=dev)
-    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
-    need = _lib.LIB.tallax_verify_workspace_size(batch, drafted, vocab, dt)
-    ws = _lib.workspace_arg(workspace, dev, max(need, 1))
-    _lib.check(_lib.LIB.tallax_verify(
-        draft.data_ptr(), logits.data_ptr(), dt, batch, drafted, vocab, _lib.ptr(counts), temp.data_ptr(),
-        _lib.ptr(draft_probs), qdt, uniforms.data_ptr(), noise.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
-        ws.data_ptr(), ws.numel(), _lib.stream_of(logits)), "speculative.verify")
-    return tokens, accepted
+    return _lib.SERVING.verify(draft_tokens, target_logits, uniforms, noise, draft_probs, temperature, counts, workspace)
 
 
 __all__ = ["verify"]
