@@ -53,6 +53,7 @@ struct AttnArgs {
   int raw_ld;
   const float* scores;
   float* out_scores;
+  int vector_scores;                    // their rows are whole 16-byte vectors
 };
 
 // What a sequence's rows see: row of query t sees slots below limit(t).
@@ -416,39 +417,45 @@ __global__ __launch_bounds__(kAttnThreads) void kv_decode_kernel(AttnArgs a) {
   }
 }
 
-// Joins the chunks: blocks with blockIdx.y == 0 the outputs of a sequence's kv
-// head, the others the sums of 1024 slots' weights over its rows.
-__global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32, int join_out) {
-  extern __shared__ float row_ml[];  // [rows]: base, then [rows]: 1 / sum, or lse in base 2 for the weights
+// Base and 1 / sum of a row over its chunks, by one wave; the same in all lanes.
+__device__ __forceinline__ float2 join_row(const float2* ml, int nch, int rows, int row) {
+  float m = -INFINITY, l = 0.0f;
+  for (int c = lane_id(); c < nch; c += kWave) {
+    const float2 x = ml[(int64_t)c * rows + row];
+    const float t = fmaxf(m, x.x), base = t == -INFINITY ? 0.0f : t;
+    l = l * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+    m = t;
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const float om = lane_xor_f(m, d), ol = lane_xor_f(l, d);
+    const float t = fmaxf(m, om), base = t == -INFINITY ? 0.0f : t;
+    l = l * __builtin_amdgcn_exp2f(m - base) + ol * __builtin_amdgcn_exp2f(om - base);
+    m = t;
+  }
+  return make_float2(m, l);
+}
+
+// Joins the chunks.  The first `rows` workgroups of a sequence's kv head (where
+// there is more than one chunk) take an output row each, the chunks shared out
+// over groups of lanes; the others sum 1024 slots' weights over the rows.
+__global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32, int out_blocks) {
+  extern __shared__ float lds[];  // an output row: 256 x 4 sums; weights: base and 1 / sum of each row
   const int unit = blockIdx.x, b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, tid = threadIdx.x;
   const Seen seen(a, b);
   const int nch = a.chunks > 1 ? (seen.len + a.chunk - 1) / a.chunk : 1;
-  const bool weights = (int)blockIdx.y >= join_out;
   const float2* ml = a.part_ml + (int64_t)unit * a.chunks * a.rows;
-  for (int row = tid; row < a.rows; row += 256) {
-    float m = -INFINITY, l = 0.0f;
-    for (int c = 0; c < nch; ++c) m = fmaxf(m, ml[(int64_t)c * a.rows + row].x);
-    const float base = m == -INFINITY ? 0.0f : m;
-    for (int c = 0; c < nch; ++c) {
-      const float2 x = ml[(int64_t)c * a.rows + row];
-      l += x.y * __builtin_amdgcn_exp2f(x.x - base);
-    }
-    row_ml[2 * row] = base;
-    row_ml[2 * row + 1] = l == 0.0f ? 0.0f : 1.0f / l;
-    if (!weights && a.lse) {
-      const int t = row / a.group;
-      a.lse[((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group)] =
-          l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
-    }
-  }
-  __syncthreads();
-  if (!weights) {
-    const int dv = a.c.dim / 4;
-    for (int i = tid; i < a.rows * dv; i += 256) {
-      const int row = i / dv, d = (i - row * dv) * 4;
-      const float base = row_ml[2 * row], inv = row_ml[2 * row + 1];
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = 0; c < nch; ++c) {
+  if ((int)blockIdx.y < out_blocks) {
+    const int row = blockIdx.y, t = row / a.group;
+    const int64_t head = ((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group);
+    const float2 j = join_row(ml, nch, a.rows, row);
+    const float base = j.x == -INFINITY ? 0.0f : j.x;
+    const int width = a.c.dim <= 64 ? 16 : a.c.dim <= 128 ? 32 : 64;  // lanes that hold a row
+    const int d = (tid & (width - 1)) * 4, groups = 256 / width;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d < a.c.dim) {
+#pragma unroll 4
+      for (int c = tid / width; c < nch; c += groups) {
         const int64_t at = ((int64_t)unit * a.chunks + c) * a.rows + row;
         const float f = __builtin_amdgcn_exp2f(a.part_ml[at].x - base);
         const float4 x = *(const float4*)(a.part_o + at * a.c.dim + d);
@@ -457,34 +464,69 @@ __global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32
         o.z += x.z * f;
         o.w += x.w * f;
       }
-      if (inv == 0.0f) {
-        o = make_float4(0.f, 0.f, 0.f, 0.f);
-      } else {
-        o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    }
+    float4* sums = (float4*)lds;
+    sums[tid] = o;
+    __syncthreads();
+    if (tid < width && d < a.c.dim) {
+      for (int k = 1; k < groups; ++k) {
+        const float4 x = sums[k * width + tid];
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
       }
-      const int t = row / a.group;
-      const int64_t head = ((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group);
+      const float inv = j.y == 0.0f ? 0.0f : 1.0f / j.y;
+      const bool none = j.y == 0.0f;
+      o.x = none ? 0.f : o.x * inv, o.y = none ? 0.f : o.y * inv, o.z = none ? 0.f : o.z * inv,
+      o.w = none ? 0.f : o.w * inv;
       if (f32)
         *(float4*)(a.out + (head * a.c.dim + d) * 4) = o;
       else
         *(uint2*)(a.out + (head * a.c.dim + d) * 2) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+      if (tid == 0 && a.lse) a.lse[head] = none ? -INFINITY : (j.x + __builtin_amdgcn_logf(j.y)) * kLn2;
     }
     return;
   }
-  const int slot0 = ((int)blockIdx.y - join_out) * 1024 + tid * 4;
-  for (int k = 0; k < 4; ++k) {
-    const int slot = slot0 + k;
-    if (slot >= a.c.capacity) break;
-    float s = 0.0f;
-    if (slot < seen.len) {
-      for (int row = 0; row < a.rows; ++row) {
-        if (seen.limit(row / a.group) <= 0) continue;
-        const float x = a.raw[((int64_t)unit * a.rows + row) * a.raw_ld + slot];
-        s += __builtin_amdgcn_exp2f(x - row_ml[2 * row]) * row_ml[2 * row + 1];
+  const int slot0 = ((int)blockIdx.y - out_blocks) * 1024 + tid * 4;
+  const bool some = slot0 - tid * 4 < seen.len;  // else this workgroup's slots are copied
+  if (some) {
+    for (int row = tid / kWave; row < a.rows; row += 4) {
+      float2 j = join_row(ml, nch, a.rows, row);
+      if (lane_id() == 0) {
+        lds[2 * row] = j.x == -INFINITY ? 0.0f : j.x;
+        lds[2 * row + 1] = j.y == 0.0f || seen.limit(row / a.group) <= 0 ? -1.0f : 1.0f / j.y;
       }
     }
-    const int64_t at = (int64_t)unit * a.c.capacity + slot;
-    a.out_scores[at] = a.scores[at] + s;
+    __syncthreads();
+  }
+  if (slot0 >= a.c.capacity) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (some && slot0 < seen.len) {  // raw rows are whole tiles: what lies past len in one is dropped below
+    const float* raw = a.raw + (int64_t)unit * a.rows * a.raw_ld + slot0;
+#pragma unroll 4
+    for (int row = 0; row < a.rows; ++row) {
+      const float inv = lds[2 * row + 1], base = lds[2 * row];
+      const float4 x = *(const float4*)(raw + (int64_t)row * a.raw_ld);
+      if (inv == -1.0f) continue;  // a row that sees nothing
+      s.x += __builtin_amdgcn_exp2f(x.x - base) * inv;
+      s.y += __builtin_amdgcn_exp2f(x.y - base) * inv;
+      s.z += __builtin_amdgcn_exp2f(x.z - base) * inv;
+      s.w += __builtin_amdgcn_exp2f(x.w - base) * inv;
+    }
+  }
+  const int64_t at = (int64_t)unit * a.c.capacity + slot0;
+  if (a.vector_scores) {
+    float4 o = *(const float4*)(a.scores + at);
+    if (slot0 < seen.len) o.x += s.x;
+    if (slot0 + 1 < seen.len) o.y += s.y;
+    if (slot0 + 2 < seen.len) o.z += s.z;
+    if (slot0 + 3 < seen.len) o.w += s.w;
+    *(float4*)(a.out_scores + at) = o;
+  } else {
+    const float ss[4] = {s.x, s.y, s.z, s.w};
+    for (int k = 0; k < 4 && slot0 + k < a.c.capacity; ++k)
+      a.out_scores[at + k] = a.scores[at + k] + (slot0 + k < seen.len ? ss[k] : 0.0f);
   }
 }
 
@@ -623,6 +665,7 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
   a.raw_ld = p.raw_ld;
   a.scores = scores;
   a.out_scores = out_scores;
+  a.vector_scores = scores && a.c.capacity % 4 == 0 && !(((uintptr_t)scores | (uintptr_t)out_scores) & 15);
   const int64_t units = cache->batch * cache->kv_heads;
   if (units * p.row_groups > INT32_MAX || p.chunks > 65535) {
     set_error("kv_decode: too many workgroups");
@@ -637,10 +680,11 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
   else
     st = f32 ? launch_decode<true, 256>(a, p, units, s) : launch_decode<false, 256>(a, p, units, s);
   if (st != kOk) return st;
-  const int join_out = p.chunks > 1;
-  const int blocks = join_out + (scores ? (a.c.capacity + 1023) / 1024 : 0);
+  const int out_blocks = p.chunks > 1 ? p.rows : 0;
+  const int blocks = out_blocks + (scores ? (a.c.capacity + 1023) / 1024 : 0);
   if (blocks == 0) return kOk;
-  kv_decode_join_kernel<<<dim3((unsigned)units, (unsigned)blocks), 256, (size_t)p.rows * 8, s>>>(a, f32, join_out);
+  const size_t lds = (size_t)p.rows * 8 > 4096 ? (size_t)p.rows * 8 : 4096;
+  kv_decode_join_kernel<<<dim3((unsigned)units, (unsigned)blocks), 256, lds, s>>>(a, f32, out_blocks);
   return launch_status("kv_decode");
 }
 
