@@ -46,6 +46,8 @@ struct AttnArgs {
   int rows;                             // queries * group
   int max_len, chunk, chunks;
   int row_groups;                       // workgroups that share a kv head's rows
+  int shift;                            // offsets in the pools are in units of 2^shift bytes
+  uint32_t k_page, k_slot, v_page, v_slot;
   float scale2;                         // scale * log2 e
   float2* part_ml;                      // [batch * kv_heads][chunks][rows]: maximum (base 2), sum
   float* part_o;                        // [batch * kv_heads][chunks][rows][dim]
@@ -83,60 +85,75 @@ __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
 template <bool F32, int DP>
 struct Tile {
   static constexpr int kTokens = F32 ? 16 : 32;
+  static constexpr int kParts = kTokens / 16;                  // 16-token parts
   static constexpr int kKeyVecs = F32 ? DP / 16 : DP / 32;     // 16-byte vectors of a key per lane and 16 tokens
   static constexpr int kValueTokens = F32 ? 4 : 8;             // tokens whose values a lane holds
   static constexpr int kValueWords = F32 ? DP / 16 : DP / 32;  // 32-bit words of each
   static constexpr int kAcc = DP / 16;                         // products (and f32x4 accumulators) per 16 rows
 };
 
+// A tile's keys (16 tokens, 16-byte vectors) and values (tokens, words) in a lane's registers.
 template <bool F32, int DP>
-using ValueWords = uint32_t[Tile<F32, DP>::kValueWords];
+using Key = uint4[Tile<F32, DP>::kKeyVecs];
+template <bool F32, int DP>
+using Value = uint32_t[Tile<F32, DP>::kValueWords];
+template <bool F32, int DP>
+using Keys = uint4[Tile<F32, DP>::kParts][Tile<F32, DP>::kKeyVecs];
+template <bool F32, int DP>
+using Values = uint32_t[Tile<F32, DP>::kValueTokens][Tile<F32, DP>::kValueWords];
 
-template <bool F32, int DP, int MT>
-struct Work {
+// x of 16 tokens for 16 rows: S^T in the accumulator layout.  q: this lane's
+// vectors of the rows' queries in LDS, one every 64 lanes.
+template <bool F32, int DP>
+__device__ __forceinline__ void scores_of(const Keys<F32, DP>& key, const uint4* q, int dim, f32x4 (&s)[Tile<F32, DP>::kParts]) {
   using T = Tile<F32, DP>;
-  uint4 q[MT][T::kKeyVecs];
-  f32x4 acc[MT][T::kAcc];
-  float m[MT], l[MT];
-};
-
-// x of a tile's 16-token part u for 16 rows: S^T in the accumulator layout
-template <bool F32, int DP>
-__device__ __forceinline__ f32x4 scores_of(const uint4 (&k)[Tile<F32, DP>::kKeyVecs],
-                                           const uint4 (&q)[Tile<F32, DP>::kKeyVecs]) {
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < Tile<F32, DP>::kKeyVecs; ++i) {
-    if constexpr (F32) {
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x), __uint_as_float(q[i].x), s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].y), __uint_as_float(q[i].y), s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].z), __uint_as_float(q[i].z), s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].w), __uint_as_float(q[i].w), s, 0, 0, 0);
-    } else {
-      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[i]),
-                                                  __builtin_bit_cast(bf16x8_t, q[i]), s, 0, 0, 0);
+  for (int u = 0; u < T::kParts; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < T::kKeyVecs; ++i) {
+    if (F32 && 16 * i >= dim) break;
+    const uint4 qi = q[i * kWave];
+#pragma unroll
+    for (int u = 0; u < T::kParts; ++u) {
+      const uint4 k = key[u][i];
+      if constexpr (F32) {
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.x), __uint_as_float(qi.x), s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.y), __uint_as_float(qi.y), s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.z), __uint_as_float(qi.z), s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.w), __uint_as_float(qi.w), s[u], 0, 0, 0);
+      } else {
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, qi),
+                                                       s[u], 0, 0, 0);
+      }
     }
   }
-  return s;
 }
 
-// O^T += V^T P^T for 16 rows.  v[j]: this lane's part of its j-th token's value.
-template <bool F32, int DP>
-__device__ __forceinline__ void add_values(const uint32_t (&v)[Tile<F32, DP>::kValueTokens][Tile<F32, DP>::kValueWords],
-                                           const float* p, f32x4 (&acc)[Tile<F32, DP>::kAcc]) {
+// O^T += V^T P^T for 16 * MT rows
+template <bool F32, int DP, int MT>
+__device__ __forceinline__ void add_values(const Values<F32, DP>& v, const float (&p)[MT][Tile<F32, DP>::kTokens / 4],
+                                           int dim, f32x4 (&acc)[MT][Tile<F32, DP>::kAcc]) {
   if constexpr (F32) {
 #pragma unroll
-    for (int j = 0; j < DP / 16; ++j)
+    for (int j = 0; j < DP / 16; ++j) {
+      if (32 * (j / 2) >= dim) break;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j]), p[r], acc[j], 0, 0, 0);
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j]), p[mt][r], acc[mt][j], 0, 0, 0);
+    }
   } else {
-    uint4 pk;
-    pk.x = pack_bf16(p[0], p[1]);
-    pk.y = pack_bf16(p[2], p[3]);
-    pk.z = pack_bf16(p[4], p[5]);
-    pk.w = pack_bf16(p[6], p[7]);
-    const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, pk);
+    bf16x8_t pb[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      uint4 pk;
+      pk.x = pack_bf16(p[mt][0], p[mt][1]);
+      pk.y = pack_bf16(p[mt][2], p[mt][3]);
+      pk.z = pack_bf16(p[mt][4], p[mt][5]);
+      pk.w = pack_bf16(p[mt][6], p[mt][7]);
+      pb[mt] = __builtin_bit_cast(bf16x8_t, pk);
+    }
 #pragma unroll
     for (int j = 0; j < DP / 16; ++j) {
       const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
@@ -145,55 +162,94 @@ __device__ __forceinline__ void add_values(const uint32_t (&v)[Tile<F32, DP>::kV
       t.y = __builtin_amdgcn_perm(v[3][j / 2], v[2][j / 2], sel);
       t.z = __builtin_amdgcn_perm(v[5][j / 2], v[4][j / 2], sel);
       t.w = __builtin_amdgcn_perm(v[7][j / 2], v[6][j / 2], sel);
-      acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, t), pb, acc[j], 0, 0, 0);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        acc[mt][j] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, t), pb[mt], acc[mt][j], 0, 0, 0);
     }
   }
 }
 
 // d of accumulator j, register r, lane group g.  bfloat16: a lane holds DP / 16
-// neighbouring elements of a value; float32: four of each 64.
+// neighbouring elements of a value; float32: two of each 32.
 template <bool F32, int DP>
 __device__ __forceinline__ int out_dim(int j, int r, int g) {
-  return F32 ? 64 * (j / 4) + 4 * (4 * g + r) + (j & 3) : (DP / 16) * (4 * g + r) + j;
+  return F32 ? 32 * (j / 2) + 2 * (4 * g + r) + (j & 1) : (DP / 16) * (4 * g + r) + j;
+}
+
+__device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
+  return (uint32_t)__builtin_amdgcn_ds_bpermute(lane << 2, (int)x);
 }
 
 template <bool F32, int DP>
-__device__ __forceinline__ void load_value(ValueWords<F32, DP>& w, const char* p, int n, int dim) {
-  if constexpr (F32) {
+__device__ __forceinline__ void load_key(Key<F32, DP>& k, const char* p, int g, int dim) {
 #pragma unroll
-    for (int c = 0; c < DP / 64; ++c) {
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (64 * c + 4 * n < dim) x = *(const uint4*)(p + (64 * c + 4 * n) * 4);
-      w[4 * c] = x.x;
-      w[4 * c + 1] = x.y;
-      w[4 * c + 2] = x.z;
-      w[4 * c + 3] = x.w;
+  for (int i = 0; i < Tile<F32, DP>::kKeyVecs; ++i) {
+    const int d = F32 ? 16 * i + 4 * g : 32 * i + 8 * g;
+    if (d < dim) k[i] = *(const uint4*)(p + d * (F32 ? 4 : 2));
+  }
+}
+
+template <bool F32, int DP>
+__device__ __forceinline__ void load_value(Value<F32, DP>& w, const char* p, int n, int dim) {
+  if constexpr (F32 || DP == 64) {
+    constexpr int E = F32 ? 2 : 4;  // elements of 8 bytes
+#pragma unroll
+    for (int c = 0; c < Tile<F32, DP>::kValueWords / 2; ++c) {
+      const int d = 16 * E * c + E * n;
+      if (d < dim) {
+        const uint2 x = *(const uint2*)(p + d * (8 / E));
+        w[2 * c] = x.x;
+        w[2 * c + 1] = x.y;
+      }
     }
-  } else if constexpr (DP == 64) {
-    uint2 x = make_uint2(0, 0);
-    if (4 * n < dim) x = *(const uint2*)(p + 8 * n);
-    w[0] = x.x;
-    w[1] = x.y;
   } else {
 #pragma unroll
     for (int c = 0; c < DP / 128; ++c) {
-      uint4 x = make_uint4(0, 0, 0, 0);
       const int d = (DP / 16) * n + 8 * c;
-      if (d < dim) x = *(const uint4*)(p + 2 * d);
-      w[4 * c] = x.x;
-      w[4 * c + 1] = x.y;
-      w[4 * c + 2] = x.z;
-      w[4 * c + 3] = x.w;
+      if (d < dim) {
+        const uint4 x = *(const uint4*)(p + 2 * d);
+        w[4 * c] = x.x;
+        w[4 * c + 1] = x.y;
+        w[4 * c + 2] = x.z;
+        w[4 * c + 3] = x.w;
+      }
     }
   }
 }
 
+// Adds weight times value where the value is not finite, for tokens from..to - 1
+// of the tile at t0, to those of 16 rows that see the token.
+template <bool F32>
+__device__ __forceinline__ void add_strange(const AttnArgs& a, const Seen& seen, const char* vbase, uint32_t v_at,
+                                            uint64_t gone, int t0, int from, int to, int row0, float* outs, int ld,
+                                            const float* weights) {
+#pragma unroll 1
+  for (int in = from; in < to; ++in) {
+    const char* p = vbase + ((uint64_t)from_lane(v_at, in) << a.shift);
+    if ((gone >> in) & 1) continue;
+#pragma unroll 1
+    for (int d = lane_id(); d < a.c.dim; d += kWave) {
+      const float v = F32 ? ((const float*)p)[d] : __uint_as_float((uint32_t)((const uint16_t*)p)[d] << 16);
+      if ((__float_as_uint(v) & 0x7f800000u) != 0x7f800000u) continue;
+#pragma unroll 1
+      for (int r = 0; r < 16 && row0 + r < a.rows; ++r)
+        if (t0 + in < seen.limit((row0 + r) / a.group)) outs[r * ld + d] += weights[in * 16 + r] * v;
+    }
+  }
+}
+
+// Waves of a SIMD that the registers of an instance are held to.
 template <bool F32, int DP, int MT>
-__global__ __launch_bounds__(kAttnThreads) void kv_decode_kernel(AttnArgs a) {
+constexpr int kWavesHeld = DP <= 128 && MT <= 2 ? (F32 && DP == 128 && MT == 1 ? 3 : 2) : 1;
+
+template <bool F32, int DP, int MT>
+__global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_decode_kernel(AttnArgs a) {
   using T = Tile<F32, DP>;
   constexpr int ES = F32 ? 4 : 2;
-  constexpr int PARTS = T::kTokens / 16;  // 16-token parts of a tile
-  extern __shared__ float lds[];          // [kAttnWaves][16][DP + 4], then m, l of the waves
+  constexpr int STEP = kAttnWaves * T::kTokens;
+  extern __shared__ float lds[];  // [kAttnWaves][16][DP + 4], m and l of the waves, the queries, weights
+  uint4* queries = (uint4*)(lds + kAttnWaves * 16 * (DP + 4) + (kAttnWaves + 1) * 32);  // [MT][kKeyVecs][64]
 
   const int rg = blockIdx.x % a.row_groups;
   const int unit = blockIdx.x / a.row_groups;  // sequence * kv_heads + kv head
@@ -205,156 +261,187 @@ __global__ __launch_bounds__(kAttnThreads) void kv_decode_kernel(AttnArgs a) {
   const int end = min(start + a.chunk, seen.len);
   const int row0 = rg * 16 * MT;
 
-  Work<F32, DP, MT> w;
+  const char* kbase = a.c.k + kvh * a.c.k_head;
+  const char* vbase = a.c.v + kvh * a.c.v_head;
+  const int32_t* table = a.c.table + (int64_t)b * a.c.width;
+  const int mine = lane & (T::kTokens - 1);
+  auto page_at = [&](int t0) { return t0 + mine < end ? page_id(a.c, table, t0 + mine) : -1; };
+  int t0 = start + wave * T::kTokens;
+  int next_page = page_at(t0);
+
+  for (int i = threadIdx.x; i < MT * T::kKeyVecs * kWave; i += kAttnThreads) {
+    const int l = i % kWave, v = i / kWave % T::kKeyVecs, mt = i / (kWave * T::kKeyVecs);
+    const int row = row0 + 16 * mt + (l & 15), t = row / a.group;
+    const int d = F32 ? 16 * v + 4 * (l >> 4) : 32 * v + 8 * (l >> 4);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (row < a.rows && d < a.c.dim)
+      x = *(const uint4*)(a.q + b * a.q_batch + t * a.q_query +
+                          (int64_t)(kvh * a.group + row - t * a.group) * a.q_head + d * ES);
+    queries[i] = x;
+  }
+  f32x4 acc[MT][T::kAcc];
+  float wm[MT], wl[MT];
   int limit[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int row = row0 + 16 * mt + n;
-    const int t = row / a.group;
-    limit[mt] = row < a.rows ? seen.limit(t) : 0;
-    const char* qp = a.q + b * a.q_batch + t * a.q_query + (int64_t)(kvh * a.group + row - t * a.group) * a.q_head;
+    limit[mt] = row < a.rows ? seen.limit(row / a.group) : 0;
+    wm[mt] = -INFINITY;
+    wl[mt] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < T::kKeyVecs; ++i) {
-      const int d = F32 ? 16 * i + 4 * g : 32 * i + 8 * g;
-      w.q[mt][i] = make_uint4(0, 0, 0, 0);
-      if (row < a.rows && d < a.c.dim) w.q[mt][i] = *(const uint4*)(qp + d * ES);
-    }
-    w.m[mt] = -INFINITY;
-    w.l[mt] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < T::kAcc; ++j) w.acc[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < T::kAcc; ++j) acc[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-
-  const char* kbase = a.c.k + kvh * a.c.k_head;
-  const char* vbase = a.c.v + kvh * a.c.v_head;
-  const int32_t* table = a.c.table + (int64_t)b * a.c.width;
   // below this every row of a query that counts sees every slot
   const int open = min(seen.first, end);
+  __syncthreads();
 
-  for (int t0 = start + wave * T::kTokens; t0 < end; t0 += kAttnWaves * T::kTokens) {
-    const int mine = t0 + (lane & (T::kTokens - 1));
-    const int page = mine < end ? page_id(a.c, table, mine) : -1;
-    const bool plain = t0 + T::kTokens <= open && __ballot(page < 0) == 0;
-
-    uint4 key[PARTS][T::kKeyVecs];
-    uint32_t val[T::kValueTokens][T::kValueWords];
-    bool gone[PARTS][4];  // this lane's tokens 4g .. 4g + 3 of each part lie past the end or in no page
+  for (; t0 < end; t0 += STEP) {
+    // each lane works out the place of one token and hands it to those that load from it
+    const int page = next_page;
+    const int off = t0 + mine - (int)page_of(a.c.div, (uint32_t)(t0 + mine)) * a.c.div.size;
+    const uint32_t k_at = (uint32_t)page * a.k_page + (uint32_t)off * a.k_slot;
+    const uint32_t v_at = (uint32_t)page * a.v_page + (uint32_t)off * a.v_slot;
+    const uint64_t gone = __ballot(page < 0);  // bit i: token i of the tile is past the end or in no page
+    const bool plain = t0 + T::kTokens <= open && gone == 0;
+    Keys<F32, DP> key;
+    Values<F32, DP> val;
+    if (gone != 0 || DP != a.c.dim) {  // what is not loaded is 0
 #pragma unroll
-    for (int u = 0; u < PARTS; ++u) {
-      const int tok = t0 + 16 * u + n;
-      const int p = __builtin_amdgcn_ds_bpermute((16 * u + n) << 2, page);
-      const int off = tok - (int)page_of(a.c.div, (uint32_t)tok) * a.c.div.size;
-      const char* kp = kbase + p * a.c.k_page + off * a.c.k_slot;
+      for (int u = 0; u < T::kParts; ++u)
 #pragma unroll
-      for (int i = 0; i < T::kKeyVecs; ++i) {
-        const int d = F32 ? 16 * i + 4 * g : 32 * i + 8 * g;
-        key[u][i] = make_uint4(0, 0, 0, 0);
-        if (p >= 0 && d < a.c.dim) key[u][i] = *(const uint4*)(kp + d * ES);
-      }
+        for (int i = 0; i < T::kKeyVecs; ++i) key[u][i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < T::kValueTokens; ++j)
+#pragma unroll
+        for (int i = 0; i < T::kValueWords; ++i) val[j][i] = 0;
+    }
+#pragma unroll
+    for (int u = 0; u < T::kParts; ++u) {
+      const int in = 16 * u + n;
+      const char* p = kbase + ((uint64_t)from_lane(k_at, in) << a.shift);
+      if (!((gone >> in) & 1)) load_key<F32, DP>(key[u], p, g, a.c.dim);
     }
 #pragma unroll
     for (int j = 0; j < T::kValueTokens; ++j) {
       const int in = 16 * (j / 4) + 4 * g + (j & 3);
-      const int tok = t0 + in;
-      const int p = __builtin_amdgcn_ds_bpermute(in << 2, page);
-      const int off = tok - (int)page_of(a.c.div, (uint32_t)tok) * a.c.div.size;
-      gone[j / 4][j & 3] = p < 0;
-#pragma unroll
-      for (int i = 0; i < T::kValueWords; ++i) val[j][i] = 0;
-      if (p >= 0) load_value<F32, DP>(val[j], vbase + p * a.c.v_page + off * a.c.v_slot, n, a.c.dim);
+      const char* p = vbase + ((uint64_t)from_lane(v_at, in) << a.shift);
+      if (!((gone >> in) & 1)) load_value<F32, DP>(val[j], p, n, a.c.dim);
     }
-    // A value that is not finite would reach rows that do not see its token
-    // through 0 * inf; such a tile is added one query at a time.
-    bool strange = false;
-    if (!plain && seen.cnt > 1) {
-#pragma unroll
-      for (int j = 0; j < T::kValueTokens; ++j)
-#pragma unroll
-        for (int i = 0; i < T::kValueWords; ++i)
-          strange = strange || (F32 ? (val[j][i] & 0x7f800000u) == 0x7f800000u : bf16_pair_not_finite(val[j][i]));
-      strange = __ballot(strange) != 0;
-    }
+    next_page = page_at(t0 + STEP);
 
+    float x[MT][4 * T::kParts];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float x[4 * PARTS];
+      f32x4 s[T::kParts];
+      scores_of<F32, DP>(key, queries + mt * T::kKeyVecs * kWave + lane, a.c.dim, s);
 #pragma unroll
-      for (int u = 0; u < PARTS; ++u) {
-        const f32x4 s = scores_of<F32, DP>(key[u], w.q[mt]);
+      for (int u = 0; u < T::kParts; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[4 * u + r] = s[r] * a.scale2;
-      }
+        for (int r = 0; r < 4; ++r) x[mt][4 * u + r] = s[u][r] * a.scale2;
       if (!plain) {
 #pragma unroll
-        for (int u = 0; u < PARTS; ++u)
+        for (int u = 0; u < T::kParts; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (gone[u][r] || t0 + 16 * u + 4 * g + r >= limit[mt]) x[4 * u + r] = -INFINITY;
+          for (int r = 0; r < 4; ++r) {
+            const int in = 16 * u + 4 * g + r;
+            if (((gone >> in) & 1) || t0 + in >= limit[mt]) x[mt][4 * u + r] = -INFINITY;
+          }
       }
       if (a.raw) {
         const int row = row0 + 16 * mt + n;
         if (row < a.rows) {
           float* rp = a.raw + ((int64_t)unit * a.rows + row) * a.raw_ld + t0 + 4 * g;
 #pragma unroll
-          for (int u = 0; u < PARTS; ++u)
-            *(float4*)(rp + 16 * u) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+          for (int u = 0; u < T::kParts; ++u)
+            *(float4*)(rp + 16 * u) = make_float4(x[mt][4 * u], x[mt][4 * u + 1], x[mt][4 * u + 2], x[mt][4 * u + 3]);
         }
       }
-      float top = x[0];
+      float top = x[mt][0];
 #pragma unroll
-      for (int i = 1; i < 4 * PARTS; ++i) top = fmaxf(top, x[i]);
+      for (int i = 1; i < 4 * T::kParts; ++i) top = fmaxf(top, x[mt][i]);
       top = fmaxf(top, lane_xor_f(top, 16));
       top = fmaxf(top, lane_xor_f(top, 32));
-      const float m = fmaxf(w.m[mt], top);
+      const float m = fmaxf(wm[mt], top);
       const float base = m == -INFINITY ? 0.0f : m;  // nothing seen yet: every weight is exp2(-inf) = 0
-      const float shrink = __builtin_amdgcn_exp2f(w.m[mt] - base);
-      w.m[mt] = m;
+      if (__ballot(m > wm[mt])) {  // seldom, after the first tiles
+        const float shrink = __builtin_amdgcn_exp2f(wm[mt] - base);
+        wm[mt] = m;
+        wl[mt] *= shrink;
+#pragma unroll
+        for (int j = 0; j < T::kAcc; ++j) acc[mt][j] *= shrink;
+      }
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4 * PARTS; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - base);
-        sum += x[i];
+      for (int i = 0; i < 4 * T::kParts; ++i) {
+        x[mt][i] = __builtin_amdgcn_exp2f(x[mt][i] - base);
+        sum += x[mt][i];
       }
-      w.l[mt] = w.l[mt] * shrink + sum;
+      wl[mt] += sum;
+    }
+    // A value that is not finite would reach rows that do not see its token
+    // through 0 * inf: those are taken out of the product and added to the rows
+    // that see them one by one.
+    if (!plain && a.queries > 1) {
+      bool strange = false;
 #pragma unroll
-      for (int j = 0; j < T::kAcc; ++j) w.acc[mt][j] *= shrink;
-      if (!strange) {
-        add_values<F32, DP>(val, x, w.acc[mt]);
-      } else {
-        const int t_of = (row0 + 16 * mt + n) / a.group;
-        for (int t = 0; t < seen.cnt; ++t) {
-          const int lim = seen.limit(t);
-          uint32_t v[T::kValueTokens][T::kValueWords];
+      for (int j = 0; j < T::kValueTokens; ++j)
 #pragma unroll
-          for (int j = 0; j < T::kValueTokens; ++j)
+        for (int i = 0; i < T::kValueWords; ++i)
+          strange = strange || (F32 ? (val[j][i] & 0x7f800000u) == 0x7f800000u : bf16_pair_not_finite(val[j][i]));
+      if (__ballot(strange)) {
+        // not a constant to the compiler: it would keep the addresses below in registers through the whole loop
+        int here = wave;
+        asm volatile("" : "+v"(here));
+        float* outs = lds + here * 16 * (DP + 4);                              // [row][DP + 4]
+        float* weights = (float*)(queries + MT * T::kKeyVecs * kWave) + here * 16 * T::kTokens;  // [token][row]
+        const int row_at = (lane & 15) * (DP + 4);
 #pragma unroll
-            for (int i = 0; i < T::kValueWords; ++i)
-              v[j][i] = t0 + 16 * (j / 4) + 4 * g + (j & 3) < lim ? val[j][i] : 0u;
-          f32x4 acc[T::kAcc];
+        for (int j = 0; j < T::kValueTokens; ++j) {
+          const bool all = t0 + 16 * (j / 4) + 4 * g + (j & 3) < open;
 #pragma unroll
-          for (int j = 0; j < T::kAcc; ++j) acc[j] = w.acc[mt][j];
-          add_values<F32, DP>(v, x, acc);
-          if (t_of == t)
+          for (int i = 0; i < T::kValueWords; ++i) {
+            uint32_t v = val[j][i];
+            if constexpr (F32) {
+              v = (v & 0x7f800000u) == 0x7f800000u ? 0u : v;
+            } else {
+              v = (v & 0x7f800000u) == 0x7f800000u ? v & 0xffffu : v;
+              v = (v & 0x7f80u) == 0x7f80u ? v & 0xffff0000u : v;
+            }
+            val[j][i] = all ? val[j][i] : v;
+          }
+        }
 #pragma unroll
-            for (int j = 0; j < T::kAcc; ++j) w.acc[mt][j] = acc[j];
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int j = 0; j < T::kAcc; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) outs[row_at + out_dim<F32, DP>(j, r, g)] = acc[mt][j][r];
+#pragma unroll
+          for (int i = 0; i < 4 * T::kParts; ++i) weights[(16 * (i / 4) + 4 * g + (i & 3)) * 16 + n] = x[mt][i];
+          add_strange<F32>(a, seen, vbase, v_at, gone, t0, max(open - t0, 0), T::kTokens, row0 + 16 * mt, outs, DP + 4,
+                           weights);
+#pragma unroll
+          for (int j = 0; j < T::kAcc; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[mt][j][r] = outs[row_at + out_dim<F32, DP>(j, r, g)];
         }
       }
     }
+    add_values<F32, DP, MT>(val, x, a.c.dim, acc);
   }
-
   // join the four waves
   float* ml = lds + kAttnWaves * 16 * (DP + 4);
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    float l = w.l[mt];
+    float l = wl[mt];
     l += lane_xor_f(l, 16);
     l += lane_xor_f(l, 32);
     if (limit[mt] <= 0) {  // a row that sees nothing
-      w.m[mt] = -INFINITY;
+      wm[mt] = -INFINITY;
       l = 0.0f;
     }
     if (g == 0) {
-      ml[(wave * 16 + n) * 2] = w.m[mt];
+      ml[(wave * 16 + n) * 2] = wm[mt];
       ml[(wave * 16 + n) * 2 + 1] = l;
     }
     __syncthreads();
@@ -362,7 +449,7 @@ __global__ __launch_bounds__(kAttnThreads) void kv_decode_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < kAttnWaves; ++i) m = fmaxf(m, ml[(i * 16 + n) * 2]);
     const float base = m == -INFINITY ? 0.0f : m;
-    const float mine = __builtin_amdgcn_exp2f(w.m[mt] - base);
+    const float mine = __builtin_amdgcn_exp2f(wm[mt] - base);
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < kAttnWaves; ++i)
@@ -372,7 +459,7 @@ __global__ __launch_bounds__(kAttnThreads) void kv_decode_kernel(AttnArgs a) {
     for (int j = 0; j < T::kAcc; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        mo[out_dim<F32, DP>(j, r, g)] = w.m[mt] == -INFINITY ? 0.0f : w.acc[mt][j][r] * mine;
+        mo[out_dim<F32, DP>(j, r, g)] = wm[mt] == -INFINITY ? 0.0f : acc[mt][j][r] * mine;
     if (wave == 0 && g == 0) {  // for the threads that write the rows
       ml[kAttnWaves * 32 + 2 * n] = m;
       ml[kAttnWaves * 32 + 2 * n + 1] = l;
@@ -557,7 +644,8 @@ static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int di
 
 template <bool F32, int DP, int MT>
 static int launch_decode_mt(const AttnArgs& a, const AttnPlan& p, int64_t units, hipStream_t s) {
-  const int bytes = (kAttnWaves * 16 * (DP + 4) + (kAttnWaves + 1) * 32) * 4;
+  const int bytes = (kAttnWaves * 16 * (DP + 4) + (kAttnWaves + 1) * 32) * 4 + MT * Tile<F32, DP>::kKeyVecs * kWave * 16 +
+                    kAttnWaves * 16 * Tile<F32, DP>::kTokens * 4;
   if (bytes > 65536) {
     const hipError_t e = set_dynamic_lds_limit((const void*)kv_decode_kernel<F32, DP, MT>, bytes, s);
     if (e != hipSuccess) {
@@ -628,6 +716,12 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
     set_error("kv_decode: q, its strides and out must be multiples of 16 bytes");
     return kUnsupported;
   }
+  // offsets in units of 16 bytes or more are 32 bits wide
+  const uint64_t far_page = cache->pages > 0 ? cache->pages - 1 : 0, far_slot = cache->page_size - 1;
+  if ((far_page * a.c.k_page + far_slot * a.c.k_slot) >> 36 || (far_page * a.c.v_page + far_slot * a.c.v_slot) >> 36) {
+    set_error("kv_decode: a pool may span up to 64 GiB");
+    return kUnsupported;
+  }
   if (max_len < 0 || max_len > a.c.capacity) {
     set_error("kv_decode: max_len %lld must be in [0, %d], the slots of a table row", (long long)max_len,
               a.c.capacity);
@@ -666,6 +760,13 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
   a.scores = scores;
   a.out_scores = out_scores;
   a.vector_scores = scores && a.c.capacity % 4 == 0 && !(((uintptr_t)scores | (uintptr_t)out_scores) & 15);
+  uint64_t bits = 1 << 20;  // offsets in units of the largest power of two that the strides share
+  for (int64_t x : {a.c.k_page, a.c.k_slot, a.c.v_page, a.c.v_slot}) bits |= (uint64_t)x;
+  a.shift = __builtin_ctzll(bits);
+  a.k_page = (uint32_t)(a.c.k_page >> a.shift);
+  a.k_slot = (uint32_t)(a.c.k_slot >> a.shift);
+  a.v_page = (uint32_t)(a.c.v_page >> a.shift);
+  a.v_slot = (uint32_t)(a.c.v_slot >> a.shift);
   const int64_t units = cache->batch * cache->kv_heads;
   if (units * p.row_groups > INT32_MAX || p.chunks > 65535) {
     set_error("kv_decode: too many workgroups");
