@@ -26,7 +26,7 @@
 namespace tx {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef short bf16x8 __attribute__((ext_vector_type(8)));
+typedef short bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -84,10 +84,10 @@ __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
 
 template <bool F32, int DP>
 struct Tile {
-  static constexpr int kTokens = F32 ? 16 : 32;
+  static constexpr int kTokens = F32 || DP > 128 ? 16 : 32;    // 16 where keys and values of 32 would fill the registers
   static constexpr int kParts = kTokens / 16;                  // 16-token parts
   static constexpr int kKeyVecs = F32 ? DP / 16 : DP / 32;     // 16-byte vectors of a key per lane and 16 tokens
-  static constexpr int kValueTokens = F32 ? 4 : 8;             // tokens whose values a lane holds
+  static constexpr int kValueTokens = kTokens / 4;             // tokens whose values a lane holds
   static constexpr int kValueWords = F32 ? DP / 16 : DP / 32;  // 32-bit words of each
   static constexpr int kAcc = DP / 16;                         // products (and f32x4 accumulators) per 16 rows
 };
@@ -111,7 +111,7 @@ __device__ __forceinline__ void scores_of(const Keys<F32, DP>& key, const uint4*
   for (int u = 0; u < T::kParts; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < T::kKeyVecs; ++i) {
-    if (F32 && 16 * i >= dim) break;
+    if (F32 && 16 * i >= dim) continue;
     const uint4 qi = q[i * kWave];
 #pragma unroll
     for (int u = 0; u < T::kParts; ++u) {
@@ -136,7 +136,7 @@ __device__ __forceinline__ void add_values(const Values<F32, DP>& v, const float
   if constexpr (F32) {
 #pragma unroll
     for (int j = 0; j < DP / 16; ++j) {
-      if (32 * (j / 2) >= dim) break;
+      if (32 * (j / 2) >= dim) continue;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -144,28 +144,30 @@ __device__ __forceinline__ void add_values(const Values<F32, DP>& v, const float
           acc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j]), p[mt][r], acc[mt][j], 0, 0, 0);
     }
   } else {
-    bf16x8_t pb[MT];
+    // element j of a lane's tokens by the rows' weights: 32 tokens a product, or 16
+    constexpr int kPairs = Tile<F32, DP>::kValueTokens / 2;
+    uint32_t pb[MT][kPairs];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      uint4 pk;
-      pk.x = pack_bf16(p[mt][0], p[mt][1]);
-      pk.y = pack_bf16(p[mt][2], p[mt][3]);
-      pk.z = pack_bf16(p[mt][4], p[mt][5]);
-      pk.w = pack_bf16(p[mt][6], p[mt][7]);
-      pb[mt] = __builtin_bit_cast(bf16x8_t, pk);
-    }
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) pb[mt][k] = pack_bf16(p[mt][2 * k], p[mt][2 * k + 1]);
 #pragma unroll
     for (int j = 0; j < DP / 16; ++j) {
       const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-      uint4 t;  // element j of the eight tokens
-      t.x = __builtin_amdgcn_perm(v[1][j / 2], v[0][j / 2], sel);
-      t.y = __builtin_amdgcn_perm(v[3][j / 2], v[2][j / 2], sel);
-      t.z = __builtin_amdgcn_perm(v[5][j / 2], v[4][j / 2], sel);
-      t.w = __builtin_amdgcn_perm(v[7][j / 2], v[6][j / 2], sel);
+      uint32_t t[kPairs];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        acc[mt][j] =
-            __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, t), pb[mt], acc[mt][j], 0, 0, 0);
+      for (int k = 0; k < kPairs; ++k) t[k] = __builtin_amdgcn_perm(v[2 * k + 1][j / 2], v[2 * k][j / 2], sel);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (kPairs == 4)
+          acc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8_t, make_uint4(t[0], t[1], t[2], t[3])),
+              __builtin_bit_cast(bf16x8_t, make_uint4(pb[mt][0], pb[mt][1], pb[mt][2], pb[mt][3])), acc[mt][j], 0, 0, 0);
+        else
+          acc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+              __builtin_bit_cast(bf16x4, make_uint2(t[0], t[1])), __builtin_bit_cast(bf16x4, make_uint2(pb[mt][0], pb[mt][1])),
+              acc[mt][j], 0, 0, 0);
+      }
     }
   }
 }
@@ -241,7 +243,7 @@ __device__ __forceinline__ void add_strange(const AttnArgs& a, const Seen& seen,
 
 // Waves of a SIMD that the registers of an instance are held to.
 template <bool F32, int DP, int MT>
-constexpr int kWavesHeld = DP <= 128 && MT <= 2 ? (F32 && DP == 128 && MT == 1 ? 3 : 2) : 1;
+constexpr int kWavesHeld = F32 && DP > 128 ? 1 : F32 && DP == 128 && MT == 1 ? 3 : 2;
 
 template <bool F32, int DP, int MT>
 __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_decode_kernel(AttnArgs a) {
@@ -624,8 +626,11 @@ struct AttnPlan {
 
 static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int dim, int dtype, int64_t max_len,
                            bool with_scores, AttnPlan* p) {
-  const int tiles = (int)((rows + 15) / 16), most = dtype == TALLAX_F32 ? 2 : 4;
-  p->mt = tiles <= 1 ? 1 : tiles <= 2 ? 2 : most;
+  const int tiles = (int)((rows + 15) / 16), most = dtype != TALLAX_F32 && dim > 128 ? 1 : 2;
+  // 32 rows of a kv head to a workgroup, or 16: rows beyond are a workgroup of their own, which reads the keys and
+  // values again.  Its registers cost more than that: with 64 rows of dim 128 and 32 of dim 256 (bfloat16) a SIMD
+  // holds one wave, and 16 sequences x 48 rows take 207 us, against 125; 13 x 40 rows of dim 192 226, against 124.
+  p->mt = tiles < most ? 1 : most;
   p->row_groups = (tiles + p->mt - 1) / p->mt;
   p->rows = (int)rows;
   p->max_len = (int)max_len;
@@ -660,10 +665,10 @@ static int launch_decode_mt(const AttnArgs& a, const AttnPlan& p, int64_t units,
 
 template <bool F32, int DP>
 static int launch_decode(const AttnArgs& a, const AttnPlan& p, int64_t units, hipStream_t s) {
-  if (p.mt == 1) return launch_decode_mt<F32, DP, 1>(a, p, units, s);
-  if (p.mt == 2) return launch_decode_mt<F32, DP, 2>(a, p, units, s);
-  if constexpr (!F32) return launch_decode_mt<F32, DP, 4>(a, p, units, s);
-  return kInvalidArgument;
+  if constexpr (F32 || DP <= 128) {
+    if (p.mt == 2) return launch_decode_mt<F32, DP, 2>(a, p, units, s);
+  }
+  return launch_decode_mt<F32, DP, 1>(a, p, units, s);
 }
 
 }  // namespace tx
