@@ -167,38 +167,58 @@ __global__ __launch_bounds__(NW * kWave) void kv_evict_select_kernel(EvictArgs a
   const int count = (len + 4 * kThreads - 1) / (4 * kThreads);
   const int first = wave * count * kGroup + 4 * lane;
   const int64_t newest = (int64_t)a.seen[b] - a.recent;
-  auto read_four = [&](int i, float (&x)[4], int32_t (&p)[4]) {
+  struct Four {
+    float x[4];
+    int32_t p[4];
+  };
+  auto read_four = [&](int i, Four& f) {
     if (i + 4 <= len) {
-      __builtin_memcpy(x, sc + i, 16);
-      __builtin_memcpy(p, ps + i, 16);
+      __builtin_memcpy(f.x, sc + i, 16);
+      __builtin_memcpy(f.p, ps + i, 16);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        x[k] = sc[min(i + k, len - 1)];
-        p[k] = ps[min(i + k, len - 1)];
+        f.x[k] = sc[min(i + k, len - 1)];
+        f.p[k] = ps[min(i + k, len - 1)];
       }
     }
   };
-  auto read_keys = [&](int i) -> uint4 {
-    float x[4];
-    int32_t p[4];
+  auto keys_from = [&](int i, const Four& f) -> uint4 {
     uint32_t key[4];
-    read_four(i, x, p);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      key[k] = p[k] < a.sinks || p[k] >= newest ? 0xFFFFFFFFu : select_key(__float_as_uint(x[k]));
+      key[k] = f.p[k] < a.sinks || f.p[k] >= newest ? 0xFFFFFFFFu : select_key(__float_as_uint(f.x[k]));
       if (i + k >= len) key[k] = 0u;  // below every key
     }
     return make_uint4(key[0], key[1], key[2], key[3]);
   };
   const int in_lds = min(count, room);
-#pragma unroll 4
-  for (int j = 0; j < in_lds; ++j) held[j * kThreads + tid] = read_keys(first + j * kGroup);
-  // The loops below are not unrolled: a workgroup runs each of them a few times,
-  // and what it waits for then is its instructions.
-  auto keys_of = [&](int j, uint32_t (&key)[4]) {
-    const uint4 four = j < in_lds ? held[j * kThreads + tid] : read_keys(first + j * kGroup);
-    key[0] = four.x, key[1] = four.y, key[2] = four.z, key[3] = four.w;
+  {
+    Four next = {};
+    if (in_lds > 0) read_four(first, next);
+#pragma unroll 2
+    for (int j = 0; j < in_lds; ++j) {
+      const Four now = next;
+      if (j + 1 < in_lds) read_four(first + (j + 1) * kGroup, next);
+      held[j * kThreads + tid] = keys_from(first + j * kGroup, now);
+    }
+  }
+  // f(slot, keys, scores and positions of four) for this thread's slots in order; all lanes of a wave take part in
+  // every call.  Scores and positions are there for slots below `with` and where the keys are not held; they are
+  // asked for one call ahead.  The loop is not unrolled: a workgroup runs it a few times, and what it waits for then
+  // is its instructions.
+  auto each = [&](int with, auto f) {
+    Four next = {};
+    if (in_lds == 0 || first < with) read_four(first, next);
+#pragma unroll 1
+    for (int j = 0; j < count; ++j) {
+      const Four now = next;
+      const int i = first + j * kGroup;
+      if (j + 1 < count && (j + 1 >= in_lds || i + kGroup < with)) read_four(i + kGroup, next);
+      const uint4 four = j < in_lds ? held[j * kThreads + tid] : keys_from(i, now);
+      const uint32_t key[4] = {four.x, four.y, four.z, four.w};
+      f(i, key, now);
+    }
   };
   // the budget-th largest key, and how many of its equals are kept
   uint32_t prefix = 0, fixed = 0;  // bits below `fixed` are 0 in the prefix: any key from it on is kept
@@ -209,14 +229,11 @@ __global__ __launch_bounds__(NW * kWave) void kv_evict_select_kernel(EvictArgs a
     const uint32_t digit = shift ? 2047u : 1023u;
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
-#pragma unroll 1
-    for (int j = 0; j < count; ++j) {
-      uint32_t key[4];
-      keys_of(j, key);
+    each(0, [&](int i, const uint32_t (&key)[4], const Four&) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (first + j * kGroup + k < len && ((key[k] ^ prefix) & fixed) == 0) atomicAdd(&hist[(key[k] >> shift) & digit], 1);
-    }
+        if (i + k < len && ((key[k] ^ prefix) & fixed) == 0) atomicAdd(&hist[(key[k] >> shift) & digit], 1);
+    });
     __syncthreads();
     int c[kBinsOf], s = 0;  // bins from the largest digit down
 #pragma unroll
@@ -250,13 +267,10 @@ __global__ __launch_bounds__(NW * kWave) void kv_evict_select_kernel(EvictArgs a
   int first_tie = 0;
   if (!all) {
     int ties = 0;
-#pragma unroll 1
-    for (int j = 0; j < count; ++j) {
-      uint32_t key[4];
-      keys_of(j, key);
+    each(0, [&](int i, const uint32_t (&key)[4], const Four&) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ties += __popcll(__ballot(first + j * kGroup + k < len && key[k] == prefix));
-    }
+      for (int k = 0; k < 4; ++k) ties += __popcll(__ballot(i + k < len && key[k] == prefix));
+    });
     __syncthreads();  // red has been read
     first_tie = before(ties, red);
   }
@@ -269,14 +283,7 @@ __global__ __launch_bounds__(NW * kWave) void kv_evict_select_kernel(EvictArgs a
 #pragma unroll 1
   for (int write = 0; write < 2; ++write) {
     int tie = first_tie;
-#pragma unroll 1
-    for (int j = 0; j < count; ++j) {
-      const int i = first + j * kGroup;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      int32_t p[4] = {0, 0, 0, 0};
-      if (write && i < nlen) read_four(i, x, p);
-      uint32_t key[4];
-      keys_of(j, key);
+    each(write ? nlen : 0, [&](int i, const uint32_t (&key)[4], const Four& here) {
       bool keep[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) keep[k] = i + k < len && key[k] >= prefix;
@@ -305,13 +312,13 @@ __global__ __launch_bounds__(NW * kWave) void kv_evict_select_kernel(EvictArgs a
         hole += __popcll(bh);
         mover += __popcll(bm);
       }
-      if (!write) continue;
+      if (!write) return;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (i + k < nlen) {
           if (keep[k]) {
-            osc[i + k] = x[k];
-            ops[i + k] = p[k];
+            osc[i + k] = here.x[k];
+            ops[i + k] = here.p[k];
           } else {
             to[h++] = i + k;
           }
@@ -319,7 +326,7 @@ __global__ __launch_bounds__(NW * kWave) void kv_evict_select_kernel(EvictArgs a
           from[m++] = i + k;
         }
       }
-    }
+    });
     if (write) break;
     __syncthreads();  // red has been read
     const int total = mover;
