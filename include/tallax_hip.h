@@ -308,7 +308,8 @@ int tallax_softmax_topk_cumsum(const float* logits, int64_t rows, int64_t cols, 
  * bf16.  Strides are in elements, for a page, a head and a slot; the dim
  * elements of a slot are contiguous, and base addresses and strides are
  * multiples of 16 bytes (any order of heads and slots inside a page fits).
- * dim: a multiple of 8 up to 256.
+ * dim: a multiple of 8 up to 256.  A pool spans at most 2^32 times the largest
+ * power of two (16 bytes to 1 MiB) that divides its page and slot strides.
  * block_table [batch, table_width] int32: slot s of sequence b lies in page
  * block_table[b][s / page_size] at place s % page_size.  An entry outside
  * [0, pages) is no page: its slots are neither written nor seen.  Only entries

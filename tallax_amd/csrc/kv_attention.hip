@@ -721,12 +721,6 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
     set_error("kv_decode: q, its strides and out must be multiples of 16 bytes");
     return kUnsupported;
   }
-  // offsets in units of 16 bytes or more are 32 bits wide
-  const uint64_t far_page = cache->pages > 0 ? cache->pages - 1 : 0, far_slot = cache->page_size - 1;
-  if ((far_page * a.c.k_page + far_slot * a.c.k_slot) >> 36 || (far_page * a.c.v_page + far_slot * a.c.v_slot) >> 36) {
-    set_error("kv_decode: a pool may span up to 64 GiB");
-    return kUnsupported;
-  }
   if (max_len < 0 || max_len > a.c.capacity) {
     set_error("kv_decode: max_len %lld must be in [0, %d], the slots of a table row", (long long)max_len,
               a.c.capacity);
@@ -768,6 +762,13 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
   uint64_t bits = 1 << 20;  // offsets in units of the largest power of two that the strides share
   for (int64_t x : {a.c.k_page, a.c.k_slot, a.c.v_page, a.c.v_slot}) bits |= (uint64_t)x;
   a.shift = __builtin_ctzll(bits);
+  const uint64_t far_page = cache->pages > 0 ? cache->pages - 1 : 0, far_slot = cache->page_size - 1;
+  if ((far_page * a.c.k_page + far_slot * a.c.k_slot) >> a.shift >> 32 ||
+      (far_page * a.c.v_page + far_slot * a.c.v_slot) >> a.shift >> 32) {
+    set_error("kv_decode: a pool may span up to 2^32 times the largest power of two that divides its strides (%d bytes)",
+              1 << a.shift);
+    return kUnsupported;
+  }
   a.k_page = (uint32_t)(a.c.k_page >> a.shift);
   a.k_slot = (uint32_t)(a.c.k_slot >> a.shift);
   a.v_page = (uint32_t)(a.c.v_page >> a.shift);

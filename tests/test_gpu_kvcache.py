@@ -452,3 +452,88 @@ def test_decode_max_len_cuts_several_queries(gpu):
     _check(out, want[0], want[3][0], "out")
     _check(lse, want[1], want[3][1], "lse")
     _check(new, want[2], want[3][2], "scores")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", [(2, 9, 32, 4, 128, 16, [300, 70], [9, 5]), (1, 5, 24, 2, 256, 24, [290], None),
+                                  (2, 3, 33, 3, 200, 8, [130, 259], [3, 1]), (1, 12, 16, 2, 16, 5, [77], None)],
+                         ids=lambda c: "x".join(map(str, c[:6])))
+def test_decode_many_rows(gpu, dtype, case):
+    """More rows of a kv head than one workgroup takes, some of them not a whole tile, all dims."""
+    b, t, hq, hkv, d, page, lens, counts = case
+    q, k, v, table, lens, counts, scores = _inputs(15, dtype, b, t, hq, hkv, d, page, lens, counts)
+    want = R.attention(q, k, v, table, lens, d ** -0.5, counts, scores)
+    out, lse, new = _decode(gpu, q, k, v, table, lens, counts, scores)
+    _check(out, want[0], want[3][0], "out")
+    _check(lse, want[1], want[3][1], "lse")
+    _check(new, want[2], want[3][2], "scores")
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("f32", 80), ("f32", 256)])
+def test_decode_values_that_are_not_finite(gpu, dtype, dim):
+    """Values of the newest tokens of 8 queries that are infinite or NaN, in more than one place and with both signs:
+    each query shows those it sees, in the places they have, and nothing else changes."""
+    q, k, v, table, lens, counts, _ = _inputs(16, dtype, 2, 8, 8, 2, dim, 16, [140, 75], [8, 6])
+    clean = R.attention(q, k, v, table, lens, 0.125, counts)
+    bad = v.clone()
+    at = {(0, 139): (5, float("inf")), (0, 137): (7, float("-inf")), (0, 133): (dim - 1, float("nan")),
+          (1, 74): (0, float("nan")), (1, 73): (0, float("inf")), (1, 70): (3, float("-inf"))}
+    for (b, s), (d, x) in at.items():
+        bad[table[b, s // 16], :, s % 16, d] = x
+    out, lse = _decode(gpu, q, k, bad, table, lens, counts, scale=0.125)
+    got, want, room = out.double().cpu(), clean[0].clone(), clean[3][0].clone()
+    for b, n in ((0, 8), (1, 6)):
+        for t in range(n):
+            end = int(lens[b]) - n + t + 1
+            for d in {d for (bb, s), (d, _) in at.items() if bb == b}:
+                xs = [x for (bb, s), (dd, x) in at.items() if bb == b and dd == d and s < end]
+                hidden = [s for (bb, s), (dd, x) in at.items() if bb == b and dd == d and s >= end]
+                if xs:
+                    want[b, t, :, d] = sum(xs[1:], xs[0])
+                    room[b, t, :, d] = 0
+                elif hidden:
+                    assert torch.isfinite(got[b, t, :, d]).all()
+    _check(got, want, room, "out")
+    _check(lse, clean[1], clean[3][1], "lse")
+
+
+@pytest.mark.parametrize("cap,lens,budget", [(40000, [39999, 33000], 35000), (70000, [70000, 20], 4097)])
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+def test_evict_long_rows(gpu, cap, lens, budget, kind):
+    """More slots than a workgroup holds at once, against a stable sort."""
+    from tallax_amd import kvcache
+    rng = np.random.default_rng(17)
+    page, b, hkv = 100, len(lens), 2
+    width = cap // page
+    k = torch.arange(b * width * hkv * page, dtype=torch.int32).reshape(b * width, hkv, page, 1)
+    k = k.repeat(1, 1, 1, 8).to(torch.float32).contiguous()  # below 2^24: exact
+    v = -k
+    table = torch.from_numpy(rng.permutation(b * width).reshape(b, width).astype(np.int32))
+    scores = rng.standard_normal((b, hkv, cap)).astype(np.float32)
+    if kind == "ties":
+        scores = np.round(scores)
+    positions = np.broadcast_to(np.arange(cap, dtype=np.int32), (b, hkv, cap)).copy()
+    up = [x.to(gpu) for x in (k.clone(), v.clone(), table, torch.tensor(lens, dtype=torch.int32),
+                              torch.from_numpy(scores), torch.from_numpy(positions),
+                              torch.tensor(lens, dtype=torch.int32))]
+    got = kvcache.evict(*up, budget=budget, recent=100, sinks=4)
+    kk, vv = up[0].cpu(), up[1].cpu()
+    for i, n in enumerate(lens):
+        m = min(n, budget)
+        assert int(got[0][i]) == m
+        for h in range(hkv):
+            key = scores[i, h, :n].astype(np.float64)
+            key[:4] = key[n - 100:n] = 1e9
+            keep = np.zeros(n, bool)
+            keep[np.argsort(-key, kind="stable")[:m]] = True
+            source = np.arange(m)
+            source[~keep[:m]] = np.arange(n)[keep & (np.arange(n) >= m)]
+            want_s, want_p = np.zeros(cap, np.float32), np.full(cap, -1, np.int32)
+            want_s[:m], want_p[:m] = scores[i, h, source], positions[i, h, source]
+            assert np.array_equal(got[1][i, h].cpu().numpy(), want_s)
+            assert np.array_equal(got[2][i, h].cpu().numpy(), want_p)
+            slot = torch.arange(m)
+            src = torch.from_numpy(source)
+            to = kk[table[i, slot // page].long(), h, slot % page, 0]
+            assert torch.equal(to, k[table[i, src // page].long(), h, src % page, 0])
+            assert torch.equal(vv[table[i, slot // page].long(), h, slot % page, 3], -to)

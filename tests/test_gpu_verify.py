@@ -208,3 +208,15 @@ def test_small_probabilities_race_closely(gpu):
     none = np.zeros((batch, 0), np.int32)
     want = _run(gpu, "f32", None, none, logits, none.astype(np.float32), noise, None, np.ones(batch, np.float32))
     assert 1000 < (want[0][:, 0] == at[1]).sum() < 2000 and ((want[0][:, 0] == at[1]) | (want[0][:, 0] == at[2])).all()
+
+
+@pytest.mark.parametrize("dtype,qdtype", [("bf16", "f32"), ("f32", None)])
+def test_many_sequences_of_long_rows(gpu, dtype, qdtype):
+    """More workgroups in the race than find the accepted drafts themselves; some sequences greedy, some masked."""
+    batch, vocab = 70, 33001
+    draft, logits, u, noise, q, temp = _inputs(10, batch, 1, vocab, dtype, qdtype or "f32")
+    temp[::7] = 0.0
+    logits[3] = -np.inf
+    logits[4, :, 1:] = -np.inf
+    counts = np.where(np.arange(batch) % 5 == 0, 0, 1).astype(np.int32)
+    _run(gpu, dtype, qdtype, draft, logits, u, noise, q if qdtype else None, temp, counts)

@@ -47,6 +47,14 @@ def test_decode_refuses_on_the_host():
     assert _decode(_cache(batch=0)) == _lib.OK
 
 
+def test_decode_refuses_pools_past_its_offsets():
+    from tallax_amd import _lib
+    far = dict(dim=8, page_size=1, kv_heads=1, k_stride_page=24, v_stride_page=24, k_stride_slot=8, v_stride_slot=8)
+    assert _decode(_cache(pages=2 ** 31 - 1, **far), heads=1, max_len=4, q=None) == _lib.INVALID_ARGUMENT
+    assert _decode(_cache(pages=2 ** 31 - 1, **far), heads=1, max_len=4) == _lib.UNSUPPORTED  # 2^31 x 48 bytes
+    assert b"2^32" in _lib.LIB.tallax_last_error()
+
+
 def test_append_evict_refuse_on_the_host():
     import ctypes
     from tallax_amd import _lib
