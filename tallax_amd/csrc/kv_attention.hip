@@ -183,12 +183,15 @@ __device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
   return (uint32_t)__builtin_amdgcn_ds_bpermute(lane << 2, (int)x);
 }
 
+// Every load of a tile is issued, in the same order, whatever there is to load:
+// waiting for one then does not mean waiting for those after it.  Elements past
+// dim are read from the token's first ones.
 template <bool F32, int DP>
 __device__ __forceinline__ void load_key(Key<F32, DP>& k, const char* p, int g, int dim) {
 #pragma unroll
   for (int i = 0; i < Tile<F32, DP>::kKeyVecs; ++i) {
     const int d = F32 ? 16 * i + 4 * g : 32 * i + 8 * g;
-    if (d < dim) k[i] = *(const uint4*)(p + d * (F32 ? 4 : 2));
+    k[i] = *(const uint4*)(p + (d < dim ? d : 0) * (F32 ? 4 : 2));
   }
 }
 
@@ -199,23 +202,19 @@ __device__ __forceinline__ void load_value(Value<F32, DP>& w, const char* p, int
 #pragma unroll
     for (int c = 0; c < Tile<F32, DP>::kValueWords / 2; ++c) {
       const int d = 16 * E * c + E * n;
-      if (d < dim) {
-        const uint2 x = *(const uint2*)(p + d * (8 / E));
-        w[2 * c] = x.x;
-        w[2 * c + 1] = x.y;
-      }
+      const uint2 x = *(const uint2*)(p + (d < dim ? d : 0) * (8 / E));
+      w[2 * c] = x.x;
+      w[2 * c + 1] = x.y;
     }
   } else {
 #pragma unroll
     for (int c = 0; c < DP / 128; ++c) {
       const int d = (DP / 16) * n + 8 * c;
-      if (d < dim) {
-        const uint4 x = *(const uint4*)(p + 2 * d);
-        w[4 * c] = x.x;
-        w[4 * c + 1] = x.y;
-        w[4 * c + 2] = x.z;
-        w[4 * c + 3] = x.w;
-      }
+      const uint4 x = *(const uint4*)(p + 2 * (d < dim ? d : 0));
+      w[4 * c] = x.x;
+      w[4 * c + 1] = x.y;
+      w[4 * c + 2] = x.z;
+      w[4 * c + 3] = x.w;
     }
   }
 }
@@ -269,7 +268,29 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
   const int mine = lane & (T::kTokens - 1);
   auto page_at = [&](int t0) { return t0 + mine < end ? page_id(a.c, table, t0 + mine) : -1; };
   int t0 = start + wave * T::kTokens;
-  int next_page = page_at(t0);
+  // Each lane works out the place of one token and hands it to those that load
+  // from it.  Tokens past the end or in no page are read from a query.
+  const char* safe = a.q + b * a.q_batch + (int64_t)(kvh * a.group) * a.q_head;
+  struct Places {
+    int page;
+    uint32_t k, v;
+  };
+  auto places_of = [&](int t, int page) {
+    const int off = t + mine - (int)page_of(a.c.div, (uint32_t)(t + mine)) * a.c.div.size;
+    return Places{page, (uint32_t)page * a.k_page + (uint32_t)off * a.k_slot,
+                  (uint32_t)page * a.v_page + (uint32_t)off * a.v_slot};
+  };
+  Keys<F32, DP> key;
+  auto load_keys = [&](const Places& pl) {
+#pragma unroll
+    for (int u = 0; u < T::kParts; ++u) {
+      const char* p = kbase + ((uint64_t)from_lane(pl.k, 16 * u + n) << a.shift);
+      load_key<F32, DP>(key[u], (int)from_lane((uint32_t)pl.page, 16 * u + n) >= 0 ? p : safe, g, a.c.dim);
+    }
+  };
+  Places next = places_of(t0, page_at(t0));
+  load_keys(next);
+  int next_page = page_at(t0 + STEP);
 
   for (int i = threadIdx.x; i < MT * T::kKeyVecs * kWave; i += kAttnThreads) {
     const int l = i % kWave, v = i / kWave % T::kKeyVecs, mt = i / (kWave * T::kKeyVecs);
@@ -298,39 +319,26 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
   __syncthreads();
 
   for (; t0 < end; t0 += STEP) {
-    // each lane works out the place of one token and hands it to those that load from it
-    const int page = next_page;
-    const int off = t0 + mine - (int)page_of(a.c.div, (uint32_t)(t0 + mine)) * a.c.div.size;
-    const uint32_t k_at = (uint32_t)page * a.k_page + (uint32_t)off * a.k_slot;
-    const uint32_t v_at = (uint32_t)page * a.v_page + (uint32_t)off * a.v_slot;
-    const uint64_t gone = __ballot(page < 0);  // bit i: token i of the tile is past the end or in no page
+    const Places here = next;
+    const uint32_t v_at = here.v;
+    const uint64_t gone = __ballot(here.page < 0);  // bit i: token i of the tile is past the end or in no page
     const bool plain = t0 + T::kTokens <= open && gone == 0;
-    Keys<F32, DP> key;
     Values<F32, DP> val;
-    if (gone != 0 || DP != a.c.dim) {  // what is not loaded is 0
-#pragma unroll
-      for (int u = 0; u < T::kParts; ++u)
-#pragma unroll
-        for (int i = 0; i < T::kKeyVecs; ++i) key[u][i] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < T::kValueTokens; ++j)
-#pragma unroll
-        for (int i = 0; i < T::kValueWords; ++i) val[j][i] = 0;
-    }
-#pragma unroll
-    for (int u = 0; u < T::kParts; ++u) {
-      const int in = 16 * u + n;
-      const char* p = kbase + ((uint64_t)from_lane(k_at, in) << a.shift);
-      if (!((gone >> in) & 1)) load_key<F32, DP>(key[u], p, g, a.c.dim);
-    }
 #pragma unroll
     for (int j = 0; j < T::kValueTokens; ++j) {
       const int in = 16 * (j / 4) + 4 * g + (j & 3);
       const char* p = vbase + ((uint64_t)from_lane(v_at, in) << a.shift);
-      if (!((gone >> in) & 1)) load_value<F32, DP>(val[j], p, n, a.c.dim);
+      load_value<F32, DP>(val[j], (gone >> in) & 1 ? safe : p, n, a.c.dim);
     }
-    next_page = page_at(t0 + STEP);
-
+    next = places_of(t0 + STEP, next_page);
+    next_page = page_at(t0 + 2 * STEP);
+    if (DP != a.c.dim) {
+#pragma unroll
+      for (int u = 0; u < T::kParts; ++u)
+#pragma unroll
+        for (int i = 0; i < T::kKeyVecs; ++i)
+          if ((F32 ? 16 * i + 4 * g : 32 * i + 8 * g) >= a.c.dim) key[u][i] = make_uint4(0, 0, 0, 0);
+    }
     float x[MT][4 * T::kParts];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -340,6 +348,13 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
       for (int u = 0; u < T::kParts; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[mt][4 * u + r] = s[u][r] * a.scale2;
+    }
+    // the next tile's keys take the registers of these
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(next);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
       if (!plain) {
 #pragma unroll
         for (int u = 0; u < T::kParts; ++u)
@@ -383,6 +398,13 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
     // A value that is not finite would reach rows that do not see its token
     // through 0 * inf: those are taken out of the product and added to the rows
     // that see them one by one.
+    if (!plain) {
+#pragma unroll
+      for (int j = 0; j < T::kValueTokens; ++j)
+#pragma unroll
+        for (int i = 0; i < T::kValueWords; ++i)
+          val[j][i] = (gone >> (16 * (j / 4) + 4 * g + (j & 3))) & 1 ? 0u : val[j][i];
+    }
     if (!plain && a.queries > 1) {
       bool strange = false;
 #pragma unroll
