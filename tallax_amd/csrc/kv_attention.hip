@@ -366,7 +366,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
       }
       if (a.raw) {
         const int row = row0 + 16 * mt + n;
-        if (row < a.rows) {
+        if (limit[mt] > 0) {
           float* rp = a.raw + ((int64_t)unit * a.rows + row) * a.raw_ld + t0 + 4 * g;
 #pragma unroll
           for (int u = 0; u < T::kParts; ++u)
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32
   const int slot0 = ((int)blockIdx.y - out_blocks) * 1024 + tid * 4;
   const bool some = slot0 - tid * 4 < seen.len;  // else this workgroup's slots are copied
   if (some) {
-    for (int row = tid / kWave; row < a.rows; row += 4) {
+    for (int row = tid / kWave; row < seen.cnt * a.group; row += 4) {
       float2 j = join_row(ml, nch, a.rows, row);
       if (lane_id() == 0) {
         lds[2 * row] = j.x == -INFINITY ? 0.0f : j.x;
@@ -616,7 +616,7 @@ __global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32
   if (some && slot0 < seen.len) {  // raw rows are whole tiles: what lies past len in one is dropped below
     const float* raw = a.raw + (int64_t)unit * a.rows * a.raw_ld + slot0;
 #pragma unroll 4
-    for (int row = 0; row < a.rows; ++row) {
+    for (int row = 0; row < seen.cnt * a.group; ++row) {
       const float inv = lds[2 * row + 1], base = lds[2 * row];
       const float4 x = *(const float4*)(raw + (int64_t)row * a.raw_ld);
       if (inv == -1.0f) continue;  // a row that sees nothing
