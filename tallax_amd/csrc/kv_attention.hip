@@ -493,6 +493,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
       const int rn = i / (DP / 4), d = (i - rn * (DP / 4)) * 4;
       const int row = row0 + 16 * mt + rn;
       if (row >= a.rows || d >= a.c.dim) continue;
+      if (a.chunks > 1 && seen.limit(row / a.group) <= 0) continue;  // nor does the second kernel read it
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < kAttnWaves; ++k) {
@@ -528,23 +529,25 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
   }
 }
 
-// Base and 1 / sum of a row over its chunks, by one wave; the same in all lanes.
-__device__ __forceinline__ float2 join_row(const float2* ml, int nch, int rows, int row) {
-  float m = -INFINITY, l = 0.0f;
-  for (int c = lane_id(); c < nch; c += kWave) {
-    const float2 x = ml[(int64_t)c * rows + row];
-    const float t = fmaxf(m, x.x), base = t == -INFINITY ? 0.0f : t;
-    l = l * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
-    m = t;
-  }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const float om = lane_xor_f(m, d), ol = lane_xor_f(l, d);
+// Maximum and sum of a row over its chunks, by `width` neighbouring lanes (a
+// power of two, `l` of them this one); the same in all of them.
+__device__ __forceinline__ float2 join_row(const float2* ml, int nch, int rows, int row, int l, int width) {
+  float m = -INFINITY, s = 0.0f;
+  auto add = [&](float om, float os) {
     const float t = fmaxf(m, om), base = t == -INFINITY ? 0.0f : t;
-    l = l * __builtin_amdgcn_exp2f(m - base) + ol * __builtin_amdgcn_exp2f(om - base);
+    s = s * __builtin_amdgcn_exp2f(m - base) + os * __builtin_amdgcn_exp2f(om - base);
     m = t;
+  };
+  for (int c = l; c < nch; c += width) {
+    const float2 x = ml[(int64_t)c * rows + row];
+    add(x.x, x.y);
   }
-  return make_float2(m, l);
+  for (int d = 1; d < width; d <<= 1) {
+    const float om = __uint_as_float(from_lane(__float_as_uint(m), lane_id() ^ d));
+    const float os = __uint_as_float(from_lane(__float_as_uint(s), lane_id() ^ d));
+    add(om, os);
+  }
+  return make_float2(m, s);
 }
 
 // Joins the chunks.  The first `rows` workgroups of a sequence's kv head (where
@@ -554,12 +557,13 @@ __global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32
   extern __shared__ float lds[];  // an output row: 256 x 4 sums; weights: base and 1 / sum of each row
   const int unit = blockIdx.x, b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, tid = threadIdx.x;
   const Seen seen(a, b);
-  const int nch = a.chunks > 1 ? (seen.len + a.chunk - 1) / a.chunk : 1;
+  const int chunks = a.chunks > 1 ? (seen.len + a.chunk - 1) / a.chunk : 1;
   const float2* ml = a.part_ml + (int64_t)unit * a.chunks * a.rows;
   if ((int)blockIdx.y < out_blocks) {
     const int row = blockIdx.y, t = row / a.group;
     const int64_t head = ((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group);
-    const float2 j = join_row(ml, nch, a.rows, row);
+    const int nch = seen.limit(t) > 0 ? chunks : 0;
+    const float2 j = join_row(ml, nch, a.rows, row, lane_id(), kWave);
     const float base = j.x == -INFINITY ? 0.0f : j.x;
     const int width = a.c.dim <= 64 ? 16 : a.c.dim <= 128 ? 32 : 64;  // lanes that hold a row
     const int d = (tid & (width - 1)) * 4, groups = 256 / width;
@@ -602,11 +606,16 @@ __global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32
   const int slot0 = ((int)blockIdx.y - out_blocks) * 1024 + tid * 4;
   const bool some = slot0 - tid * 4 < seen.len;  // else this workgroup's slots are copied
   if (some) {
-    for (int row = tid / kWave; row < seen.cnt * a.group; row += 4) {
-      float2 j = join_row(ml, nch, a.rows, row);
-      if (lane_id() == 0) {
+    int width = 1;  // lanes of a row
+    while (width < chunks && width < kWave) width <<= 1;
+    const int used = seen.cnt * a.group, at_once = kWave / width;
+    for (int row0 = tid / kWave * at_once; row0 < used; row0 += 4 * at_once) {
+      const int row = row0 + lane_id() / width, l = lane_id() & (width - 1);
+      const bool sees = row < used && seen.limit(row / a.group) > 0;
+      const float2 j = join_row(ml, sees ? chunks : 0, a.rows, row, l, width);
+      if (l == 0 && row < used) {
         lds[2 * row] = j.x == -INFINITY ? 0.0f : j.x;
-        lds[2 * row + 1] = j.y == 0.0f || seen.limit(row / a.group) <= 0 ? -1.0f : 1.0f / j.y;
+        lds[2 * row + 1] = j.y == 0.0f ? -1.0f : 1.0f / j.y;
       }
     }
     __syncthreads();
@@ -615,15 +624,21 @@ __global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (some && slot0 < seen.len) {  // raw rows are whole tiles: what lies past len in one is dropped below
     const float* raw = a.raw + (int64_t)unit * a.rows * a.raw_ld + slot0;
-#pragma unroll 4
-    for (int row = 0; row < seen.cnt * a.group; ++row) {
-      const float inv = lds[2 * row + 1], base = lds[2 * row];
-      const float4 x = *(const float4*)(raw + (int64_t)row * a.raw_ld);
-      if (inv == -1.0f) continue;  // a row that sees nothing
-      s.x += __builtin_amdgcn_exp2f(x.x - base) * inv;
-      s.y += __builtin_amdgcn_exp2f(x.y - base) * inv;
-      s.z += __builtin_amdgcn_exp2f(x.z - base) * inv;
-      s.w += __builtin_amdgcn_exp2f(x.w - base) * inv;
+    // eight rows are asked for before the first is used
+    const int used = seen.cnt * a.group;
+    for (int row0 = 0; row0 < used; row0 += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) x[r] = *(const float4*)(raw + (int64_t)min(row0 + r, used - 1) * a.raw_ld);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (row0 + r >= used || lds[2 * (row0 + r) + 1] == -1.0f) continue;  // a row that sees nothing
+        const float base = lds[2 * (row0 + r)], inv = lds[2 * (row0 + r) + 1];
+        s.x += __builtin_amdgcn_exp2f(x[r].x - base) * inv;
+        s.y += __builtin_amdgcn_exp2f(x[r].y - base) * inv;
+        s.z += __builtin_amdgcn_exp2f(x[r].z - base) * inv;
+        s.w += __builtin_amdgcn_exp2f(x[r].w - base) * inv;
+      }
     }
   }
   const int64_t at = (int64_t)unit * a.c.capacity + slot0;
