@@ -676,9 +676,10 @@ static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int di
   // card.  With few kv heads in all 512 longer ones lose less to their beginnings and ends: 32 of 131071 slots 289 us
   // against 303, 128 of 4000 34 against 40; with 512 of 4096 they take 170 against 162, and 108 float32 ones of 2050,
   // whose products take longer, 44 against 35.  Chunks of 128 slots, not 256, where those are too few for the card:
-  // 5 kv heads of 2756 slots 11.2 us against 12.6.
+  // 5 kv heads of 2756 slots 11.2 us against 12.6; but up to 256 slots are one chunk, which needs no second launch
+  // (2 kv heads of 200 slots 6.4 us against 9.6).
   const int64_t target = units <= (dtype == TALLAX_F32 ? 32 : 128) ? 512 : 2048;
-  const int64_t least = max_len * units < 256 * 256 ? 128 : 256;
+  const int64_t least = max_len > 256 && max_len * units < 256 * 256 ? 128 : 256;
   int64_t chunk = (max_len * units / target + 127) / 128 * 128;
   if (chunk < least) chunk = least;
   p->chunk = (int)chunk;
