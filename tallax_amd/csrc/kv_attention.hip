@@ -7,17 +7,24 @@
 // are joined by a second kernel.
 //
 // Both products have the tokens of a tile as a matrix dimension and are laid
-// out so that nothing is exchanged between lanes and nothing goes through LDS:
+// out so that nothing is exchanged between lanes, and neither keys nor values go
+// through LDS:
 //   S^T = K Q^T   operand A: lane (n, g) holds 16 bytes of token n's key,
-//                 B: of row n's query; the result has row n's scores of tokens
-//                 4g .. 4g + 3 in lane (n, g)   (n = lane % 16, g = lane / 16);
+//                 B: of row n's query (from LDS); the result has row n's scores
+//                 of tokens 4g .. 4g + 3 in lane (n, g)
+//                 (n = lane % 16, g = lane / 16);
 //   O^T = V^T P^T operand B: those scores as they lie; operand A: the values of
-//                 the same tokens, which lane (n, g) has loaded whole (dim / 16
-//                 of each token, so 16 lanes read a token's value in one
-//                 piece) and transposes in its own registers.  Product j of
-//                 dim / 16 then has output d = n * dim / 16 + j.
-// bfloat16 takes the 16x16x32 products on tiles of 32 tokens, float32 the
-// 16x16x4 ones on tiles of 16.
+//                 the same tokens, which lane (n, g) has loaded (dim / 16 of
+//                 each token, so 16 lanes read a token's value in one piece) and
+//                 transposes in its own registers.  out_dim has the order in
+//                 which the outputs then lie.
+// bfloat16 takes the 16x16x32 products on tiles of 32 tokens (above dim 128
+// 16x16x16 ones on 16), float32 the 16x16x4 ones on tiles of 16.
+//
+// Bound by memory.  64 sequences of up to 4096 slots, 8 kv heads of 128
+// (bfloat16), 685 MB: 149 us here and 12 in the join, 4.2 TB/s; 4 of up to
+// 131071, 1.54 GB: 284 and 5 us, 5.35 TB/s; the loads alone take 136 and 277 us.
+// Float32, 9 of up to 2050, 12 heads of 80, 90 MB: 30 and 5 us, loads alone 22.
 #include <math.h>
 
 #include "tx_common.h"
