@@ -247,7 +247,11 @@ __device__ __forceinline__ void add_strange(const AttnArgs& a, const Seen& seen,
   }
 }
 
-// Waves of a SIMD that the registers of an instance are held to.
+// Waves of a SIMD that the registers of an instance are held to.  Left to itself
+// the compiler takes 350 registers for <bfloat16, 128, 2>, which is one wave: 32
+// sequences of up to 8191 slots with 5 queries 231 us without scores, against 160
+// with two.  A third spills (414 us), but for <float32, 128, 1>, where it holds: 9
+// sequences of up to 2050 with 12 heads 35 us against 42.
 template <bool F32, int DP, int MT>
 constexpr int kWavesHeld = F32 && DP > 128 ? 1 : F32 && DP == 128 && MT == 1 ? 3 : 2;
 
@@ -486,11 +490,19 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
     for (int i = 0; i < kAttnWaves; ++i)
       l += ml[(i * 16 + n) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(i * 16 + n) * 2] - base);
     float* mo = lds + (wave * 16 + n) * (DP + 4);
+    // four neighbouring outputs are one register of four products, or two registers of two (out_dim)
+    const bool none = wm[mt] == -INFINITY;
+    if (row0 + 16 * mt + n < a.rows) {
 #pragma unroll
-    for (int j = 0; j < T::kAcc; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        mo[out_dim<F32, DP>(j, r, g)] = wm[mt] == -INFINITY ? 0.0f : acc[mt][j][r] * mine;
+      for (int i = 0; i < T::kAcc; ++i) {
+        const int j = F32 ? i / 2 * 2 : i / 4 * 4, r = F32 ? i % 2 * 2 : i % 4;
+        const f32x4(&o)[T::kAcc] = acc[mt];
+        const float4 x = F32 ? make_float4(o[j][r], o[j + 1][r], o[j][r + 1], o[j + 1][r + 1])
+                             : make_float4(o[j][r], o[F32 ? 0 : j + 1][r], o[F32 ? 0 : j + 2][r], o[F32 ? 0 : j + 3][r]);
+        *(float4*)(mo + out_dim<F32, DP>(j, r, g)) =
+            none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * mine, x.y * mine, x.z * mine, x.w * mine);
+      }
+    }
     if (wave == 0 && g == 0) {  // for the threads that write the rows
       ml[kAttnWaves * 32 + 2 * n] = m;
       ml[kAttnWaves * 32 + 2 * n + 1] = l;
@@ -682,10 +694,10 @@ static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int di
   // Chunks of about 2048 workgroups: sequences of uneven length leave some without work, and the rest still fill the
   // card.  With few kv heads in all 512 longer ones lose less to their beginnings and ends: 32 of 131071 slots 289 us
   // against 303, 128 of 4000 34 against 40; with 512 of 4096 they take 170 against 162, and 108 float32 ones of 2050,
-  // whose products take longer, 44 against 35.  Chunks of 128 slots, not 256, where those are too few for the card:
+  // whose products take longer, 44 against 35; 26 with three workgroups of rows each 138 against 127.  Chunks of 128 slots, not 256, where those are too few for the card:
   // 5 kv heads of 2756 slots 11.2 us against 12.6; but up to 256 slots are one chunk, which needs no second launch
   // (2 kv heads of 200 slots 6.4 us against 9.6).
-  const int64_t target = units <= (dtype == TALLAX_F32 ? 32 : 128) ? 512 : 2048;
+  const int64_t target = p->row_groups == 1 && units <= (dtype == TALLAX_F32 ? 32 : 128) ? 512 : 2048;
   const int64_t least = max_len > 256 && max_len * units < 256 * 256 ? 128 : 256;
   int64_t chunk = (max_len * units / target + 127) / 128 * 128;
   if (chunk < least) chunk = least;
