@@ -250,13 +250,16 @@ __device__ __forceinline__ void add_strange(const AttnArgs& a, const Seen& seen,
 // Waves of a SIMD that the registers of an instance are held to.  Left to itself
 // the compiler takes 350 registers for <bfloat16, 128, 2>, which is one wave: 32
 // sequences of up to 8191 slots with 5 queries 231 us without scores, against 160
-// with two.  A third spills (414 us), but for <float32, 128, 1>, where it holds: 9
-// sequences of up to 2050 with 12 heads 35 us against 42.
-template <bool F32, int DP, int MT>
-constexpr int kWavesHeld = F32 && DP > 128 ? 1 : F32 && DP == 128 && MT == 1 ? 3 : 2;
+// with two; a third spills (414 us).  Instances for one query leave out what takes
+// values that are not finite apart (half of the code and 35 registers), and those
+// of 16 rows hold three waves: float32, 9 sequences of up to 2050 slots with 12
+// heads of 80 31.5 us, with two 38.8 (7 of 2985 with 8 28.8, with two 25.0).
+template <bool F32, int DP, int MT, bool MANY>
+constexpr int kWavesHeld = F32 && DP > 128 ? 1 : DP == 128 && MT == 1 && (F32 || !MANY) ? 3 : 2;
 
-template <bool F32, int DP, int MT>
-__global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_decode_kernel(AttnArgs a) {
+// MANY: more queries than one, so that some rows do not see the newest tokens.
+template <bool F32, int DP, int MT, bool MANY>
+__global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT, MANY>)) void kv_decode_kernel(AttnArgs a) {
   using T = Tile<F32, DP>;
   constexpr int ES = F32 ? 4 : 2;
   constexpr int STEP = kAttnWaves * T::kTokens;
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT>)) void kv_de
         for (int i = 0; i < T::kValueWords; ++i)
           val[j][i] = (gone >> (16 * (j / 4) + 4 * g + (j & 3))) & 1 ? 0u : val[j][i];
     }
-    if (!plain && a.queries > 1) {
+    if (MANY && !plain) {
       bool strange = false;
 #pragma unroll
       for (int j = 0; j < T::kValueTokens; ++j)
@@ -711,18 +714,18 @@ static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int di
   if (p->chunks == 1 && !with_scores) p->ml_bytes = 0;
 }
 
-template <bool F32, int DP, int MT>
+template <bool F32, int DP, int MT, bool MANY>
 static int launch_decode_mt(const AttnArgs& a, const AttnPlan& p, int64_t units, hipStream_t s) {
   const int bytes = (kAttnWaves * 16 * (DP + 4) + (kAttnWaves + 1) * 32) * 4 + MT * Tile<F32, DP>::kKeyVecs * kWave * 16 +
-                    kAttnWaves * 16 * Tile<F32, DP>::kTokens * 4;
+                    (MANY ? kAttnWaves * 16 * Tile<F32, DP>::kTokens * 4 : 0);
   if (bytes > 65536) {
-    const hipError_t e = set_dynamic_lds_limit((const void*)kv_decode_kernel<F32, DP, MT>, bytes, s);
+    const hipError_t e = set_dynamic_lds_limit((const void*)kv_decode_kernel<F32, DP, MT, MANY>, bytes, s);
     if (e != hipSuccess) {
       set_error("kv_decode: %s", hipGetErrorString(e));
       return kHipError;
     }
   }
-  kv_decode_kernel<F32, DP, MT>
+  kv_decode_kernel<F32, DP, MT, MANY>
       <<<dim3((unsigned)(units * p.row_groups), (unsigned)p.chunks), kAttnThreads, bytes, s>>>(a);
   return launch_status("kv_decode");
 }
@@ -730,9 +733,12 @@ static int launch_decode_mt(const AttnArgs& a, const AttnPlan& p, int64_t units,
 template <bool F32, int DP>
 static int launch_decode(const AttnArgs& a, const AttnPlan& p, int64_t units, hipStream_t s) {
   if constexpr (F32 || DP <= 128) {
-    if (p.mt == 2) return launch_decode_mt<F32, DP, 2>(a, p, units, s);
+    if (p.mt == 2)
+      return a.queries > 1 ? launch_decode_mt<F32, DP, 2, true>(a, p, units, s)
+                           : launch_decode_mt<F32, DP, 2, false>(a, p, units, s);
   }
-  return launch_decode_mt<F32, DP, 1>(a, p, units, s);
+  return a.queries > 1 ? launch_decode_mt<F32, DP, 1, true>(a, p, units, s)
+                       : launch_decode_mt<F32, DP, 1, false>(a, p, units, s);
 }
 
 }  // namespace tx
