@@ -22,9 +22,9 @@
 // 16x16x16 ones on 16), float32 the 16x16x4 ones on tiles of 16.
 //
 // Bound by memory.  64 sequences of up to 4096 slots, 8 kv heads of 128
-// (bfloat16), 685 MB: 149 us here and 12 in the join, 4.2 TB/s; 4 of up to
-// 131071, 1.54 GB: 284 and 5 us, 5.35 TB/s; the loads alone take 136 and 277 us.
-// Float32, 9 of up to 2050, 12 heads of 80, 90 MB: 30 and 5 us, loads alone 22.
+// (bfloat16), 685 MB: 148 us here and 12 in the join, 4.2 TB/s; 4 of up to
+// 131071, 1.54 GB: 284 and 5 us, 5.4 TB/s; the loads alone take 136 and 277 us.
+// Float32, 9 of up to 2050, 12 heads of 80, 90 MB: 26 and 5 us, loads alone 22.
 #include <math.h>
 
 #include "tx_common.h"
@@ -253,7 +253,7 @@ __device__ __forceinline__ void add_strange(const AttnArgs& a, const Seen& seen,
 // with two; a third spills (414 us).  Instances for one query leave out what takes
 // values that are not finite apart (half of the code and 35 registers), and those
 // of 16 rows hold three waves: float32, 9 sequences of up to 2050 slots with 12
-// heads of 80 31.5 us, with two 38.8 (7 of 2985 with 8 28.8, with two 25.0).
+// heads of 80 31 us, with two 39 (7 of 2985 with 8 28.8, with two 25.0).
 template <bool F32, int DP, int MT, bool MANY>
 constexpr int kWavesHeld = F32 && DP > 128 ? 1 : DP == 128 && MT == 1 && (F32 || !MANY) ? 3 : 2;
 

@@ -11,8 +11,8 @@
 // joins the chunks and writes the tokens.
 //
 // Bound by memory: 64 sequences of 5 rows of 128256 bfloat16, with the draft's
-// probabilities, 43.6 us for 148 MB (3.4 TB/s: 19 us for the rows, 4 and 22
-// for the rest); 130 of 8 rows of 151937 float32, drafts without, 117 us for
+// probabilities, 42 us for 148 MB (3.5 TB/s: 20 us for the rows, 5 and 23
+// for the rest); 130 of 8 rows of 151937 float32, drafts without, 116 us for
 // 711 MB (6.1 TB/s).  At one sequence (14 us) each launch is a chain of loads
 // that wait for each other.
 //
