@@ -537,3 +537,47 @@ def test_evict_long_rows(gpu, cap, lens, budget, kind):
             to = kk[table[i, slot // page].long(), h, slot % page, 0]
             assert torch.equal(to, k[table[i, src // page].long(), h, src % page, 0])
             assert torch.equal(vv[table[i, slot // page].long(), h, slot % page, 3], -to)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_decode_keys_that_weigh_nothing(gpu, dtype):
+    """Scores of -inf: such slots get no weight, and a query whose every score is -inf gives 0 and -inf."""
+    q, k, v, table, lens, _, scores = _inputs(18, dtype, 3, 1, 8, 2, 64, 16, [300, 40, 500], None)
+    q[..., 0] = 1.0
+    k[..., 0] = k[..., 0].nan_to_num(0.0)
+    for b, slots in ((0, range(0, 300, 3)), (1, range(40)), (2, range(0, 256))):
+        for s in slots:
+            k[table[b, s // 16], :, s % 16, 0] = -float("inf")
+    out, lse, new = _decode(gpu, q, k, v, table, lens, None, scores, scale=0.125)
+    for i in (0, 2):  # the same as without those slots
+        n = int(lens[i])
+        keep = torch.tensor([t for t in range(n) if not (t % 3 == 0 if i == 0 else t < 256)])
+        pages = -(-len(keep) // 16)
+        pools = []
+        for x in (k, v):
+            dense = torch.zeros((pages * 16, 2, 64), dtype=x.dtype)
+            dense[:len(keep)] = x[table[i, keep // 16].long(), :, keep % 16]
+            pools.append(dense.reshape(pages, 16, 2, 64).transpose(1, 2))
+        left = torch.zeros((1, 2, pages * 16))
+        left[0, :, :len(keep)] = scores[i][:, keep]
+        want = R.attention(q[i:i + 1], *pools, torch.arange(pages, dtype=torch.int32)[None],
+                           torch.tensor([len(keep)], dtype=torch.int32), 0.125, None, left)
+        _check(out[i:i + 1], want[0], want[3][0], "out")
+        _check(lse[i:i + 1], want[1], want[3][1], "lse")
+        got = new[i].cpu()
+        _check(got[:, keep], want[2][0][:, :len(keep)], want[3][2][0][:, :len(keep)], "scores")
+        rest = torch.ones(scores.shape[2], dtype=torch.bool)
+        rest[keep] = False
+        assert torch.equal(got[:, rest], scores[i][:, rest])
+    assert float(out[1].float().abs().max()) == 0 and bool((lse[1] == -float("inf")).all())
+    assert torch.equal(new[1].cpu(), scores[1])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_decode_scales(gpu, scale):
+    q, k, v, table, lens, counts, scores = _inputs(19, "bf16", 2, 2, 8, 2, 128, 16, [290, 17], [2, 1])
+    want = R.attention(q, k, v, table, lens, scale, counts, scores)
+    out, lse, new = _decode(gpu, q, k, v, table, lens, counts, scores, scale=scale)
+    _check(out, want[0], want[3][0], "out")
+    _check(lse, want[1], want[3][1], "lse")
+    _check(new, want[2], want[3][2], "scores")
