@@ -641,7 +641,7 @@ static VerifyPlan plan_verify(int64_t batch, int64_t drafted, int64_t vocab, int
   p.stat_chunks = (int)((blocks + p.stat_vecs - 1) / p.stat_vecs);
   // and of the race about 2048: the same rows 31 us, with 512 49
   const int64_t size = kVerThreads * (vocab < kRaceVec ? 1 : kRaceVec);
-  steps = vocab * batch / (2048 * size);
+  steps = (vocab * batch + 1024 * size) / (2048 * size);
   p.race_size = (steps < 1 ? 1 : steps) * size;
   p.race_chunks = (int)((vocab + p.race_size - 1) / p.race_size);
   p.part_bytes = align_up((size_t)rows * p.stat_chunks * sizeof(RowPart), 256);
