@@ -56,6 +56,18 @@ int tallax_testing_top_dynamic_k_path(const void* x, int dtype, int64_t rows, in
                                       int32_t* out_idx, int32_t* out_valid, int32_t* out_depths, float* out_cutoff,
                                       void* workspace, size_t workspace_bytes, tallax_stream_t stream, int path);
 
+/* tallax_verify with `stat_steps` steps of 1024 16-byte blocks to a workgroup of
+ * the rows' sums and `race_steps` steps of 2048 elements (256 in vocabularies
+ * below 8) to one of the race, 0: as many as tallax_verify takes.  It takes
+ * more than one only where there are thousands of workgroups; tests ask for
+ * them at small sizes.  Other arguments and results as tallax_verify;
+ * its workspace holds any number from tallax_verify's own on. */
+int tallax_testing_verify_steps(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch,
+                                int64_t drafted, int64_t vocab, const int32_t* counts, const float* temperature,
+                                const void* draft_probs, int probs_dtype, const float* uniforms, const float* noise,
+                                int32_t* out_tokens, int32_t* out_accepted, void* workspace, size_t workspace_bytes,
+                                tallax_stream_t stream, int stat_steps, int race_steps);
+
 /* Reads nbytes of src with `width`-byte loads (4, 8 or 16; src aligned to it,
  * nbytes a multiple of it) and writes one word per workgroup to out (2048
  * words): the calibration launch for the FETCH_SIZE counter. */

@@ -89,6 +89,8 @@ _SIGNATURES = {
     "tallax_testing_top_dynamic_k_path": ([_c_p, _c_int, _c_i64, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_int,
                                            _c_int, _c_int, _c_d, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p, _c_int],
                                           _c_int),
+    "tallax_testing_verify_steps": ([_c_p, _c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_int, _c_p, _c_p,
+                                     _c_p, _c_p, _c_p, _c_sz, _c_p, _c_int, _c_int], _c_int),
 }
 
 

@@ -28,7 +28,7 @@
 #include "tx_common.h"
 #include "tx_host.h"
 
-#include "tallax_hip.h"
+#include "tallax_hip_testing.h"
 
 namespace tx {
 
@@ -170,10 +170,12 @@ __device__ __forceinline__ float element(const uint4& w, int e) {
 }
 
 // One row's chunk.  Inside a row, and where no element is NaN or +inf, an
-// element takes its maximum, two products for its exponent
-//   (l - m) * f = fma(l, lo, fma(l, hi, c)),  c = -m * hi rounded
-// (what c was rounded by goes into the sum as one factor), exp2 and an addition:
-// about 9 issue slots of the 14 that a bf16 element has at the rate of memory.
+// element takes its maximum, the difference d = l - m to the largest of its
+// thread so far, two products for its exponent d * f = fma(d, hi, d * lo), exp2
+// and an addition: about 10 issue slots of the 14 that a bf16 element has at the
+// rate of memory.  The difference comes first: m may be a mask's -1e9 or a
+// forced token's 1e9, of which m * f alone is rounded by more than a whole
+// exponent.  It is at most 0, so that neither product nor their sum is NaN.
 // Everything else takes the second form, element by element.
 template <int DT>
 __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a) {
@@ -230,14 +232,13 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
       slow = !(top <= FLT_MAX);  // +inf, or a signalling NaN
       if (!slow && !greedy && top > -INFINITY) {
         const float nm = fmaxf(m, top);
-        const float c = -nm * scale.hi;
         float t = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
           for (int e = 0; e < N; ++e) {
-            const float l = element<DT>(w[v], e);
-            t += __builtin_amdgcn_exp2f(__builtin_fmaf(l, scale.lo, __builtin_fmaf(l, scale.hi, c)));
+            const float d = element<DT>(w[v], e) - nm;
+            t += __builtin_amdgcn_exp2f(__builtin_fmaf(d, scale.hi, d * scale.lo));
           }
         slow = !(t <= FLT_MAX);  // a NaN among them
         if (!slow) {
@@ -245,8 +246,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
             s = m == -INFINITY ? 0.0f : s * scale.weight(m - nm);
             m = nm;
           }
-          const float off = __builtin_fmaf(-nm, scale.hi, -c) - nm * scale.lo;
-          s += t * __builtin_amdgcn_exp2f(off);
+          s += t;
         }
       } else if (!slow && greedy && top > m) {
         m = top;
@@ -628,20 +628,22 @@ struct VerifyPlan {
   size_t part_bytes, draft_bytes, drawn_bytes, race_bytes, bytes;
 };
 
-static VerifyPlan plan_verify(int64_t batch, int64_t drafted, int64_t vocab, int dtype) {
+// stat_steps, race_steps: steps of a workgroup (0: as many as are best).
+static VerifyPlan plan_verify(int64_t batch, int64_t drafted, int64_t vocab, int dtype, int stat_steps = 0,
+                              int race_steps = 0) {
   VerifyPlan p;
   const int64_t n = dtype == TALLAX_BF16 ? 8 : 4;
   const int64_t blocks = (vocab + n - 1) / n + 1;  // a row may begin inside a block
   // up to about 8192 workgroups of whole steps (a thread's 4 blocks): at 1040 rows of 151937 float32 86 us,
   // with 4096 of them 86 to 92, with 2048 129 (the last ones of uneven rows run alone)
   const int64_t step = kVerThreads * 4, rows = batch * (drafted + 1);
-  int64_t steps = blocks * rows / (8192 * step);
+  int64_t steps = stat_steps ? stat_steps : blocks * rows / (8192 * step);
   if (steps < 1) steps = 1;
   p.stat_vecs = steps * step;
   p.stat_chunks = (int)((blocks + p.stat_vecs - 1) / p.stat_vecs);
   // and of the race about 2048: the same rows 31 us, with 512 49
   const int64_t size = kVerThreads * (vocab < kRaceVec ? 1 : kRaceVec);
-  steps = (vocab * batch + 1024 * size) / (2048 * size);
+  steps = race_steps ? race_steps : (vocab * batch + 1024 * size) / (2048 * size);
   p.race_size = (steps < 1 ? 1 : steps) * size;
   p.race_chunks = (int)((vocab + p.race_size - 1) / p.race_size);
   p.part_bytes = align_up((size_t)rows * p.stat_chunks * sizeof(RowPart), 256);
@@ -673,22 +675,11 @@ static int launch_verify(const VerifyArgs& a, hipStream_t s) {
   return launch_status("verify");
 }
 
-}  // namespace tx
-
-using namespace tx;
-
-extern "C" {
-
-size_t tallax_verify_workspace_size(int64_t batch, int64_t drafted, int64_t vocab, int logits_dtype) {
-  if (batch < 0 || drafted < 0 || vocab < 1) return 0;
-  const VerifyPlan p = plan_verify(batch, drafted, vocab, logits_dtype);
-  return p.bytes;
-}
-
-int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch, int64_t drafted,
+static int verify(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch, int64_t drafted,
                   int64_t vocab, const int32_t* counts, const float* temperature, const void* draft_probs,
                   int probs_dtype, const float* uniforms, const float* noise, int32_t* out_tokens,
-                  int32_t* out_accepted, void* workspace, size_t workspace_bytes, tallax_stream_t stream) {
+                  int32_t* out_accepted, void* workspace, size_t workspace_bytes, tallax_stream_t stream,
+                  int stat_steps, int race_steps) {
   if (batch < 0 || drafted < 0 || vocab < 1 || vocab > INT32_MAX) {
     set_error("verify: batch %lld, drafted %lld, vocab %lld", (long long)batch, (long long)drafted, (long long)vocab);
     return kInvalidArgument;
@@ -708,7 +699,7 @@ int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, in
     set_error("verify: null pointer");
     return kInvalidArgument;
   }
-  const VerifyPlan p = plan_verify(batch, drafted, vocab, logits_dtype);
+  const VerifyPlan p = plan_verify(batch, drafted, vocab, logits_dtype, stat_steps, race_steps);
   if (!workspace || workspace_bytes < p.bytes) {
     set_error("verify: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
     return kWorkspaceTooSmall;
@@ -738,6 +729,39 @@ int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, in
   a.race_size = p.race_size;
   return logits_dtype == TALLAX_BF16 ? launch_verify<kBF16>(a, (hipStream_t)stream)
                                      : launch_verify<kF32>(a, (hipStream_t)stream);
+}
+
+}  // namespace tx
+
+using namespace tx;
+
+extern "C" {
+
+size_t tallax_verify_workspace_size(int64_t batch, int64_t drafted, int64_t vocab, int logits_dtype) {
+  if (batch < 0 || drafted < 0 || vocab < 1) return 0;
+  const VerifyPlan p = plan_verify(batch, drafted, vocab, logits_dtype);
+  return p.bytes;
+}
+
+int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch, int64_t drafted,
+                  int64_t vocab, const int32_t* counts, const float* temperature, const void* draft_probs,
+                  int probs_dtype, const float* uniforms, const float* noise, int32_t* out_tokens,
+                  int32_t* out_accepted, void* workspace, size_t workspace_bytes, tallax_stream_t stream) {
+  return verify(draft, logits, logits_dtype, batch, drafted, vocab, counts, temperature, draft_probs, probs_dtype,
+                uniforms, noise, out_tokens, out_accepted, workspace, workspace_bytes, stream, 0, 0);
+}
+
+int tallax_testing_verify_steps(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch,
+                                int64_t drafted, int64_t vocab, const int32_t* counts, const float* temperature,
+                                const void* draft_probs, int probs_dtype, const float* uniforms, const float* noise,
+                                int32_t* out_tokens, int32_t* out_accepted, void* workspace, size_t workspace_bytes,
+                                tallax_stream_t stream, int stat_steps, int race_steps) {
+  if (stat_steps < 0 || race_steps < 0 || stat_steps > 65536 || race_steps > 65536) {
+    set_error("verify: %d and %d steps (0 to 65536)", stat_steps, race_steps);
+    return kInvalidArgument;
+  }
+  return verify(draft, logits, logits_dtype, batch, drafted, vocab, counts, temperature, draft_probs, probs_dtype,
+                uniforms, noise, out_tokens, out_accepted, workspace, workspace_bytes, stream, stat_steps, race_steps);
 }
 
 }  // extern "C"
