@@ -355,7 +355,7 @@ int tallax_kv_append(const tallax_kv_cache* cache, const int32_t* lens, const in
  * same buffer): out_scores = scores + the sum of w_j over the queries and the heads of
  * a kv head; other slots are copied.  lens above max_len are taken as max_len
  * (max_len: a bound on lens that the host knows, at most the capacity).
- * Workspace: tallax_kv_decode_workspace_size bytes.
+ * Workspace: tallax_kv_decode_workspace_size bytes, on a multiple of 16.
  * ---------------------------------------------------------------------- */
 size_t tallax_kv_decode_workspace_size(const tallax_kv_cache* cache, int64_t queries, int64_t heads, int64_t max_len,
                                        int with_scores);
@@ -375,7 +375,7 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
  * kv_heads, table_width * page_size] are written to out_scores and
  * out_positions, distinct buffers, with 0 and -1 from new_len on.  out_lens
  * [batch] = new_len.  Slots in no page take part in the choice but are not
- * moved.  Workspace: tallax_kv_evict_workspace_size bytes.
+ * moved.  Workspace: tallax_kv_evict_workspace_size bytes, on a multiple of 16.
  * ---------------------------------------------------------------------- */
 size_t tallax_kv_evict_workspace_size(const tallax_kv_cache* cache, int64_t budget);
 int tallax_kv_evict(const tallax_kv_cache* cache, const int32_t* lens, const float* scores, const int32_t* positions,
@@ -403,7 +403,8 @@ int tallax_kv_evict(const tallax_kv_cache* cache, const int32_t* lens, const flo
  * logits share the whole weight.  A draft outside [0, vocab) is refused.
  * out_tokens [batch, drafted + 1] int32: the accepted drafts, the next token,
  * then -1; out_accepted [batch] int32 = n.  A row with no admissible logit
- * gives the token -1.  Workspace: tallax_verify_workspace_size bytes.
+ * gives the token -1.  Workspace: tallax_verify_workspace_size bytes, on a
+ * multiple of 16.
  * ---------------------------------------------------------------------- */
 size_t tallax_verify_workspace_size(int64_t batch, int64_t drafted, int64_t vocab, int logits_dtype);
 int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch, int64_t drafted,

@@ -798,11 +798,8 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
   }
   AttnPlan p;
   plan_attention(cache->batch, cache->kv_heads, rows, a.c.dim, cache->dtype, max_len, scores != nullptr, &p);
-  const size_t need = p.ml_bytes + p.o_bytes + p.raw_bytes;
-  if (need && (!workspace || workspace_bytes < need)) {
-    set_error("kv_decode: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    return kWorkspaceTooSmall;
-  }
+  st = check_workspace("kv_decode", workspace, workspace_bytes, p.ml_bytes + p.o_bytes + p.raw_bytes);
+  if (st != kOk) return st;
   a.q = (const char*)q;
   a.q_batch = q_stride_batch * es;
   a.q_query = q_stride_query * es;

@@ -480,11 +480,8 @@ int tallax_kv_evict(const tallax_kv_cache* cache, const int32_t* lens, const flo
     return kInvalidArgument;
   }
   budget = clamp_budget(budget, a.c.capacity);
-  const size_t bytes = tallax_kv_evict_workspace_size(cache, budget);
-  if (!workspace || workspace_bytes < bytes) {
-    set_error("kv_evict: workspace of %zu bytes, %zu needed", workspace_bytes, bytes);
-    return kWorkspaceTooSmall;
-  }
+  st = check_workspace("kv_evict", workspace, workspace_bytes, tallax_kv_evict_workspace_size(cache, budget));
+  if (st != kOk) return st;
   a.lens = lens;
   a.scores = scores;
   a.positions = positions;

@@ -28,6 +28,20 @@ inline int launch_status(const char* what) {
   return kOk;
 }
 
+// A serving call's workspace: large enough, and on 16 bytes, since whole vectors and 64-bit atomics go into it.
+inline int check_workspace(const char* what, const void* at, size_t bytes, size_t need) {
+  if (need == 0) return kOk;
+  if (!at || bytes < need) {
+    set_error("%s: workspace of %zu bytes, %zu needed", what, bytes, need);
+    return kWorkspaceTooSmall;
+  }
+  if ((uintptr_t)at & 15) {
+    set_error("%s: the workspace must begin on a multiple of 16 bytes", what);
+    return kInvalidArgument;
+  }
+  return kOk;
+}
+
 // float -> nearest bfloat16 (ties to even; NaN stays NaN), as a float
 inline float round_to_bf16(float f) {
   uint32_t b;

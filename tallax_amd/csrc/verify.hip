@@ -700,10 +700,8 @@ static int verify(const int32_t* draft, const void* logits, int logits_dtype, in
     return kInvalidArgument;
   }
   const VerifyPlan p = plan_verify(batch, drafted, vocab, logits_dtype, stat_steps, race_steps);
-  if (!workspace || workspace_bytes < p.bytes) {
-    set_error("verify: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
-    return kWorkspaceTooSmall;
-  }
+  const int st = check_workspace("verify", workspace, workspace_bytes, p.bytes);
+  if (st != kOk) return st;
   VerifyArgs a;
   a.draft = draft;
   a.logits = logits;

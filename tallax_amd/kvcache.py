@@ -60,8 +60,9 @@ def decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_
 
     scale: default dim ** -0.5.  max_len: a bound on lens known to the caller
     (default: what the table can hold); the length is split by it, and lens
-    above it are taken as max_len.  workspace: a uint8 device tensor used
-    instead of the shared per-device buffer.
+    above it are taken as max_len.  workspace: a uint8 device tensor that
+    begins on a multiple of 16 bytes, used instead of the shared per-device
+    buffer.
     """
     return _lib.SERVING.decode(q, k_pages, v_pages, block_table, lens, scale, counts, scores, out_scores, max_len,
                                workspace)
@@ -80,7 +81,7 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tenso
     and only as many as that takes; returns (new_lens, new_scores,
     new_positions), new tensors, with 0 and -1 in the slots from the new length
     on.  Sequences of at most `budget` slots are left alone.  recent + sinks
-    must not exceed budget.
+    must not exceed budget.  workspace: as decode's.
     """
     return _lib.SERVING.evict(k_pages, v_pages, block_table, lens, scores, positions, seen, budget, recent, sinks,
                               workspace)

@@ -35,7 +35,9 @@ def verify(draft_tokens: torch.Tensor, target_logits: torch.Tensor, uniforms: to
     the next token is that one).  -inf logits (a mask's) are never drawn.
 
     Returns (tokens [batch, drafted + 1] int32: the accepted drafts, the next
-    token, then -1; accepted [batch] int32).
+    token, then -1; accepted [batch] int32).  workspace: a uint8 device tensor
+    that begins on a multiple of 16 bytes, used instead of the shared
+    per-device buffer.
     """
     return _lib.SERVING.verify(draft_tokens, target_logits, uniforms, noise, draft_probs, temperature, counts, workspace)
 
