@@ -209,7 +209,10 @@ def _load_serving():
         raise ImportError(
             f"tallax_amd extension not built: {_LIB_PATH.parent / 'serving_ext.so'} is missing. "
             "Run `python -c 'import __graft_entry__ as g; g.build()'` (hipcc, gfx950).")
-    from ._build import serving_ext
+    try:
+        from ._build import serving_ext
+    except ImportError as e:
+        raise ImportError(f"tallax_amd/_build/serving_ext.so cannot be loaded (built against another torch?): {e}") from e
 
     def per_row(value, rows, device):
         from .sampling import _per_row
@@ -219,7 +222,15 @@ def _load_serving():
     return serving_ext
 
 
-SERVING = _load_serving()
+globals().pop("SERVING", None)  # a reload sets the module up again
+
+
+def __getattr__(name: str):
+    """SERVING is loaded on first use: sort, selection and sampling do without it."""
+    if name != "SERVING":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()[name] = module = _load_serving()
+    return module
 
 
 def select_plan(rows: int, cols: int, dtype: int, k: int = 128, sample: bool = True) -> dict:
