@@ -249,17 +249,24 @@ __device__ __forceinline__ void add_strange(const AttnArgs& a, const Seen& seen,
 
 // Waves of a SIMD that the registers of an instance are held to.  Left to itself
 // the compiler takes 350 registers for <bfloat16, 128, 2>, which is one wave: 32
-// sequences of up to 8191 slots with 5 queries 231 us without scores, against 160
+// sequences of up to 8191 slots with 5 queries 231 us without scores, against 142
 // with two; a third spills (414 us).  Instances for one query leave out what takes
 // values that are not finite apart (half of the code and 35 registers), and those
-// of 16 rows hold three waves: float32, 9 sequences of up to 2050 slots with 12
-// heads of 80 31 us, with two 39 (7 of 2985 with 8 28.8, with two 25.0).
+// of 16 rows hold three waves.  In float32 that pays where two would leave
+// workgroups waiting for a place on the card.  Of 152 cases of one query, those
+// with 769 to 1152 workgroups are 2 to 19 % faster with three in 13 of 14 (9
+// sequences of up to 2050 slots with 12 heads of 80 31.1 us, with two 38.3), and
+// those with more by 2 % in the mean; those with 513 to 768, three to a CU, are 4
+// to 21 % slower in 14 of 16 (7 of 2985 with 8 of 128 36.8, with two 31.9), and
+// those with fewer the same.  With several queries two are faster in 35 of 41, by
+// 2 % in the mean.
 template <bool F32, int DP, int MT, bool MANY>
-constexpr int kWavesHeld = F32 && DP > 128 ? 1 : DP == 128 && MT == 1 && (F32 || !MANY) ? 3 : 2;
+constexpr int kWavesHeld = F32 && DP > 128 ? 1 : DP == 128 && MT == 1 && !MANY ? 3 : 2;
+constexpr int64_t kTwoWavesUpTo = 3 * 256;  // workgroups of a float32 launch of one query
 
 // MANY: more queries than one, so that some rows do not see the newest tokens.
-template <bool F32, int DP, int MT, bool MANY>
-__global__ __launch_bounds__(kAttnThreads, (kWavesHeld<F32, DP, MT, MANY>)) void kv_decode_kernel(AttnArgs a) {
+template <bool F32, int DP, int MT, bool MANY, int WAVES>
+__global__ __launch_bounds__(kAttnThreads, WAVES) void kv_decode_kernel(AttnArgs a) {
   using T = Tile<F32, DP>;
   constexpr int ES = F32 ? 4 : 2;
   constexpr int STEP = kAttnWaves * T::kTokens;
@@ -714,18 +721,20 @@ static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int di
   if (p->chunks == 1 && !with_scores) p->ml_bytes = 0;
 }
 
-template <bool F32, int DP, int MT, bool MANY>
+template <bool F32, int DP, int MT, bool MANY, int WAVES = kWavesHeld<F32, DP, MT, MANY>>
 static int launch_decode_mt(const AttnArgs& a, const AttnPlan& p, int64_t units, hipStream_t s) {
+  if constexpr (F32 && WAVES == 3)
+    if (units * p.row_groups * p.chunks <= kTwoWavesUpTo) return launch_decode_mt<F32, DP, MT, MANY, 2>(a, p, units, s);
   const int bytes = (kAttnWaves * 16 * (DP + 4) + (kAttnWaves + 1) * 32) * 4 + MT * Tile<F32, DP>::kKeyVecs * kWave * 16 +
                     (MANY ? kAttnWaves * 16 * Tile<F32, DP>::kTokens * 4 : 0);
   if (bytes > 65536) {
-    const hipError_t e = set_dynamic_lds_limit((const void*)kv_decode_kernel<F32, DP, MT, MANY>, bytes, s);
+    const hipError_t e = set_dynamic_lds_limit((const void*)kv_decode_kernel<F32, DP, MT, MANY, WAVES>, bytes, s);
     if (e != hipSuccess) {
       set_error("kv_decode: %s", hipGetErrorString(e));
       return kHipError;
     }
   }
-  kv_decode_kernel<F32, DP, MT, MANY>
+  kv_decode_kernel<F32, DP, MT, MANY, WAVES>
       <<<dim3((unsigned)(units * p.row_groups), (unsigned)p.chunks), kAttnThreads, bytes, s>>>(a);
   return launch_status("kv_decode");
 }
