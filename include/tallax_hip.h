@@ -399,12 +399,12 @@ int tallax_kv_evict(const tallax_kv_cache* cache, const int32_t* lens, const flo
  *   the lowest v), r = max(p_n - q_n, 0) where draft n was refused, r = p_n
  *   where all were accepted or p_n - q_n is nowhere positive.
  * A row with temperature < 1e-5 is greedy: p is 1 at the largest logit (lowest
- * index), and the next token is that one.  NaN logits count as -inf; +inf
- * logits share the whole weight.  A draft outside [0, vocab) is refused.
- * out_tokens [batch, drafted + 1] int32: the accepted drafts, the next token,
- * then -1; out_accepted [batch] int32 = n.  A row with no admissible logit
- * gives the token -1.  Workspace: tallax_verify_workspace_size bytes, on a
- * multiple of 16.
+ * index), and the next token is that one.  The sums of p are of 32-bit weights,
+ * off by some 1e-7 of themselves.  NaN logits count as -inf; +inf logits share
+ * the whole weight.  A draft outside [0, vocab) is refused.  out_tokens [batch,
+ * drafted + 1] int32: the accepted drafts, the next token, then -1;
+ * out_accepted [batch] int32 = n.  A row with no admissible logit gives the
+ * token -1.  Workspace: tallax_verify_workspace_size bytes, on a multiple of 16.
  * ---------------------------------------------------------------------- */
 size_t tallax_verify_workspace_size(int64_t batch, int64_t drafted, int64_t vocab, int logits_dtype);
 int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, int64_t batch, int64_t drafted,

@@ -22,9 +22,13 @@
 // 16x16x16 ones on 16), float32 the 16x16x4 ones on tiles of 16.
 //
 // Bound by memory.  64 sequences of up to 4096 slots, 8 kv heads of 128
-// (bfloat16), 685 MB: 148 us here and 12 in the join, 4.2 TB/s; 4 of up to
-// 131071, 1.54 GB: 284 and 5 us, 5.4 TB/s; the loads alone take 136 and 277 us.
+// (bfloat16), 685 MB: 148 us here and 13 in the join, 4.2 TB/s; 4 of up to
+// 131071, 1.54 GB: 285 and 5 us, 5.3 TB/s; the loads alone take 136 and 277 us.
 // Float32, 9 of up to 2050, 12 heads of 80, 90 MB: 26 and 5 us, loads alone 22.
+//
+// The length is split by max_len, which is the table's width unless the caller
+// knows a smaller bound: 4 sequences of up to 4096 slots with 8 kv heads take 16 us,
+// also in a table of 131072 slots with max_len 4096, and 54 there without it.
 #include <math.h>
 
 #include "tx_common.h"
@@ -151,7 +155,11 @@ __device__ __forceinline__ void add_values(const Values<F32, DP>& v, const float
           acc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][j]), p[mt][r], acc[mt][j], 0, 0, 0);
     }
   } else {
-    // element j of a lane's tokens by the rows' weights: 32 tokens a product, or 16
+    // Element j of a lane's tokens by the rows' weights: 32 tokens a product, or 16.  The product takes both sides in
+    // bfloat16: the weights, at most 1, are rounded to it (by 2^-8 of each at most), and their sum, by which the output
+    // is divided, is of the unrounded ones.  The roundings are of either sign and meet the output's own to bfloat16:
+    // against 64 bits the output is off by 5 to 8 % more than with 32-bit weights, which would take two products or
+    // the float32 ones at an eighth of the rate.
     constexpr int kPairs = Tile<F32, DP>::kValueTokens / 2;
     uint32_t pb[MT][kPairs];
 #pragma unroll

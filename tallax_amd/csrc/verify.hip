@@ -11,15 +11,18 @@
 // joins the chunks and writes the tokens.
 //
 // Bound by memory: 64 sequences of 5 rows of 128256 bfloat16, with the draft's
-// probabilities, 42 us for 148 MB (3.5 TB/s: 20 us for the rows, 5 and 23
-// for the rest); 130 of 8 rows of 151937 float32, drafts without, 116 us for
-// 711 MB (6.1 TB/s).  At one sequence (14 us) each launch is a chain of loads
-// that wait for each other.
+// probabilities, 42 us for the 136 MB that it reads, rows past a sequence's
+// drafts left out (3.2 TB/s: 19 us for the rows, 5 and 20 for the rest); 130 of 8
+// rows of 151937 float32, drafts without, 116 us for 666 MB (5.7 TB/s).  At one
+// sequence (14 us) each launch is a chain of loads that wait for each other.
 //
-// A token hangs on every comparison, so comparisons are made in 64 bits:
-// sums of 32-bit weights are joined in 64, an accepted draft's probability is
-// computed in 64, and the race computes 32-bit scores with a bound on their
-// error and evaluates in 64 bits only those that may be the largest.
+// A token hangs on every comparison, so comparisons are made in 64 bits: an
+// accepted draft's probability is computed in 64, and the race computes 32-bit
+// scores with a bound on their error and evaluates in 64 bits only those that
+// may be the largest.  A row's sum is of 32-bit weights, added up in 32 bits by
+// each thread and joined in 64: 64-bit exponentials of every logit would take
+// longer than reading it.  The sum is off by some 1e-7 of itself, so a draft
+// whose u q is as near as that to p may fall on either side.
 #include <float.h>
 #include <math.h>
 
@@ -498,8 +501,9 @@ __device__ __forceinline__ RacePart race_chunk(const VerifyArgs& a, int b, const
     for (int k = 0; k < VEC; ++k) {
       l[k] = span.from + k >= span.own ? clean(l[k]) : -INFINITY;
       const float p = scale.weight(l[k] - d.max) * inv_sum;
-      // p is off by at most 2^-17 of itself (its exponent is as low as -150 and rounded to half of 2^-16; exp2
-      // and four roundings add little) and by what lies below the normal numbers, the quotient by 2^-21 more.
+      // p is off by at most 1.2e-5 of itself, below 2^-16: its exponent is as low as -150 and rounded to half of
+      // 2^-16 (ln 2 of which is 5.3e-6), l - max by 2^-24 of itself (150 ln 2 2^-24 = 6.2e-6), and exp2, the sum's
+      // reciprocal and three roundings add 4e-7; and by what lies below the normal numbers, the quotient by 2^-21 more.
       // The reciprocal of noise below the normal numbers may be infinite: it bounds from above only.
       const float slack = p * 0x1p-16f + 0x1p-120f;
       const float r = __builtin_amdgcn_rcpf(e[k]);

@@ -32,7 +32,9 @@ def verify(draft_tokens: torch.Tensor, target_logits: torch.Tensor, uniforms: to
     max(p - q, 0)(v) / noise(v) in the row of the first refused draft, or of
     p(v) / noise(v) after the last accepted one, ties to the lowest id
     (temperature < 1e-5: the drafts are compared with the largest logit, and
-    the next token is that one).  -inf logits (a mask's) are never drawn.
+    the next token is that one).  -inf logits (a mask's) are never drawn.  The
+    sums of p are of 32-bit weights, off by some 1e-7 of themselves; a draft as
+    near as that to its border may fall on either side.
 
     Returns (tokens [batch, drafted + 1] int32: the accepted drafts, the next
     token, then -1; accepted [batch] int32).  workspace: a uint8 device tensor
