@@ -33,20 +33,20 @@ def listed():
         {"name": "rotate video", "op": "rotate", "batch": 3, "tokens": 2501, "heads": 12, "kv_heads": 12, "dim": 80,
          "pairs": 30, "page": 24, "longest": 8192, "dtype": "f32", "axes": 3, "interleaved": True},
         # a few users of one short instruction, few heads
-        {"name": "shared short", "op": "shared", "batch": 4, "queries": 1, "heads": 8, "kv_heads": 2, "dim": 64,
+        {"name": "shared short", "op": "shared", "prompts": 1, "batch": 4, "queries": 1, "heads": 8, "kv_heads": 2, "dim": 64,
          "page": 16, "prefix": 500, "longest": 100, "dtype": "bf16"},
         # a batch of chats behind one long instruction
-        {"name": "shared batch", "op": "shared", "batch": 64, "queries": 1, "heads": 32, "kv_heads": 8, "dim": 128,
-         "page": 16, "prefix": 8192, "longest": 1024, "dtype": "bf16"},
+        {"name": "shared batch", "op": "shared", "prompts": 1, "batch": 64, "queries": 1, "heads": 32, "kv_heads": 8,
+         "dim": 128, "page": 16, "prefix": 8192, "longest": 1024, "dtype": "bf16"},
         # questions about one long document
-        {"name": "shared long", "op": "shared", "batch": 16, "queries": 1, "heads": 64, "kv_heads": 8, "dim": 128,
-         "page": 64, "prefix": 131071, "longest": 300, "dtype": "bf16"},
+        {"name": "shared long", "op": "shared", "prompts": 1, "batch": 16, "queries": 1, "heads": 64, "kv_heads": 8,
+         "dim": 128, "page": 64, "prefix": 131071, "longest": 300, "dtype": "bf16"},
         # a large batch, drafted tokens to be verified: products of matrices
-        {"name": "shared drafted", "op": "shared", "batch": 128, "queries": 5, "heads": 32, "kv_heads": 8, "dim": 128,
-         "page": 32, "prefix": 4099, "longest": 700, "dtype": "bf16"},
-        # float32, a head per query head, pages that are no power of two
-        {"name": "shared f32", "op": "shared", "batch": 9, "queries": 1, "heads": 12, "kv_heads": 12, "dim": 80,
-         "page": 24, "prefix": 2050, "longest": 333, "dtype": "f32"},
+        {"name": "shared drafted", "op": "shared", "prompts": 1, "batch": 128, "queries": 5, "heads": 32, "kv_heads": 8,
+         "dim": 128, "page": 32, "prefix": 4099, "longest": 700, "dtype": "bf16"},
+        # three samples of each of three prompts; float32, a head per query head, pages that are no power of two
+        {"name": "shared f32", "op": "shared", "prompts": 3, "batch": 9, "queries": 1, "heads": 12, "kv_heads": 12,
+         "dim": 80, "page": 24, "prefix": 2050, "longest": 333, "dtype": "f32"},
         # one token through a small router
         {"name": "route one", "op": "route", "tokens": 1, "experts": 64, "k": 6, "score": "softmax", "bias": False,
          "groups": 1, "top_groups": 1, "group_score": "max", "renormalise": True, "dtype": "bf16"},
@@ -102,13 +102,16 @@ def draw(rng):
     c["queries"] = rng.choice([1, 1, 1, rng.randint(2, 9)])
     c["prefix"], c["longest"] = _log_int(rng, 33, 131071), _log_int(rng, 1, 4096)
     c["longest"] = max(c["longest"], c["queries"])
+    c["prompts"] = rng.choice([1, 1, 1, 2, 3, 8])
     size = c["dim"] * (1 if dtype == "bf16" else 4)
     while c["batch"] * c["queries"] * c["heads"] * (c["prefix"] + c["longest"]) * size > 16 * 64 * 131071 * 128 or \
-            c["batch"] * c["longest"] * c["kv_heads"] * size > 131071 * 8 * 128:
+            (c["batch"] * c["longest"] + c["prompts"] * c["prefix"]) * c["kv_heads"] * size > 131071 * 8 * 128:
         if c["batch"] > 1:
             c["batch"] //= 2
         else:
-            c["prefix"] = max(c["prefix"] // 2, 1)
+            c["prefix"], c["prompts"] = max(c["prefix"] // 2, 1), 1
+    c["prompts"] = min(c["prompts"], c["batch"])
+    c["batch"] -= c["batch"] % c["prompts"]
     return c
 
 
@@ -123,6 +126,10 @@ def _lens(c):
     if b >= 8 and c["op"] == "shared":
         lens[-1] = 0
     return lens
+
+
+def _prefix_lens(c):
+    return [c["prefix"] - c["prefix"] // 2 * i // c["prompts"] for i in range(c["prompts"])]
 
 
 def _randn(gen, shape, dtype, scale=1.0):
@@ -142,8 +149,9 @@ def prepare(case, seed):
     lens = torch.tensor(_lens(c), dtype=torch.int32, device="cuda")[order].contiguous()
     new = c["tokens"] if c["op"] == "rotate" else 0
     width = -(-(c["longest"] + new) // ps)
+    prompts = c["prompts"] if c["op"] == "shared" else 0
     front = -(-c["prefix"] // ps) if c["op"] == "shared" else 0
-    pages = b * width + front + 2
+    pages = b * width + prompts * front + 2
     perm = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)
     table = perm[:b * width].reshape(b, width)
     used = (lens + new + ps - 1) // ps
@@ -152,7 +160,11 @@ def prepare(case, seed):
     s["lens"] = lens
     if c["op"] == "shared":
         t = c["queries"]
-        s["prefix"], s["prefix_len"] = perm[b * width:b * width + front].clone(), c["prefix"]
+        begins = torch.tensor(_prefix_lens(c), dtype=torch.int32, device="cuda")
+        at = perm[b * width:b * width + prompts * front].reshape(prompts, front)
+        used = (begins + ps - 1) // ps
+        s["prefix"] = torch.where(torch.arange(front, device="cuda")[None] < used[:, None], at, -1).to(torch.int32)
+        s["prefix_lens"] = begins
         s["q"] = _randn(gen, (b, t, c["heads"], c["dim"]), c["dtype"], 2.0)
         s["scale"] = c["dim"] ** -0.5
         n = torch.randint(1, t + 1, (b,), generator=gen, device="cuda")  # some have fewer drafted tokens
@@ -202,8 +214,8 @@ def _run_own(s):
                                          interleaved=s["interleaved"])
         return s["k"], s["v"], lens, q
     if s["op"] == "shared":
-        return kvcache.decode_shared(s["q"], s["k"], s["v"], s["prefix"], s["prefix_len"], s["table"], s["lens"],
-                                     scale=s["scale"], counts=s["counts"])
+        return kvcache.decode_shared(s["q"], s["k"], s["v"], s["prefix"], s["prefix_lens"], s["table"],
+                                     s["lens"], scale=s["scale"], counts=s["counts"])
     return experts.route(s["logits"], s["k"], bias=s["bias"], **s["how"])
 
 
@@ -242,40 +254,39 @@ def _rotate(s):
     return s["k"], s["v"], (s["lens"] + t).clamp(max=table.shape[1] * ps), turned(q)
 
 
-def _shared(s):
-    """Softmax attention over the prefix, which all queries that count see, and each sequence's own slots."""
-    q, table = s["q"], s["table"]
-    b, t, hq, d = q.shape
-    pages, hkv, ps, _ = s["k"].shape
-    g = hq // hkv
-    counts = s["counts"]
-    step = torch.arange(t, device=q.device)
-    rows = q.float().reshape(b, t, hkv, g, d).permute(2, 0, 1, 3, 4)  # [hkv, b, t, g, d]
-    at = torch.arange(s["prefix_len"], device=q.device)
-    ids = s["prefix"].long()
-    there = ((ids >= 0) & (ids < pages))[at // ps]
-    kp, vp = (x[ids.clamp(0, pages - 1)[at // ps], :, at % ps].permute(1, 0, 2).float() for x in (s["k"], s["v"]))
-    x = ((rows.reshape(hkv, b * t * g, d) @ kp.transpose(-1, -2)) * s["scale"]).masked_fill(~there, -math.inf)
-    x = x.reshape(hkv, b, t * g, -1)
-
-    slot = torch.arange(table.shape[1] * ps, device=q.device)
+def _slots(s, table, lens, limit):
+    """Keys and values [hkv, rows of table, slots, d] in float32, and which slots each of limit [rows, n] sees."""
+    pages, _, ps, _ = s["k"].shape
+    slot = torch.arange(table.shape[1] * ps, device=table.device)
     page = table[:, slot // ps].long()
-    held = (page >= 0) & (page < pages)
+    held = (page >= 0) & (page < pages) & (slot < lens[:, None])
     page, off = page.clamp(0, pages - 1), slot % ps
-    ko, vo = (c[page, :, off].permute(2, 0, 1, 3).float() for c in (s["k"], s["v"]))  # [hkv, b, slots, d]
-    limit = torch.minimum(s["lens"][:, None] - counts[:, None] + step + 1, s["lens"][:, None])
-    seen = held[:, None] & (slot < limit[..., None])  # [b, t, slots]
-    seen = seen.repeat_interleave(g, 1)[None]
-    y = (rows.reshape(hkv, b, t * g, d) @ ko.transpose(-1, -2)) * s["scale"]
-    y = y.masked_fill(~seen, -math.inf)
+    k, v = (c[page, :, off].permute(2, 0, 1, 3).float() for c in (s["k"], s["v"]))
+    return k, v.masked_fill(~held[..., None], 0.0), held[:, None] & (slot < limit[..., None])
 
+
+def _shared(s):
+    """Softmax attention over a prefix, which all queries of its sequences see, and each sequence's own slots: query t
+    of counts[b] sees those below lens[b] - counts[b] + t + 1.  Sequences b of one prefix follow one another."""
+    q, lens, counts = s["q"], s["lens"], s["counts"]
+    b, t, hq, d = q.shape
+    hkv, prompts = s["k"].shape[1], s["prefix"].shape[0]
+    g = hq // hkv
+    step = torch.arange(t, device=q.device)
+    rows = q.float().reshape(b, t, hkv, g, d).permute(2, 0, 1, 3, 4).reshape(hkv, b, t * g, d)
+    whole = s["prefix_lens"][:, None]
+    kp, vp, seen = _slots(s, s["prefix"], s["prefix_lens"], whole)
+    x = (rows.reshape(hkv, prompts, -1, d) @ kp.transpose(-1, -2)) * s["scale"]
+    x = x.masked_fill(~seen, -math.inf).reshape(hkv, b, t * g, -1)
+    limit = torch.minimum(lens[:, None] - counts[:, None] + step + 1, lens[:, None])
+    ko, vo, seen = _slots(s, s["table"], lens, limit)
+    y = (rows @ ko.transpose(-1, -2)) * s["scale"]
+    y = y.masked_fill(~seen.repeat_interleave(g, 1)[None], -math.inf)
     top = torch.maximum(x.amax(-1, keepdim=True), y.amax(-1, keepdim=True))
     base = top.masked_fill(top == -math.inf, 0.0)
     x, y = (x - base).exp(), (y - base).exp()
     total = x.sum(-1, keepdim=True) + y.sum(-1, keepdim=True)
-    vp = vp.masked_fill(~there[:, None], 0.0)
-    vo = vo.masked_fill(~seen.any(2)[..., None], 0.0)
-    out = (x.reshape(hkv, b * t * g, -1) @ vp).reshape(hkv, b, t * g, d) + y @ vo
+    out = (x.reshape(hkv, prompts, b // prompts * t * g, -1) @ vp).reshape(hkv, b, t * g, d) + y @ vo
     out = out / total.masked_fill(total == 0, 1.0)
     lse = (top + total.log()).masked_fill(total == 0, -math.inf)
     none = (step >= counts[:, None]).repeat_interleave(g, 1)[None, ..., None]  # a query that does not count
@@ -322,9 +333,10 @@ def work(case):
         n = c["batch"] * c["tokens"]
         return {"bytes": 2 * n * (c["heads"] + 2 * c["kv_heads"]) * c["dim"] * es,
                 "flops": 6 * n * (c["heads"] + c["kv_heads"]) * c["pairs"]}
-    slots = c["prefix"] + sum(_lens(c))
+    begins = sum(_prefix_lens(c))
+    slots = begins + sum(_lens(c))
     rows = c["batch"] * c["queries"] * c["heads"]
-    flops = 4 * c["dim"] * c["queries"] * c["heads"] * (c["batch"] * c["prefix"] + sum(_lens(c)))
+    flops = 4 * c["dim"] * c["queries"] * c["heads"] * (c["batch"] // c["prompts"] * begins + sum(_lens(c)))
     return {"bytes": 2 * c["kv_heads"] * c["dim"] * es * slots + 2 * rows * c["dim"] * es + 4 * rows, "flops": flops}
 
 
@@ -362,13 +374,17 @@ def _exact_shared(s):
     """One sequence and kv head at a time, over its prefix and its own slots as one list."""
     b, t, hq, d = s["q"].shape
     _, hkv, ps, _ = s["k"].shape
-    g, p = hq // hkv, s["prefix_len"]
+    g, prompts = hq // hkv, s["prefix"].shape[0]
     out = torch.zeros((b, t, hq, d), dtype=torch.float64, device="cuda")
     lse = torch.full((b, t, hq), -math.inf, dtype=torch.float64, device="cuda")
-    lens, counts = s["lens"].tolist(), s["counts"].tolist()
+    lens, counts, begins = s["lens"].tolist(), s["counts"].tolist(), s["prefix_lens"].tolist()
     for h in range(hkv):
-        front = [x[s["prefix"].long(), h].reshape(-1, d)[:p].double() for x in (s["k"], s["v"])]
         for i, (n, c) in enumerate(zip(lens, counts)):
+            at = i // (b // prompts)
+            p = begins[at]
+            if i % (b // prompts) == 0:
+                ids = s["prefix"][at, :-(-p // ps)].long()
+                front = [x[ids, h].reshape(-1, d)[:p].double() for x in (s["k"], s["v"])]
             if c == 0:
                 continue
             ids = s["table"][i, :-(-n // ps)].long()
