@@ -365,6 +365,64 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
                      float* out_scores, void* workspace, size_t workspace_bytes, tallax_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * tallax_kv_append with the rotation of positions on the way.  q [batch,
+ * tokens, heads, dim], k, v [batch, tokens, kv_heads, dim], the cache's dtype,
+ * with element strides (of q, k and v in this order) for their first three
+ * axes, multiples of 16 bytes as their addresses are: parts of one
+ * projection's output fit.  Element pairs i < `pairs` of q and k, which are
+ * elements i and i + pairs, or 2i and 2i + 1 where `neighbours` is not 0, are
+ * turned by the angle a = p * frequencies[i] (float32, radians):
+ *   y0 = x0 cos a - x1 sin a,  y1 = x1 cos a + x0 sin a,
+ * in float32, rounded once; elements from 2 * pairs on are copied.  p is
+ * places[b][t][pair_axes[i]] (places [batch, tokens, axes] int32, pair_axes
+ * [pairs] int32, clamped to [0, axes); null: axis 0), or without places
+ * seen[b] + t (seen null: lens[b] + t).  Angles are computed in 64 bits.
+ * The turned keys and the values go to the cache as tallax_kv_append's do,
+ * the turned queries to out_q [batch, tokens, heads, dim] (dense), 0 for
+ * tokens from counts[b] on.  seen may be given without scores.
+ * ---------------------------------------------------------------------- */
+typedef struct tallax_kv_tokens {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t tokens, heads;
+  int64_t stride_batch[3], stride_token[3], stride_head[3];
+} tallax_kv_tokens;
+
+typedef struct tallax_rotation {
+  const float* frequencies;
+  int64_t pairs;
+  int32_t neighbours;
+  const int32_t* places;
+  int64_t axes;
+  const int32_t* pair_axes;
+} tallax_rotation;
+
+int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, const int32_t* counts,
+                             const tallax_kv_tokens* fresh, const tallax_rotation* turn, float* scores,
+                             int32_t* positions, const int32_t* seen, void* out_q, int32_t* out_lens,
+                             tallax_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * tallax_kv_decode (without scores) for sequences that begin with a shared
+ * prefix, whose keys and values are read once for all of them.  prefix_table
+ * [prefixes, prefix_width] int32 and prefix_lens [prefixes] int32 are a block
+ * table and lengths in the same pools; sequences b of prefix p are those with
+ * b / (batch / prefixes) = p.  Query t < counts[b] sees the whole prefix and
+ * what it sees in tallax_kv_decode of its sequence's own slots (block_table,
+ * lens); queries from counts[b] on see nothing.  max_prefix bounds prefix_lens
+ * as max_len bounds lens.  Workspace: tallax_kv_decode_shared_workspace_size
+ * bytes, on a multiple of 16.
+ * ---------------------------------------------------------------------- */
+size_t tallax_kv_decode_shared_workspace_size(const tallax_kv_cache* cache, int64_t prefixes, int64_t prefix_width,
+                                              int64_t queries, int64_t heads, int64_t max_prefix, int64_t max_len);
+int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_table, int64_t prefixes,
+                            int64_t prefix_width, const int32_t* prefix_lens, const void* q, int64_t q_stride_batch,
+                            int64_t q_stride_query, int64_t q_stride_head, int64_t queries, int64_t heads, double scale,
+                            const int32_t* lens, const int32_t* counts, int64_t max_prefix, int64_t max_len, void* out,
+                            float* out_lse, void* workspace, size_t workspace_bytes, tallax_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Eviction by accumulated attention weight: keeps new_len = min(lens[b],
  * budget) slots of every head.  Slots whose position is below `sinks` or at
  * least seen[b] - recent come first, then larger scores (NaN last), ties to
@@ -411,6 +469,29 @@ int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, in
                   int64_t vocab, const int32_t* counts, const float* temperature, const void* draft_probs,
                   int probs_dtype, const float* uniforms, const float* noise, int32_t* out_tokens,
                   int32_t* out_accepted, void* workspace, size_t workspace_bytes, tallax_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Routing tokens to experts.  NO COUNTERPART IN THE REFERENCE (its top-k picks
+ * from logits as they are).  logits [tokens, experts] f32/bf16, row stride in
+ * elements; score s = softmax over a token's experts (sigmoid 0) or
+ * 1 / (1 + exp(-logit)) (sigmoid 1); bias [experts] f32 or null is added for
+ * the choice only.  Experts are `groups` runs of experts / groups; the
+ * top_groups groups rank first by the largest s + bias in them (group_top 1)
+ * or the sum of the two largest (2), ties to the lowest group.  The k largest
+ * s + bias of those groups are chosen, in descending order, ties to the lowest
+ * expert; without a bias the choice is by the logits themselves.
+ *   weight = s * scale, with renormalise s / (sum of the chosen s) * scale (0
+ *   where that sum is 0).
+ * Scores that a choice hangs on are compared in 64 bits.  Experts whose logit
+ * is NaN or -inf, or whose bias is NaN, are not there: they score 0, add
+ * nothing to a group, and are chosen after all others of the chosen groups,
+ * lowest first, with weight 0.  +inf logits and infinite biases count as the
+ * largest finite ones.  experts up to 1024, groups up to 64, k up to 64 and to
+ * top_groups * experts / groups.  out_weights f32, out_ids int32 [tokens, k].
+ * ---------------------------------------------------------------------- */
+int tallax_route(const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t row_stride, int64_t k,
+                 int sigmoid, const float* bias, int64_t groups, int64_t top_groups, int group_top, int renormalise,
+                 double scale, float* out_weights, int32_t* out_ids, tallax_stream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

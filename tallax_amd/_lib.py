@@ -33,6 +33,18 @@ class KvCache(ctypes.Structure):
                 ("v_stride_slot", _c_i64), ("block_table", _c_p), ("batch", _c_i64), ("table_width", _c_i64)]
 
 
+class KvTokens(ctypes.Structure):
+    """tallax_kv_tokens of include/tallax_hip.h."""
+    _fields_ = [("q", _c_p), ("k", _c_p), ("v", _c_p), ("tokens", _c_i64), ("heads", _c_i64),
+                ("stride_batch", _c_i64 * 3), ("stride_token", _c_i64 * 3), ("stride_head", _c_i64 * 3)]
+
+
+class Rotation(ctypes.Structure):
+    """tallax_rotation of include/tallax_hip.h."""
+    _fields_ = [("frequencies", _c_p), ("pairs", _c_i64), ("neighbours", _c_i32), ("places", _c_p), ("axes", _c_i64),
+                ("pair_axes", _c_p)]
+
+
 _c_kv = ctypes.POINTER(KvCache)
 
 _SIGNATURES = {
@@ -72,6 +84,13 @@ _SIGNATURES = {
     "tallax_kv_decode_workspace_size": ([_c_kv, _c_i64, _c_i64, _c_i64, _c_int], _c_sz),
     "tallax_kv_decode": ([_c_kv, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_d, _c_p, _c_p, _c_i64, _c_p, _c_p,
                           _c_p, _c_p, _c_p, _c_sz, _c_p], _c_int),
+    "tallax_kv_append_rotated": ([_c_kv, _c_p, _c_p, ctypes.POINTER(KvTokens), ctypes.POINTER(Rotation), _c_p, _c_p, _c_p,
+                                  _c_p, _c_p, _c_p], _c_int),
+    "tallax_kv_decode_shared_workspace_size": ([_c_kv, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64], _c_sz),
+    "tallax_kv_decode_shared": ([_c_kv, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_d,
+                                 _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_sz, _c_p], _c_int),
+    "tallax_route": ([_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_int, _c_int, _c_d,
+                      _c_p, _c_p, _c_p], _c_int),
     "tallax_kv_evict_workspace_size": ([_c_kv, _c_i64], _c_sz),
     "tallax_kv_evict": ([_c_kv, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p],
                         _c_int),
@@ -204,7 +223,7 @@ def require_cuda(*ts: torch.Tensor) -> None:
 
 
 def _load_serving():
-    """The module behind kvcache and speculative: the same library, called without ctypes."""
+    """The module behind kvcache, speculative and experts: the same library, called without ctypes."""
     if not (_LIB_PATH.parent / "serving_ext.so").exists():
         raise ImportError(
             f"tallax_amd extension not built: {_LIB_PATH.parent / 'serving_ext.so'} is missing. "

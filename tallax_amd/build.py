@@ -39,6 +39,9 @@ SOURCES = [
     "sample_wide.hip",
     "kv_cache.hip",
     "kv_attention.hip",
+    "kv_rotate.hip",
+    "kv_shared.hip",
+    "route.hip",
     "verify.hip",
     "testing.hip",
 ]

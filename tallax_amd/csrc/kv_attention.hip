@@ -29,65 +29,12 @@
 // The length is split by max_len, which is the table's width unless the caller
 // knows a smaller bound: 4 sequences of up to 4096 slots with 8 kv heads take 16 us,
 // also in a table of 131072 slots with max_len 4096, and 54 there without it.
-#include <math.h>
-
-#include "tx_common.h"
-#include "tx_kv.h"
+#include "tx_attention.h"
 
 namespace tx {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef short bf16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.693147180559945309417f;
 constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = 4;
-
-struct AttnArgs {
-  KvView c;
-  const char* q;
-  int64_t q_batch, q_query, q_head;  // strides in bytes
-  const int32_t* lens;
-  const int32_t* counts;
-  char* out;
-  float* lse;
-  int queries, heads, kv_heads, group;  // group = heads / kv_heads
-  int rows;                             // queries * group
-  int max_len, chunk, chunks;
-  int row_groups;                       // workgroups that share a kv head's rows
-  int shift;                            // offsets in the pools are in units of 2^shift bytes
-  uint32_t k_page, k_slot, v_page, v_slot;
-  float scale2;                         // scale * log2 e
-  float2* part_ml;                      // [batch * kv_heads][chunks][rows]: maximum (base 2), sum
-  float* part_o;                        // [batch * kv_heads][chunks][rows][dim]
-  float* raw;                           // [batch * kv_heads][rows][raw_ld]: scores (base 2), or null
-  int raw_ld;
-  const float* scores;
-  float* out_scores;
-  int vector_scores;                    // their rows are whole 16-byte vectors
-};
-
-// What a sequence's rows see: row of query t sees slots below limit(t).
-struct Seen {
-  int len, cnt, first;  // first + t = limit of query t
-  __device__ __forceinline__ Seen(const AttnArgs& a, int b) {
-    len = min(max(a.lens[b], 0), a.max_len);
-    cnt = a.queries;
-    if (a.counts) cnt = min(max(a.counts[b], 0), a.queries);
-    first = len - cnt + 1;
-  }
-  __device__ __forceinline__ int limit(int t) const { return t < cnt ? min(first + t, len) : 0; }
-};
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // round to nearest even
-  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-  bf16x2_t r;
-  r[0] = (__bf16)lo;
-  r[1] = (__bf16)hi;
-  return __builtin_bit_cast(uint32_t, r);
-}
 
 __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
   return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
@@ -194,10 +141,6 @@ __device__ __forceinline__ int out_dim(int j, int r, int g) {
   return F32 ? 32 * (j / 2) + 2 * (4 * g + r) + (j & 1) : (DP / 16) * (4 * g + r) + j;
 }
 
-__device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
-  return (uint32_t)__builtin_amdgcn_ds_bpermute(lane << 2, (int)x);
-}
-
 // Every load of a tile is issued, in the same order, whatever there is to load:
 // waiting for one then does not mean waiting for those after it.  Elements past
 // dim are read from the token's first ones.
@@ -242,7 +185,7 @@ __device__ __forceinline__ void add_strange(const AttnArgs& a, const Seen& seen,
                                             const float* weights) {
 #pragma unroll 1
   for (int in = from; in < to; ++in) {
-    const char* p = vbase + ((uint64_t)from_lane(v_at, in) << a.shift);
+    const char* p = vbase + ((uint64_t)from_lane(v_at, in) << a.at.shift);
     if ((gone >> in) & 1) continue;
 #pragma unroll 1
     for (int d = lane_id(); d < a.c.dim; d += kWave) {
@@ -306,14 +249,14 @@ __global__ __launch_bounds__(kAttnThreads, WAVES) void kv_decode_kernel(AttnArgs
   };
   auto places_of = [&](int t, int page) {
     const int off = t + mine - (int)page_of(a.c.div, (uint32_t)(t + mine)) * a.c.div.size;
-    return Places{page, (uint32_t)page * a.k_page + (uint32_t)off * a.k_slot,
-                  (uint32_t)page * a.v_page + (uint32_t)off * a.v_slot};
+    return Places{page, (uint32_t)page * a.at.k_page + (uint32_t)off * a.at.k_slot,
+                  (uint32_t)page * a.at.v_page + (uint32_t)off * a.at.v_slot};
   };
   Keys<F32, DP> key;
   auto load_keys = [&](const Places& pl) {
 #pragma unroll
     for (int u = 0; u < T::kParts; ++u) {
-      const char* p = kbase + ((uint64_t)from_lane(pl.k, 16 * u + n) << a.shift);
+      const char* p = kbase + ((uint64_t)from_lane(pl.k, 16 * u + n) << a.at.shift);
       load_key<F32, DP>(key[u], (int)from_lane((uint32_t)pl.page, 16 * u + n) >= 0 ? p : safe, g, a.c.dim);
     }
   };
@@ -356,7 +299,7 @@ __global__ __launch_bounds__(kAttnThreads, WAVES) void kv_decode_kernel(AttnArgs
 #pragma unroll
     for (int j = 0; j < T::kValueTokens; ++j) {
       const int in = 16 * (j / 4) + 4 * g + (j & 3);
-      const char* p = vbase + ((uint64_t)from_lane(v_at, in) << a.shift);
+      const char* p = vbase + ((uint64_t)from_lane(v_at, in) << a.at.shift);
       load_value<F32, DP>(val[j], (gone >> in) & 1 ? safe : p, n, a.c.dim);
     }
     next = places_of(t0 + STEP, next_page);
@@ -693,13 +636,8 @@ __global__ __launch_bounds__(256) void kv_decode_join_kernel(AttnArgs a, int f32
   }
 }
 
-struct AttnPlan {
-  int mt, row_groups, chunk, chunks, max_len, rows, raw_ld;
-  size_t ml_bytes, o_bytes, raw_bytes;
-};
-
-static void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int dim, int dtype, int64_t max_len,
-                           bool with_scores, AttnPlan* p) {
+void plan_attention(int64_t batch, int64_t kv_heads, int64_t rows, int dim, int dtype, int64_t max_len, bool with_scores,
+                    AttnPlan* p) {
   const int tiles = (int)((rows + 15) / 16), most = dtype != TALLAX_F32 && dim > 128 ? 1 : 2;
   // 32 rows of a kv head to a workgroup, or 16: rows beyond are a workgroup of their own, which reads the keys and
   // values again.  Its registers cost more than that: with 64 rows of dim 128 and 32 of dim 256 (bfloat16) a SIMD
@@ -756,6 +694,30 @@ static int launch_decode(const AttnArgs& a, const AttnPlan& p, int64_t units, hi
   }
   return a.queries > 1 ? launch_decode_mt<F32, DP, 1, true>(a, p, units, s)
                        : launch_decode_mt<F32, DP, 1, false>(a, p, units, s);
+}
+
+int launch_attention(const AttnArgs& a, const AttnPlan& p, int64_t units, bool f32, hipStream_t s) {
+  if (a.c.dim <= 64) return f32 ? launch_decode<true, 64>(a, p, units, s) : launch_decode<false, 64>(a, p, units, s);
+  if (a.c.dim <= 128) return f32 ? launch_decode<true, 128>(a, p, units, s) : launch_decode<false, 128>(a, p, units, s);
+  return f32 ? launch_decode<true, 256>(a, p, units, s) : launch_decode<false, 256>(a, p, units, s);
+}
+
+int pool_offsets(const tallax_kv_cache* cache, const KvView& c, const char* what, PoolOffsets* out) {
+  uint64_t bits = 1 << 20;  // offsets in units of the largest power of two that the strides share
+  for (int64_t x : {c.k_page, c.k_slot, c.v_page, c.v_slot}) bits |= (uint64_t)x;
+  out->shift = __builtin_ctzll(bits);
+  const uint64_t far_page = cache->pages > 0 ? cache->pages - 1 : 0, far_slot = cache->page_size - 1;
+  if ((far_page * c.k_page + far_slot * c.k_slot) >> out->shift >> 32 ||
+      (far_page * c.v_page + far_slot * c.v_slot) >> out->shift >> 32) {
+    set_error("%s: a pool may span up to 2^32 times the largest power of two that divides its strides (%d bytes)", what,
+              1 << out->shift);
+    return kUnsupported;
+  }
+  out->k_page = (uint32_t)(c.k_page >> out->shift);
+  out->k_slot = (uint32_t)(c.k_slot >> out->shift);
+  out->v_page = (uint32_t)(c.v_page >> out->shift);
+  out->v_slot = (uint32_t)(c.v_slot >> out->shift);
+  return kOk;
 }
 
 }  // namespace tx
@@ -843,20 +805,8 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
   a.scores = scores;
   a.out_scores = out_scores;
   a.vector_scores = scores && a.c.capacity % 4 == 0 && !(((uintptr_t)scores | (uintptr_t)out_scores) & 15);
-  uint64_t bits = 1 << 20;  // offsets in units of the largest power of two that the strides share
-  for (int64_t x : {a.c.k_page, a.c.k_slot, a.c.v_page, a.c.v_slot}) bits |= (uint64_t)x;
-  a.shift = __builtin_ctzll(bits);
-  const uint64_t far_page = cache->pages > 0 ? cache->pages - 1 : 0, far_slot = cache->page_size - 1;
-  if ((far_page * a.c.k_page + far_slot * a.c.k_slot) >> a.shift >> 32 ||
-      (far_page * a.c.v_page + far_slot * a.c.v_slot) >> a.shift >> 32) {
-    set_error("kv_decode: a pool may span up to 2^32 times the largest power of two that divides its strides (%d bytes)",
-              1 << a.shift);
-    return kUnsupported;
-  }
-  a.k_page = (uint32_t)(a.c.k_page >> a.shift);
-  a.k_slot = (uint32_t)(a.c.k_slot >> a.shift);
-  a.v_page = (uint32_t)(a.c.v_page >> a.shift);
-  a.v_slot = (uint32_t)(a.c.v_slot >> a.shift);
+  st = pool_offsets(cache, a.c, "kv_decode", &a.at);
+  if (st != kOk) return st;
   const int64_t units = cache->batch * cache->kv_heads;
   if (units * p.row_groups > INT32_MAX || p.chunks > 65535) {
     set_error("kv_decode: too many workgroups");
@@ -864,12 +814,7 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
   }
   hipStream_t s = (hipStream_t)stream;
   const bool f32 = cache->dtype == TALLAX_F32;
-  if (a.c.dim <= 64)
-    st = f32 ? launch_decode<true, 64>(a, p, units, s) : launch_decode<false, 64>(a, p, units, s);
-  else if (a.c.dim <= 128)
-    st = f32 ? launch_decode<true, 128>(a, p, units, s) : launch_decode<false, 128>(a, p, units, s);
-  else
-    st = f32 ? launch_decode<true, 256>(a, p, units, s) : launch_decode<false, 256>(a, p, units, s);
+  st = launch_attention(a, p, units, f32, s);
   if (st != kOk) return st;
   const int out_blocks = p.chunks > 1 ? p.rows : 0;
   const int blocks = out_blocks + (scores ? (a.c.capacity + 1023) / 1024 : 0);

@@ -1,12 +1,12 @@
-// The serving calls (kvcache, speculative) between torch tensors and the C ABI.
+// The serving calls (kvcache, speculative, experts) between torch tensors and the C ABI.
 //
 // These calls are made once per decoded token, and at small batches the time of
 // a call is the host's: their checks, two to three allocations and one
 // foreign-function call of up to 20 arguments took 14 to 19 us in Python, the
 // kernels 5 to 10.  Here the same checks read the tensors directly.
 //
-// Every function takes positional arguments (the modules kvcache and
-// speculative hold the signatures and their documentation) and raises
+// Every function takes positional arguments (the modules kvcache,
+// speculative and experts hold the signatures and their documentation) and raises
 // ValueError, NotImplementedError or TallaxError as _lib.check does.
 #include <Python.h>
 
@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <cstring>
 #include <sstream>
 #include <stdexcept>
 
@@ -174,6 +175,16 @@ at::Tensor dense_16(const at::Tensor& t) {
   return on_16(c) ? c : c.clone();
 }
 
+// A tensor whose last axis is dense and whose address and strides are multiples of 16 bytes: t itself, or a copy.
+const at::Tensor& strided_16(const at::Tensor& t, at::Tensor& copy) {
+  const int64_t es = t.element_size();
+  bool fits = t.stride(t.dim() - 1) == 1 && on_16(t);
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) fits = fits && t.stride(i) * es % 16 == 0;
+  if (fits) return t;
+  copy = t.clone(at::MemoryFormat::Contiguous);
+  return copy;
+}
+
 tallax_stream_t stream_of(const c10::Device& d) { return c10::hip::getCurrentHIPStream(d.index()).stream(); }
 
 int64_t integer(PyObject* o) {
@@ -322,6 +333,116 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// k_pages, v_pages, block_table, lens, q, k_new, v_new, frequencies, token_positions, pair_axes, interleaved, counts,
+// scores, positions, seen
+PyObject* append_rotated(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arguments(n, 15);
+    Operands on;
+    const Cache c(on, a[0], a[1], a[2], a[3]);
+    const at::Tensor &lens = on.need(a[3]), &q_in = on.need(a[4]), &k_in = on.need(a[5]), &v_in = on.need(a[6]),
+                     &f_in = on.need(a[7]);
+    if (k_in.dim() != 4 || k_in.sizes() != v_in.sizes() || k_in.size(0) != c.c.batch ||
+        k_in.size(2) != c.c.kv_heads || k_in.size(3) != c.c.dim)
+      throw ValueError(text("k_new and v_new must be [", c.c.batch, ", tokens, ", c.c.kv_heads, ", ", c.c.dim,
+                            "], got ", shape_text(k_in.sizes()), " and ", shape_text(v_in.sizes())));
+    const int64_t tokens = k_in.size(1);
+    if (q_in.dim() != 4 || q_in.size(0) != c.c.batch || q_in.size(1) != tokens || q_in.size(3) != c.c.dim)
+      throw ValueError(text("q must be [", c.c.batch, ", ", tokens, ", heads, ", c.c.dim, "], got ",
+                            shape_text(q_in.sizes())));
+    if (q_in.scalar_type() != c.dtype || k_in.scalar_type() != c.dtype || v_in.scalar_type() != c.dtype)
+      throw ValueError(text("q, k_new and v_new must be ", c.dtype, ", as the cache"));
+    if (f_in.scalar_type() != at::kFloat || f_in.dim() != 1 || f_in.size(0) < 1 || 2 * f_in.size(0) > c.c.dim)
+      throw ValueError(text("frequencies must be float32 [pairs], 1 to ", c.c.dim / 2, " pairs, got ",
+                            f_in.scalar_type(), " ", shape_text(f_in.sizes())));
+    const int64_t pairs = f_in.size(0);
+    const at::Tensor *places = on.may(a[8]), *axes = on.may(a[9]);
+    int64_t n_axes = 1;
+    if (axes) {
+      if (!places) throw ValueError("pair_axes without token_positions");
+      if (axes->scalar_type() != at::kInt || axes->dim() != 1 || axes->size(0) != pairs)
+        throw ValueError(text("pair_axes must be an int32 tensor of shape (", pairs, ",)"));
+    }
+    if (places) {
+      const bool shaped = places->dim() == (axes ? 3 : 2) && places->size(0) == c.c.batch && places->size(1) == tokens;
+      if (!shaped || places->scalar_type() != at::kInt || (axes && places->size(2) < 1))
+        throw ValueError(text("token_positions must be an int32 tensor of shape (", c.c.batch, ", ", tokens,
+                              axes ? ", axes)" : ")", ", got ", places->scalar_type(), " ", shape_text(places->sizes())));
+      if (axes) n_axes = places->size(2);
+    }
+    const int neighbours = PyObject_IsTrue(a[10]);
+    if (neighbours < 0) throw Raised();
+    if ((a[12] == Py_None) != (a[13] == Py_None) || (a[12] != Py_None && a[14] == Py_None))
+      throw ValueError("scores, positions and seen go together");
+    const at::Tensor *counts = on.may(a[11]), *scores = on.may(a[12]), *positions = on.may(a[13]), *seen = on.may(a[14]);
+    if (scores) {
+      c.per_slot("scores", *scores, at::kFloat);
+      c.per_slot("positions", *positions, at::kInt);
+    }
+    if (seen) int_rows("seen", *seen, c.c.batch);
+    if (counts) int_rows("counts", *counts, c.c.batch);
+    const c10::DeviceGuard guard(on.device);
+    at::Tensor copies[3];
+    const at::Tensor* in[3] = {&strided_16(q_in, copies[0]), &strided_16(k_in, copies[1]), &strided_16(v_in, copies[2])};
+    const at::Tensor f = f_in.contiguous(), p = places ? places->contiguous() : at::Tensor(),
+                     ax = axes ? axes->contiguous() : at::Tensor();
+    at::Tensor out = at::empty(q_in.sizes(), q_in.options()), new_lens = at::empty_like(lens);
+    tallax_kv_tokens t{in[0]->data_ptr(), in[1]->data_ptr(), in[2]->data_ptr(), tokens, q_in.size(2), {}, {}, {}};
+    for (int i = 0; i < 3; ++i) {
+      t.stride_batch[i] = in[i]->stride(0);
+      t.stride_token[i] = in[i]->stride(1);
+      t.stride_head[i] = in[i]->stride(2);
+    }
+    const tallax_rotation r{static_cast<const float*>(f.data_ptr()), pairs, neighbours,
+                            places ? data<int32_t>(&p) : nullptr, n_axes, axes ? data<int32_t>(&ax) : nullptr};
+    check(tallax_kv_append_rotated(&c.c, data<int32_t>(&lens), data<int32_t>(counts), &t, &r, data<float>(scores),
+                                   data<int32_t>(positions), data<int32_t>(seen), out.data_ptr(),
+                                   data<int32_t>(&new_lens), stream_of(on.device)),
+          "kvcache.append_rotated");
+    PyObject *pl = THPVariable_Wrap(std::move(new_lens)), *po = THPVariable_Wrap(std::move(out));
+    return tuple_of({pl, po});
+  });
+}
+
+// q, k_pages, v_pages, prefix_table, prefix_lens, block_table, lens, scale, counts, max_prefix, max_len, workspace
+PyObject* decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arguments(n, 12);
+    Operands on;
+    const Cache c(on, a[1], a[2], a[5], a[6]);
+    const at::Tensor &lens = on.need(a[6]), &q_in = on.need(a[0]), &table = on.need(a[3]), &begins = on.need(a[4]);
+    if (q_in.dim() != 4 || q_in.size(0) != c.c.batch || q_in.size(3) != c.c.dim)
+      throw ValueError(text("q must be [", c.c.batch, ", queries, heads, ", c.c.dim, "], got ",
+                            shape_text(q_in.sizes())));
+    if (q_in.scalar_type() != c.dtype)
+      throw ValueError(text("q must be ", c.dtype, ", as the cache, got ", q_in.scalar_type()));
+    if (table.dim() != 2 || table.scalar_type() != at::kInt || !table.is_contiguous())
+      throw ValueError("prefix_table must be a contiguous int32 [prefixes, prefix_width] tensor");
+    const int64_t prefixes = table.size(0), width = table.size(1), queries = q_in.size(1), heads = q_in.size(2);
+    int_rows("prefix_lens", begins, prefixes);
+    const at::Tensor* counts = on.may(a[8]);
+    if (counts) int_rows("counts", *counts, c.c.batch);
+    const double scale = a[7] == Py_None ? 1.0 / std::sqrt(static_cast<double>(c.c.dim)) : real(a[7]);
+    const int64_t max_prefix = a[9] == Py_None ? width * c.c.page_size : integer(a[9]);
+    const int64_t max_len = a[10] == Py_None ? c.capacity() : integer(a[10]);
+    const c10::DeviceGuard guard(on.device);
+    at::Tensor copy;
+    const at::Tensor& q = strided_16(q_in, copy);
+    at::Tensor out = at::empty({c.c.batch, queries, heads, c.c.dim}, q.options());
+    at::Tensor lse = at::empty({c.c.batch, queries, heads}, lens.options().dtype(at::kFloat));
+    const size_t need =
+        tallax_kv_decode_shared_workspace_size(&c.c, prefixes, width, queries, heads, max_prefix, max_len);
+    const Workspace ws(a[11], on.device, need);
+    check(tallax_kv_decode_shared(&c.c, data<int32_t>(&table), prefixes, width, data<int32_t>(&begins), q.data_ptr(),
+                                  q.stride(0), q.stride(1), q.stride(2), queries, heads, scale, data<int32_t>(&lens),
+                                  data<int32_t>(counts), max_prefix, max_len, out.data_ptr(), data<float>(&lse), ws.at,
+                                  ws.bytes, stream_of(on.device)),
+          "kvcache.decode_shared");
+    PyObject *po = THPVariable_Wrap(std::move(out)), *pl = THPVariable_Wrap(std::move(lse));
+    return tuple_of({po, pl});
+  });
+}
+
 // k_pages, v_pages, block_table, lens, scores, positions, seen, budget, recent, sinks, workspace
 PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -410,6 +531,50 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// One of two names, as 0 or 1.
+int choice(const char* what, PyObject* o, const char* zero, const char* one) {
+  const char* s = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : nullptr;
+  if (PyErr_Occurred()) throw Raised();
+  if (s && !strcmp(s, zero)) return 0;
+  if (s && !strcmp(s, one)) return 1;
+  throw ValueError(text(what, " must be \"", zero, "\" or \"", one, "\""));
+}
+
+// logits, k, score, bias, groups, top_groups, group_score, renormalise, scale
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arguments(n, 9);
+    Operands on;
+    const at::Tensor& logits_in = on.need(a[0]);
+    if (logits_in.dim() != 2 || logits_in.size(1) < 1)
+      throw ValueError(text("logits must be [tokens, experts], got ", shape_text(logits_in.sizes())));
+    const int dt = dtype_code(logits_in);
+    if (dt == TALLAX_I32) throw Unsupported("route needs float logits");
+    const int64_t tokens = logits_in.size(0), experts = logits_in.size(1), k = integer(a[1]);
+    const int sigmoid = choice("score", a[2], "softmax", "sigmoid");
+    const at::Tensor* bias_in = on.may(a[3]);
+    if (bias_in) shaped("bias", *bias_in, {experts}, at::kFloat);
+    const int64_t groups = integer(a[4]), top_groups = a[5] == Py_None ? groups : integer(a[5]);
+    const int group_top = 1 + choice("group_score", a[6], "max", "top2");
+    const int renormalise = PyObject_IsTrue(a[7]);
+    if (renormalise < 0) throw Raised();
+    const double scale = real(a[8]);
+    const c10::DeviceGuard guard(on.device);
+    const bool rows = (experts == 1 || logits_in.stride(1) == 1) && logits_in.stride(0) >= 0;
+    const at::Tensor logits = rows ? logits_in : logits_in.contiguous(),
+                     bias = bias_in ? bias_in->contiguous() : at::Tensor();
+    if (tokens > 0 && k > 0 && k > (int64_t{1} << 40) / tokens) throw Unsupported(text("route: k = ", k));
+    at::Tensor weights = at::empty({tokens, k < 0 ? 0 : k}, logits.options().dtype(at::kFloat)),
+               ids = at::empty({tokens, k < 0 ? 0 : k}, logits.options().dtype(at::kInt));
+    check(tallax_route(logits.data_ptr(), dt, tokens, experts, logits.stride(0), k, sigmoid,
+                       bias_in ? data<float>(&bias) : nullptr, groups, top_groups, group_top, renormalise, scale,
+                       data<float>(&weights), data<int32_t>(&ids), stream_of(on.device)),
+          "experts.route");
+    PyObject *p0 = THPVariable_Wrap(std::move(weights)), *p1 = THPVariable_Wrap(std::move(ids));
+    return tuple_of({p0, p1});
+  });
+}
+
 // The error classes and what is called back: the workspace's and the per-row parameter's functions.
 PyObject* setup(PyObject*, PyObject* args) {
   PyObject** const to[4] = {&g_error, &g_out_of_memory, &g_workspace, &g_per_row};
@@ -429,9 +594,12 @@ PyCFunction method(F f) {
 }
 
 PyMethodDef methods[] = {{"append", method(append), METH_FASTCALL, nullptr},
+                         {"append_rotated", method(append_rotated), METH_FASTCALL, nullptr},
                          {"decode", method(decode), METH_FASTCALL, nullptr},
+                         {"decode_shared", method(decode_shared), METH_FASTCALL, nullptr},
                          {"evict", method(evict), METH_FASTCALL, nullptr},
                          {"verify", method(verify), METH_FASTCALL, nullptr},
+                         {"route", method(route), METH_FASTCALL, nullptr},
                          {"setup", setup, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 

@@ -1,9 +1,11 @@
-"""Paged key-value cache: appending tokens, the attention of the newest ones, and
+"""Paged key-value cache: appending tokens, with the rotation of their positions or
+without, the attention of the newest ones, also behind a shared prefix, and
 eviction by accumulated attention weight.
 
 No counterpart in the reference, which begins at the logits; these are the steps
 of a serving loop before them.  Every call runs hand-written gfx950 kernels
-(include/tallax_hip.h: tallax_kv_append, tallax_kv_decode, tallax_kv_evict).
+(include/tallax_hip.h: tallax_kv_append, tallax_kv_append_rotated,
+tallax_kv_decode, tallax_kv_decode_shared, tallax_kv_evict).
 
 A cache is two pools of pages k_pages, v_pages [pages, kv_heads, page_size, dim]
 (bfloat16 or float32; dim a multiple of 8 up to 256, contiguous; any strides of
@@ -40,6 +42,39 @@ def append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tens
     return _lib.SERVING.append(k_pages, v_pages, block_table, lens, k_new, v_new, counts, scores, positions, seen)
 
 
+def append_rotated(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                   q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, frequencies: torch.Tensor, *,
+                   token_positions: torch.Tensor | None = None, pair_axes: torch.Tensor | None = None,
+                   interleaved: bool = False, counts: torch.Tensor | None = None, scores: torch.Tensor | None = None,
+                   positions: torch.Tensor | None = None,
+                   seen: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """append, with queries and keys rotated by their tokens' positions.  Returns (new lens, rotated q).
+
+    q [batch, tokens, heads, dim] and k_new, v_new [batch, tokens, kv_heads,
+    dim] in the cache's dtype, any heads; parts of one projection's output are
+    read where they lie (strides and addresses of 16 bytes, else they are
+    copied first).  frequencies [pairs] float32, up to dim / 2 pairs: pair i of
+    a head's elements is (i, i + pairs), or (2i, 2i + 1) if interleaved, and
+    turns by the angle p * frequencies[i] (radians) of its token's position p:
+
+        y0 = x0 cos a - x1 sin a,    y1 = x1 cos a + x0 sin a
+
+    in float32 from angles in 64 bits, rounded once; elements past the pairs
+    are copied.
+
+    token_positions: int32 [batch, tokens], any value; the default is seen[b] +
+    t where seen is given, else lens[b] + t.  With pair_axes [pairs] int32 the
+    positions have several axes (time, height, width: [batch, tokens, axes]),
+    and pair i turns by that of axis pair_axes[i] (clamped to those there are).
+
+    Keys, values, counts, scores, positions and seen go as append's do; the
+    rotated q is a new dense tensor, 0 for tokens from counts[b] on.  Queries
+    of tokens whose keys are dropped are rotated all the same.
+    """
+    return _lib.SERVING.append_rotated(k_pages, v_pages, block_table, lens, q, k_new, v_new, frequencies,
+                                       token_positions, pair_axes, interleaved, counts, scores, positions, seen)
+
+
 def decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
            lens: torch.Tensor, *, scale: float | None = None, counts: torch.Tensor | None = None,
            scores: torch.Tensor | None = None, out_scores: torch.Tensor | None = None, max_len: int | None = None,
@@ -71,6 +106,33 @@ def decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_
                                workspace)
 
 
+def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, prefix_table: torch.Tensor,
+                  prefix_lens: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+                  scale: float | None = None, counts: torch.Tensor | None = None, max_prefix: int | None = None,
+                  max_len: int | None = None,
+                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """decode, for sequences that begin with a shared prefix, which is read once for all of them.
+
+    prefix_table [prefixes, prefix_width] int32 and prefix_lens [prefixes]
+    int32: the pages, in the same pools, and the slots of each prefix.  batch
+    is a multiple of prefixes, and the sequences of a prefix follow one
+    another: sequence b has prefix b // (batch // prefixes) (one prompt for
+    all, or several samples of each of several prompts).  block_table and lens
+    hold what each sequence has behind its prefix.
+
+    Query t of counts[b] sees its whole prefix and the slots that decode would
+    show it of its own; queries from counts[b] on see nothing.  A sequence may
+    have none of its own (lens 0, or a block_table of width 0).  Returns (out,
+    lse) as decode does, over both parts as one softmax.
+
+    max_prefix and max_len bound prefix_lens and lens (default: what the tables
+    can hold); larger lengths are taken as them, and both parts are split by
+    them.  workspace: as decode's.
+    """
+    return _lib.SERVING.decode_shared(q, k_pages, v_pages, prefix_table, prefix_lens, block_table, lens, scale, counts,
+                                      max_prefix, max_len, workspace)
+
+
 def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
           scores: torch.Tensor, positions: torch.Tensor, seen: torch.Tensor, *, budget: int, recent: int = 0,
           sinks: int = 0, workspace: torch.Tensor | None = None):
@@ -90,4 +152,4 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tenso
                               workspace)
 
 
-__all__ = ["append", "decode", "evict"]
+__all__ = ["append", "append_rotated", "decode", "decode_shared", "evict"]
