@@ -34,142 +34,168 @@ struct SharedArgs {
 };
 
 // Places of 16-byte vectors in a tile: vector c of a token's row is stored at
-// c ^ swizzle, so that the lanes of a read, which take the same vectors of
-// neighbouring tokens, meet different banks.
+// c ^ swizzle(token), so that the lanes of a read, which take the same vectors
+// of neighbouring tokens, meet different banks.  A swizzle is made of single
+// bits of the token, so that it may be taken of parts of a token's number.
 template <int VECS>
-__device__ __forceinline__ int key_place(int token, int c) {
-  return token * VECS + (c ^ (VECS >= 16 ? token & 15 : (token >> 1) & 7));
+__host__ __device__ constexpr int key_swizzle(int token) {
+  return VECS >= 16 ? token & 15 : (token >> 1) & 7;
 }
 
 template <bool F32, int VECS>
-__device__ __forceinline__ int value_place(int token, int c) {
-  if (F32) return token * VECS + (c ^ (8 * ((token >> 2) & 1)));
-  return token * VECS + (c ^ (VECS >= 16 ? 4 * (token & 3) : 4 * ((token >> 1) & 1)));
+__host__ __device__ constexpr int value_swizzle(int token) {
+  return F32 ? 8 * ((token >> 2) & 1) : VECS >= 16 ? 4 * (token & 3) : 4 * ((token >> 1) & 1);
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <class T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)(lds_char*)at;
 }
 
 template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
-__global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(SharedArgs a) {
-  constexpr int ES = F32 ? 4 : 2, NW = RG * TG, kThreads = NW * kWave;
-  constexpr int VECS = DP * ES / 16;               // 16-byte vectors of a token's key
-  constexpr int LOADS = WT * VECS / (kWave * RG);  // of a tile's keys, per lane
-  constexpr int QV = VECS / 2;                     // of a row's query, per lane
-  constexpr int NB = WT / 32, ACC = DP / 32, STEP = TG * WT, PAD = 36;
-  extern __shared__ uint4 tiles[];  // [2][TG][keys, values][WT * VECS]
+struct Prefix {
+  static constexpr int ES = F32 ? 4 : 2, NW = RG * TG, kThreads = NW * kWave;
+  static constexpr int VECS = DP * ES / 16;               // 16-byte vectors of a token's key
+  static constexpr int ROW = VECS * 16;
+  static constexpr int LOADS = WT * VECS / (kWave * RG);  // of a tile's keys, per lane
+  static constexpr int TPL = kWave / VECS;                // tokens of a load
+  static constexpr int QV = VECS / 2;                     // of a row's query, per lane
+  static constexpr int NB = WT / 32, ACC = DP / 32, STEP = TG * WT, PAD = 36;
+  static constexpr int kTile = 2 * WT * ROW;  // bytes of a tile: keys, then values
+  static constexpr int kRoom = 2 * TG * kTile, kJoin = NW * 32 * (8 + PAD * 4);
+  static constexpr int kBytes = kRoom > kJoin ? kRoom : kJoin;
+  static_assert(kBytes <= 160 * 1024, "LDS");
+  static_assert(VECS <= kWave && LOADS >= 1, "whole tokens in a load");
 
-  // The row tiles of a piece (chunk of a prefix's kv head) are workgroups of one XCD, that follow one another: their
-  // numbers are the same modulo 8.
-  const int step = blockIdx.x >> 3, piece = (step / a.row_tiles) * 8 + (blockIdx.x & 7);
-  if (piece >= a.pieces) return;
-  const int unit = piece / a.chunks, chunk = piece - unit * a.chunks;
-  const AttnArgs& o = a.own;
-  const int p = unit / o.kv_heads, kvh = unit - p * o.kv_heads;
-  const int len = min(max(a.lens[p], 0), a.max_len);
-  const int start = chunk * a.chunk;
-  if (start >= len) return;
-  const int end = min(start + a.chunk, len);
-  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), n = lane & 31, h = lane >> 5;
-  const int rg = wave % RG, tg = wave / RG;
-  const int row0 = (step % a.row_tiles) * 32 * RG + rg * 32;
-
-  const char* kbase = o.c.k + kvh * o.c.k_head;
-  const char* vbase = o.c.v + kvh * o.c.v_head;
-  const int32_t* table = a.table + (int64_t)p * a.width;
-  const char* safe = o.q;  // what is read in the place of a vector that is not there
-
-  uint4 ks[LOADS], vs[LOADS];
-  uint32_t holes = 0;  // bit j: vectors j of this lane are not there
-  uint64_t gone = 0, next_gone = 0;
-  auto load_tile = [&](int t0) {
-    const int t = t0 + (lane & (WT - 1));
-    const int page = t < end ? page_id(o.c, table, t) : -1;
-    const int off = t - (int)page_of(o.c.div, (uint32_t)t) * o.c.div.size;
-    const uint32_t k_at = (uint32_t)page * o.at.k_page + (uint32_t)off * o.at.k_slot;
-    const uint32_t v_at = (uint32_t)page * o.at.v_page + (uint32_t)off * o.at.v_slot;
-    next_gone = __ballot(page < 0);
-    holes = 0;
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int i = (rg * LOADS + j) * kWave + lane, token = i / VECS, c = i % VECS;
-      const char* pk = kbase + ((uint64_t)from_lane(k_at, token) << o.at.shift) + c * 16;
-      const char* pv = vbase + ((uint64_t)from_lane(v_at, token) << o.at.shift) + c * 16;
-      const bool hole = ((next_gone >> token) & 1) || c * 16 >= o.c.dim * ES;
-      holes |= (uint32_t)hole << j;
-      ks[j] = *(const uint4*)(hole ? safe : pk);
-      vs[j] = *(const uint4*)(hole ? safe : pv);
-    }
-  };
-  load_tile(start + tg * WT);
-
+  const SharedArgs& a;
+  int lane, n, h, end;
+  int source;           // lane that works out the place of this lane's token of a tile's first load
+  const char *kbase, *vbase;  // with this lane's vector of a token
+  const int32_t* table;
   uint4 q[QV];
-  {
-    const int row = row0 + n, seq = row / o.rows, rr = row - seq * o.rows, t = rr / o.group;
-    const char* at = o.q + (int64_t)(p * a.per + seq) * o.q_batch + t * o.q_query +
-                     (int64_t)(kvh * o.group + rr - t * o.group) * o.q_head;
-#pragma unroll
-    for (int i = 0; i < QV; ++i) {
-      const int c = 2 * i + h;
-      q[i] = make_uint4(0, 0, 0, 0);
-      if (row < a.rows && c * 16 < o.c.dim * ES) {
-        q[i] = *(const uint4*)(at + c * 16);
-        q[i] = make_uint4(q[i].x ^ a.flip, q[i].y ^ a.flip, q[i].z ^ a.flip, q[i].w ^ a.flip);
-      }
-    }
-  }
+  uint4 staged[2 * LOADS];  // of a tile on its way to LDS: keys and values in turn
   f32x16 acc[ACC];
-#pragma unroll
-  for (int j = 0; j < ACC; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[j][r] = 0.0f;
-  float m = -INFINITY, l = 0.0f;  // of q.k, which times scale2 is the exponent of a weight
+  float m, l;  // of q.k, which times scale2 is the exponent of a weight
 
-  const int rounds = (end - start + STEP - 1) / STEP;
-  for (int it = 0; it < rounds; ++it) {
-    const int t0 = start + it * STEP + tg * WT;
-    uint4* keys = tiles + ((it & 1) * TG + tg) * 2 * WT * VECS;
-    uint4* values = keys + WT * VECS;
-    gone = next_gone;
-    if (gone != 0 || DP != o.c.dim) {
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j)
-        if ((holes >> j) & 1) ks[j] = vs[j] = make_uint4(0, 0, 0, 0);
+  __device__ __forceinline__ explicit Prefix(const SharedArgs& args) : a(args) {}
+
+  // The table's entry of this lane's token of the tile at t0.
+  __device__ __forceinline__ int entry_at(int t0) const {
+    return table[page_of(a.own.c.div, (uint32_t)min(t0 + (lane & (WT - 1)), end - 1))];
+  }
+
+  // Where a tile's tokens lie: each lane works out the place of one token and
+  // hands it to those that load from it.  Tokens that are not there are read
+  // from the pool's first slot, and cleared on the way to LDS.
+  struct Places {
+    uint32_t k, v;
+    uint64_t gone;
+  };
+  __device__ __forceinline__ Places places_of(int t0, int entry) const {
+    const AttnArgs& o = a.own;
+    const int t = t0 + (lane & (WT - 1));
+    const bool there = (t < end) & ((uint32_t)entry < (uint32_t)o.c.pages);
+    const uint32_t off = (uint32_t)t - page_of(o.c.div, (uint32_t)t) * (uint32_t)o.c.div.size;
+    return Places{there ? (uint32_t)entry * o.at.k_page + off * o.at.k_slot : 0u,
+                  there ? (uint32_t)entry * o.at.v_page + off * o.at.v_slot : 0u, __ballot(!there)};
+  }
+
+  __device__ __forceinline__ uint32_t place(int i, const Places& at) const {
+    return from_lane(i & 1 ? at.v : at.k, source + i / 2 * TPL);
+  }
+
+  __device__ __forceinline__ void load(int i, uint32_t place) {
+    staged[i] = *(const uint4*)((i & 1 ? vbase : kbase) + ((uint64_t)place << a.own.at.shift));
+  }
+
+  // to: this lane's place of the first load in the tile's keys, or values.  What is not there must not be infinite or NaN
+  // in values, where its weight is 0, nor in what queries do not have; scores of tokens that are not there are masked.
+  __device__ __forceinline__ void store(int i, uint64_t gone, uint32_t to) const {
+    const int j = i / 2;
+    uint4 x = staged[i];
+    if (((i & 1) && gone != 0) || DP != a.own.c.dim) {
+      const int c = lane % VECS;
+      if (((gone >> (source + j * TPL)) & 1) || c * 16 >= a.own.c.dim * ES) x = make_uint4(0, 0, 0, 0);
     }
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int i = (rg * LOADS + j) * kWave + lane, token = i / VECS, c = i % VECS;
-      keys[key_place<VECS>(token, c)] = ks[j];
-      values[value_place<F32, VECS>(token, c)] = vs[j];
-    }
-    if (it + 1 < rounds) load_tile(t0 + STEP);
-    // One barrier a round: what is written in the next round was read in the last one, before this.
-    lds_barrier();
+    const int turn = i & 1 ? value_swizzle<F32, VECS>(j * TPL) : key_swizzle<VECS>(j * TPL);
+    *(__attribute__((address_space(3))) u32x4*)(lds_char*)((to ^ (turn << 4)) + j * TPL * ROW) = __builtin_bit_cast(u32x4, x);
+  }
+
+  // One tile's keys and values into this wave's rows.  Meanwhile the next tile
+  // goes from registers to LDS and the one after it is asked for, a vector at a
+  // time between the products: loads that are asked for all at once hold a wave
+  // up until the memory has taken them.
+  // keys, values: this lane's first places in the tile that is read; next_k, next_v: in the one that is written
+  __device__ __forceinline__ void round(uint32_t keys, uint32_t values, uint32_t next_k, uint32_t next_v, uint64_t gone,
+                                        uint64_t next_gone, const Places& after) {
     f32x16 s[NB];
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[u][r] = 0.0f;
+    // Vectors are read a group of products ahead: a read's way through LDS takes longer than a product.
+    constexpr int GROUP = 4 / NB < QV ? 4 / NB : QV;
+    constexpr int JG = ACC < 4 ? ACC : 4, STEPS = F32 ? 4 * NB : 2 * NB * (ACC / JG), SLOTS = QV / GROUP + STEPS;
+    // A place is handed over in the slot before its load: it comes through LDS, behind the reads that were made before.
+    constexpr int EACH = (2 * LOADS + SLOTS - 1) / SLOTS;
+    uint32_t places[2][EACH];
+    auto hand_over = [&](int slot) {
 #pragma unroll
-    for (int i = 0; i < QV; ++i) {
+      for (int i = 0; i < 2 * LOADS; ++i)
+        if (i / EACH == slot) places[slot & 1][i % EACH] = place(i, after);
+    };
+    auto pass_on = [&](int slot) {
 #pragma unroll
-      for (int u = 0; u < NB; ++u) {
-        const uint4 k = keys[key_place<VECS>(32 * u + n, 2 * i + h)];
-        if constexpr (F32) {
-          s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.x), __uint_as_float(q[i].x), s[u], 0, 0, 0);
-          s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.y), __uint_as_float(q[i].y), s[u], 0, 0, 0);
-          s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.z), __uint_as_float(q[i].z), s[u], 0, 0, 0);
-          s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.w), __uint_as_float(q[i].w), s[u], 0, 0, 0);
-        } else {
-          s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k),
-                                                         __builtin_bit_cast(bf16x8_t, q[i]), s[u], 0, 0, 0);
-        }
+      for (int i = 0; i < 2 * LOADS; ++i) {
+        if (i / EACH != slot) continue;
+        store(i, next_gone, i & 1 ? next_v : next_k);
+        load(i, places[slot & 1][i % EACH]);
       }
+    };
+    hand_over(0);
+    uint4 kv[2][GROUP][NB];
+    auto read_keys = [&](int g) {
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i)
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+          kv[g & 1][i][u] = __builtin_bit_cast(uint4, lds_read<u32x4>((keys ^ (2 * (g * GROUP + i) << 4)) + 32 * u * ROW));
+    };
+    read_keys(0);
+#pragma unroll
+    for (int g = 0; g < QV / GROUP; ++g) {
+      hand_over(g + 1);
+      if (g + 1 < QV / GROUP) read_keys(g + 1);
+      pass_on(g);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i)
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+          const uint4 k = kv[g & 1][i][u], x = q[g * GROUP + i];
+          if constexpr (F32) {
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.x), __uint_as_float(x.x), s[u], 0, 0, 0);
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.y), __uint_as_float(x.y), s[u], 0, 0, 0);
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.z), __uint_as_float(x.z), s[u], 0, 0, 0);
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.w), __uint_as_float(x.w), s[u], 0, 0, 0);
+          } else {
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k),
+                                                           __builtin_bit_cast(bf16x8_t, x), s[u], 0, 0, 0);
+          }
+        }
+      __builtin_amdgcn_sched_barrier(0);
     }
     // lane (n, h) holds row n's scores of tokens 32 u + 8 (r / 4) + 4 h + r % 4
     if (gone != 0) {
 #pragma unroll
-      for (int u = 0; u < NB; ++u)
+      for (int u = 0; u < NB; ++u) {
+        const uint32_t here = (uint32_t)(gone >> (32 * u)) >> (4 * h);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if ((gone >> (32 * u + 8 * (r / 4) + 4 * h + r % 4)) & 1) s[u][r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) s[u][r] = (here >> (8 * (r / 4) + r % 4)) & 1 ? -INFINITY : s[u][r];
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -196,45 +222,149 @@ __global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(Share
       }
     l += sum;
     if constexpr (F32) {
-      const float* v = (const float*)values;
 #pragma unroll
       for (int u = 0; u < NB; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-          for (int j = 0; j < ACC; ++j) {
-            const int token = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
-            acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[value_place<true, VECS>(token, 8 * j + n / 4) * 4 + n % 4],
-                                                          s[u][r], acc[j], 0, 0, 0);
+        for (int r = 0; r < 16; ++r) {
+          if (r % 4 == 0) {
+            hand_over(QV / GROUP + 4 * u + r / 4 + 1);
+            pass_on(QV / GROUP + 4 * u + r / 4);
           }
+#pragma unroll
+          for (int j = 0; j < ACC; ++j)
+            acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                lds_read<float>((values ^ (8 * j << 4)) + (32 * u + 8 * (r / 4) + r % 4) * ROW), s[u][r], acc[j], 0, 0, 0);
+        }
     } else {
       // The product takes both sides in bfloat16: the weights, at most 1, are rounded to it (by 2^-8 of each at most);
       // their sum, by which the output is divided, is of the unrounded ones.
+      uint2 vv[2][JG][2];
+      auto read_values = [&](int i) {  // of 16 tokens and 32 JG elements
+        typedef __attribute__((address_space(3))) bf16x4 lds_x4;
+        // 16 lanes read 16 neighbouring elements of four tokens, and get four tokens of one element each
 #pragma unroll
-      for (int u = 0; u < NB; ++u)
+        for (int j = 0; j < JG; ++j)
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          uint32_t w[4];
+          for (int half = 0; half < 2; ++half)
+            vv[i & 1][j][half] = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (lds_x4*)(lds_char*)((values ^ (4 * (i % (ACC / JG) * JG + j) << 4)) +
+                                                (16 * (i / (ACC / JG)) + 8 * half) * ROW)));
+      };
+      read_values(0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = pack_bf16(s[u][8 * kk + 2 * i], s[u][8 * kk + 2 * i + 1]);
-          const bf16x8_t weights = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+      for (int i = 0; i < STEPS; ++i) {
+        hand_over(QV / GROUP + i + 1);
+        if (i + 1 < STEPS) read_values(i + 1);
+        pass_on(QV / GROUP + i);
+        const int u = i / (ACC / JG) / 2, r = 8 * (i / (ACC / JG) % 2);
+        uint32_t w[4];
 #pragma unroll
-          for (int j = 0; j < ACC; ++j) {
-            // 16 lanes read 16 neighbouring elements of four tokens, and get four tokens of one element each
-            typedef __attribute__((address_space(3))) bf16x4 lds_x4;
-            const int token = 32 * u + 16 * kk + 4 * h + (lane & 15) / 4;
-            const int c = 4 * j + 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
-            const char* lo = (const char*)(values + value_place<false, VECS>(token, c)) + (lane & 1) * 8;
-            const char* hi = (const char*)(values + value_place<false, VECS>(token + 8, c)) + (lane & 1) * 8;
-            const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4*)lo);
-            const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_x4*)hi);
-            const uint2 xu = __builtin_bit_cast(uint2, x), yu = __builtin_bit_cast(uint2, y);
-            acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                __builtin_bit_cast(bf16x8_t, make_uint4(xu.x, xu.y, yu.x, yu.y)), weights, acc[j], 0, 0, 0);
-          }
+        for (int k = 0; k < 4; ++k) w[k] = pack_bf16(s[u][r + 2 * k], s[u][r + 2 * k + 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < JG; ++j) {
+          f32x16& to = acc[i % (ACC / JG) * JG + j];
+          to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8_t, make_uint4(vv[i & 1][j][0].x, vv[i & 1][j][0].y, vv[i & 1][j][1].x, vv[i & 1][j][1].y)),
+              __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3])), to, 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
+};
+
+template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
+__global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(SharedArgs a) {
+  using P = Prefix<F32, DP, RG, TG, WT, WAVES>;
+  constexpr int NW = P::NW, PAD = P::PAD, STEP = P::STEP;
+  extern __shared__ __attribute__((aligned(1024))) uint4 tiles[];  // [2][TG][keys, values][WT * VECS]
+
+  // The row tiles of a piece (chunk of a prefix's kv head) are workgroups of one XCD, that follow one another: their
+  // numbers are the same modulo 8.
+  const int step = blockIdx.x >> 3, piece = (step / a.row_tiles) * 8 + (blockIdx.x & 7);
+  if (piece >= a.pieces) return;
+  const int unit = piece / a.chunks, chunk = piece - unit * a.chunks;
+  const AttnArgs& o = a.own;
+  const int p = unit / o.kv_heads, kvh = unit - p * o.kv_heads;
+  const int len = min(max(a.lens[p], 0), a.max_len);
+  const int start = chunk * a.chunk;
+  if (start >= len) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), tg = wave / RG;
+  P w(a);
+  const int rg = wave % RG;
+  w.lane = lane_id();
+  w.n = w.lane & 31;
+  w.h = w.lane >> 5;
+  w.end = min(start + a.chunk, len);
+  w.source = rg * P::LOADS * P::TPL + w.lane / P::VECS;
+  const int c0 = w.lane % P::VECS, c = c0 * 16 < o.c.dim * P::ES ? c0 : 0;  // vectors past dim are cleared too
+  w.kbase = o.c.k + kvh * o.c.k_head + c * 16;
+  w.vbase = o.c.v + kvh * o.c.v_head + c * 16;
+  w.table = a.table + (int64_t)p * a.width;
+  const int n = w.n, h = w.h, row0 = (step % a.row_tiles) * 32 * RG + rg * 32;
+
+  // this lane's first places in the first of two tiles; the other is TG * kTile away
+  const uint32_t keys = (uint32_t)(uintptr_t)(lds_char*)(char*)tiles + tg * P::kTile, values = keys + WT * P::ROW;
+  const uint32_t put_k = keys + w.source * P::ROW + ((c0 ^ key_swizzle<P::VECS>(w.source)) << 4);
+  const uint32_t put_v = values + w.source * P::ROW + ((c0 ^ value_swizzle<F32, P::VECS>(w.source)) << 4);
+  const uint32_t get_k = keys + n * P::ROW + ((h ^ key_swizzle<P::VECS>(n)) << 4);
+  // bfloat16: token 4 h + (lane % 16) / 4, 8 bytes of its elements each; float32: token 4 h, an element each
+  const int first = F32 ? 4 * h : 4 * h + (w.lane & 15) / 4;
+  const int vec = F32 ? n / 4 : 2 * ((w.lane >> 4) & 1) + (w.lane & 3) / 2;
+  const uint32_t get_v = values + first * P::ROW + ((vec ^ value_swizzle<F32, P::VECS>(first)) << 4) +
+                         (F32 ? n % 4 * 4 : (w.lane & 1) * 8);
+
+  int t0 = start + tg * WT;
+  typename P::Places at = w.places_of(t0, w.entry_at(t0));
+#pragma unroll
+  for (int i = 0; i < 2 * P::LOADS; ++i) w.load(i, w.place(i, at));
+  int entry = w.entry_at(t0 + STEP);
+  {
+    const int row = row0 + n, seq = row / o.rows, rr = row - seq * o.rows, t = rr / o.group;
+    const char* at = o.q + (int64_t)(p * a.per + seq) * o.q_batch + t * o.q_query +
+                     (int64_t)(kvh * o.group + rr - t * o.group) * o.q_head;
+#pragma unroll
+    for (int i = 0; i < P::QV; ++i) {
+      const int c = 2 * i + h;
+      w.q[i] = make_uint4(0, 0, 0, 0);
+      if (row < a.rows && c * 16 < o.c.dim * P::ES) {
+        const uint4 x = *(const uint4*)(at + c * 16);
+        w.q[i] = make_uint4(x.x ^ a.flip, x.y ^ a.flip, x.z ^ a.flip, x.w ^ a.flip);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < P::ACC; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w.acc[j][r] = 0.0f;
+  w.m = -INFINITY;
+  w.l = 0.0f;
+
+  const int rounds = (w.end - start + STEP - 1) / STEP;
+  uint64_t gone = at.gone;
+  at = w.places_of(t0 + STEP, entry);
+  entry = w.entry_at(t0 + 2 * STEP);
+#pragma unroll
+  for (int i = 0; i < 2 * P::LOADS; ++i) {
+    w.store(i, gone, i & 1 ? put_v : put_k);
+    w.load(i, w.place(i, at));
+  }
+#pragma unroll 1
+  for (int it = 0; it < rounds; ++it, t0 += STEP) {
+    // One barrier a round: the tile that is written in it was read in the round before.
+    lds_barrier();
+    const uint64_t next_gone = at.gone;
+    at = w.places_of(t0 + 2 * STEP, entry);
+    entry = w.entry_at(t0 + 3 * STEP);
+    const uint32_t here = (it & 1) * TG * P::kTile, there = TG * P::kTile - here;
+    w.round(get_k + here, get_v + here, put_k + there, put_v + there, gone, next_gone, at);
+    gone = next_gone;
+  }
+  f32x16(&acc)[P::ACC] = w.acc;
+  const float m = w.m;
+  float l = w.l;
   // join the token groups, 32 elements of the outputs at a time
   l += lane_xor_f(l, 32);
   const float m2 = m == -INFINITY ? m : m * a.scale2;
@@ -259,9 +389,9 @@ __global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(Share
     a.part_ml[out + row0 + n] = make_float2(all, total);
   }
   const bool none = m2 == -INFINITY;
-  const int first = (step % a.row_tiles) * 32 * RG;
+  const int row1 = (step % a.row_tiles) * 32 * RG;
 #pragma unroll
-  for (int j = 0; j < ACC; ++j) {
+  for (int j = 0; j < P::ACC; ++j) {
     float* mo = sums + (wave * 32 + n) * PAD;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -271,9 +401,9 @@ __global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(Share
       *(float4*)(mo + 8 * i + 4 * h) = x;
     }
     __syncthreads();
-    for (int i = tid; i < RG * 32 * 8; i += kThreads) {
+    for (int i = tid; i < RG * 32 * 8; i += P::kThreads) {
       const int row = i / 8, d = 32 * j + i % 8 * 4;
-      if (first + row >= a.rows || d >= o.c.dim) continue;
+      if (row1 + row >= a.rows || d >= o.c.dim) continue;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < TG; ++k) {
@@ -283,7 +413,7 @@ __global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(Share
         x.z += y.z;
         x.w += y.w;
       }
-      *(float4*)(a.part_o + (out + first + row) * o.c.dim + d) = x;
+      *(float4*)(a.part_o + (out + row1 + row) * o.c.dim + d) = x;
     }
     __syncthreads();
   }
@@ -369,16 +499,30 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t rows
   const bool f32 = c->dtype == TALLAX_F32;
   const int64_t all = c->batch / prefixes * rows, units = prefixes * c->kv_heads;
   p->rg = all <= 32 && !(f32 && c->dim > 128) ? 1 : all <= 64 ? 2 : 4;
-  const int tg = c->dim > 128 ? (f32 || p->rg == 4 ? 1 : 2) : f32 ? (c->dim > 64 ? 2 : p->rg == 4 ? 2 : 4) : p->rg == 4 ? 2 : 4;
-  const int wt = !f32 && c->dim <= 128 && p->rg == 4 ? 64 : 32;
+  const int tg = c->dim > 128 ? (f32 || p->rg == 4 ? 1 : 2) : f32 ? (c->dim > 64 ? 2 : p->rg == 4 ? 2 : 4) : p->rg == 4 ? 1 : p->rg == 2 ? 2 : 4;
+  const int wt = !f32 && c->dim <= 128 && p->rg >= 2 ? 64 : 32;
+  const int places = !f32 && c->dim <= 128 ? (p->rg == 4 ? 512 : p->rg == 2 ? 256 : 256) : 256;
   p->step = tg * wt;
   p->row_tiles = (int)((all + 32 * p->rg - 1) / (32 * p->rg));
-  int64_t chunk = (max_prefix * units * p->row_tiles + 255) / 256;
-  if (chunk < p->step) chunk = p->step;
-  chunk = (chunk + p->step - 1) / p->step * p->step;
-  p->chunk = (int)chunk;
-  p->chunks = (int)((max_prefix + chunk - 1) / chunk);
-  if (p->chunks < 1) p->chunks = 1;
+  // Chunks, so that the workgroups take whole rounds of the card's 256 places: of one to four rounds that which leaves
+  // the fewest steps one after another, each round with some six more for its beginning and end.
+  const int64_t steps = (max_prefix + p->step - 1) / p->step, pieces = units * p->row_tiles;
+  int64_t best = INT64_MAX;
+  p->chunks = 1;
+  p->chunk = (int)(steps > 0 ? steps : 1) * p->step;
+  for (int rounds = 1; rounds <= 4; ++rounds) {
+    int64_t n = places * rounds / pieces;
+    if (n < 1) n = 1;
+    if (n > steps) n = steps;
+    if (n < 1) break;
+    const int64_t each = (steps + n - 1) / n;
+    const int64_t turns = (pieces * n + places - 1) / places, cost = turns * (each + 6);
+    if (cost < best) {
+      best = cost;
+      p->chunk = (int)(each * p->step);
+      p->chunks = (int)((steps + each - 1) / each);
+    }
+  }
   plan_attention(c->batch, c->kv_heads, rows, c->dim, c->dtype, max_len, false, &p->own);
   p->own_chunks = p->own.chunks > 1 ? p->own.chunks : 2;  // with one the kernel would write outputs, not parts
   p->ml_bytes = align_up((size_t)(units * p->chunks * all) * sizeof(float2), 256);
@@ -390,22 +534,20 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t rows
 
 template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
 static int launch_prefix(const SharedArgs& a, int step, hipStream_t s) {
-  if (step != TG * WT) {  // the plan and the instance must agree
+  using P = Prefix<F32, DP, RG, TG, WT, WAVES>;
+  if (step != P::STEP) {  // the plan and the instance must agree
     set_error("kv_decode_shared: no kernel for steps of %d", step);
     return kUnsupported;
   }
-  constexpr int kTiles = 2 * TG * 2 * WT * DP * (F32 ? 4 : 2), kJoin = RG * TG * 32 * (8 + 36 * 4);
-  constexpr int kBytes = kTiles > kJoin ? kTiles : kJoin;
-  static_assert(kBytes <= 160 * 1024, "LDS");
-  if (kBytes > 48 * 1024) {
-    const hipError_t e = set_dynamic_lds_limit((const void*)kv_prefix_kernel<F32, DP, RG, TG, WT, WAVES>, kBytes, s);
+  if (P::kBytes > 48 * 1024) {
+    const hipError_t e = set_dynamic_lds_limit((const void*)kv_prefix_kernel<F32, DP, RG, TG, WT, WAVES>, P::kBytes, s);
     if (e != hipSuccess) {
       set_error("kv_decode_shared: %s", hipGetErrorString(e));
       return kHipError;
     }
   }
   const unsigned grid = (unsigned)((a.pieces + 7) / 8 * 8) * (unsigned)a.row_tiles;
-  kv_prefix_kernel<F32, DP, RG, TG, WT, WAVES><<<grid, RG * TG * kWave, kBytes, s>>>(a);
+  kv_prefix_kernel<F32, DP, RG, TG, WT, WAVES><<<grid, P::kThreads, P::kBytes, s>>>(a);
   return launch_status("kv_decode_shared");
 }
 
@@ -424,12 +566,12 @@ static int launch_prefix_any(const SharedArgs& a, int rg, int step, bool f32, hi
   }
   if (dim <= 64)
     return rg == 1   ? launch_prefix<false, 64, 1, 4, 32, 1>(a, step, s)
-           : rg == 2 ? launch_prefix<false, 64, 2, 4, 32, 2>(a, step, s)
-                     : launch_prefix<false, 64, 4, 2, 64, 2>(a, step, s);
+           : rg == 2 ? launch_prefix<false, 64, 2, 2, 64, 1>(a, step, s)
+                     : launch_prefix<false, 64, 4, 1, 64, 2>(a, step, s);
   if (dim <= 128)
     return rg == 1   ? launch_prefix<false, 128, 1, 4, 32, 1>(a, step, s)
-           : rg == 2 ? launch_prefix<false, 128, 2, 4, 32, 2>(a, step, s)
-                     : launch_prefix<false, 128, 4, 2, 64, 2>(a, step, s);
+           : rg == 2 ? launch_prefix<false, 128, 2, 2, 64, 1>(a, step, s)
+                     : launch_prefix<false, 128, 4, 1, 64, 2>(a, step, s);
   return rg == 1   ? launch_prefix<false, 256, 1, 2, 32, 1>(a, step, s)
          : rg == 2 ? launch_prefix<false, 256, 2, 2, 32, 1>(a, step, s)
                    : launch_prefix<false, 256, 4, 1, 32, 1>(a, step, s);
@@ -546,7 +688,7 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
   a.table = prefix_table;
   a.lens = prefix_lens;
   a.width = (int)prefix_width;
-  a.max_len = (int)max_prefix;
+  a.max_len = cache->pages > 0 ? (int)max_prefix : 0;  // without a page there is nothing to see, nor to read
   a.per = (int)(cache->batch / prefixes);
   a.rows = (int)(a.per * rows);
   a.row_tiles = p.row_tiles;
@@ -557,7 +699,7 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
   a.scale2 = fmaxf(fabsf(o.scale2), 1.1754944e-38f);
   hipStream_t s = (hipStream_t)stream;
   const bool f32 = cache->dtype == TALLAX_F32;
-  if (max_prefix > 0) {
+  if (a.max_len > 0) {
     st = launch_prefix_any(a, p.rg, p.step, f32, s);
     if (st != kOk) return st;
   }
