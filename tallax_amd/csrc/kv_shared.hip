@@ -13,7 +13,7 @@
 // weights are the second operand of the second product as they lie; its first
 // operand, values by dim, is read transposed from LDS (bfloat16), or in single
 // elements (float32).
-#include "tx_attention.h"
+#include "tx_decode.h"
 
 namespace tx {
 
@@ -26,7 +26,9 @@ struct SharedArgs {
   int width, max_len;
   int per;               // sequences of a prefix
   int rows;              // of a prefix's kv head
-  int row_tiles, chunk, chunks, pieces;
+  int row_tiles, chunk, chunks;
+  int pieces;            // chunks of all kv heads of all prefixes
+  int own_units;         // workgroups of a chunk of the sequences' own slots
   uint32_t flip;         // sign bits of q, where the scale is negative
   float scale2;          // its size, above 0: -inf, of what is not seen, stays -inf
   float2* part_ml;       // [prefixes * kv_heads][chunks][rows]: maximum (base 2), sum
@@ -275,15 +277,15 @@ struct Prefix {
   }
 };
 
+// Rows 32 RG times the tile's number and on of a prefix's kv head, over one chunk: workgroup f of those for prefixes.
 template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
-__global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(SharedArgs a) {
+__device__ __forceinline__ void prefix_chunk(const SharedArgs& a, int f, uint4* tiles) {
   using P = Prefix<F32, DP, RG, TG, WT, WAVES>;
   constexpr int NW = P::NW, PAD = P::PAD, STEP = P::STEP;
-  extern __shared__ __attribute__((aligned(1024))) uint4 tiles[];  // [2][TG][keys, values][WT * VECS]
 
   // The row tiles of a piece (chunk of a prefix's kv head) are workgroups of one XCD, that follow one another: their
   // numbers are the same modulo 8.
-  const int step = blockIdx.x >> 3, piece = (step / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int step = f >> 3, piece = (step / a.row_tiles) * 8 + (f & 7);
   if (piece >= a.pieces) return;
   const int unit = piece / a.chunks, chunk = piece - unit * a.chunks;
   const AttnArgs& o = a.own;
@@ -419,6 +421,55 @@ __global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_prefix_kernel(Share
   }
 }
 
+// A prefix's slots, as its sequences' rows see them: all of them.
+struct PrefixRows {
+  static constexpr bool kOutputs = false;
+  const SharedArgs& a;
+  int unit, p, kvh, length;
+  __device__ __forceinline__ PrefixRows(const SharedArgs& args, int u) : a(args), unit(u) {
+    p = u / a.own.kv_heads;
+    kvh = u - p * a.own.kv_heads;
+    length = min(max(a.lens[p], 0), a.max_len);
+  }
+  __device__ __forceinline__ int count() const { return a.rows; }
+  __device__ __forceinline__ int len() const { return length; }
+  __device__ __forceinline__ int chunk() const { return a.chunk; }
+  __device__ __forceinline__ bool parts() const { return true; }
+  __device__ __forceinline__ int limit(int) const { return length; }
+  __device__ __forceinline__ int open() const { return length; }
+  __device__ __forceinline__ const int32_t* table() const { return a.table + (int64_t)p * a.width; }
+  __device__ __forceinline__ const char* query(int row) const {
+    const AttnArgs& o = a.own;
+    const int seq = row / o.rows, rr = row - seq * o.rows, t = rr / o.group;
+    return o.q + (int64_t)(p * a.per + seq) * o.q_batch + t * o.q_query + (int64_t)(kvh * o.group + rr - t * o.group) * o.q_head;
+  }
+  __device__ __forceinline__ int64_t output(int) const { return 0; }
+  __device__ __forceinline__ int64_t part(int c) const { return ((int64_t)unit * a.chunks + c) * a.rows; }
+  __device__ __forceinline__ float2* part_ml() const { return a.part_ml; }
+  __device__ __forceinline__ float* part_o() const { return a.part_o; }
+};
+
+// Many rows behind a prefix.
+template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
+__global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_shared_tiles_kernel(SharedArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) uint4 tiles[];  // [2][TG][keys, values][WT * VECS]
+  prefix_chunk<F32, DP, RG, TG, WT, WAVES>(a, blockIdx.x, tiles);
+}
+
+// Few rows behind a prefix, and the sequences' own slots in the same launch.
+template <bool F32, int DP, int MT, bool MANY, int WAVES>
+__global__ __launch_bounds__(kAttnThreads, WAVES) void kv_shared_rows_kernel(SharedArgs a) {
+  extern __shared__ float lds[];
+  const int i = blockIdx.x;
+  if (i < a.pieces) {
+    const int unit = i / a.chunks;
+    decode_chunk<F32, DP, MT, false>(a.own, PrefixRows(a, unit), 0, i - unit * a.chunks, lds);
+  } else {
+    const int j = i - a.pieces, chunk = j / a.own_units, k = j - chunk * a.own_units, unit = k / a.own.row_groups;
+    decode_chunk<F32, DP, MT, MANY>(a.own, OwnRows(a.own, unit), k - unit * a.own.row_groups, chunk, lds);
+  }
+}
+
 // Joins the chunks of the prefix and of the sequence's own slots.  A row's
 // parts are shared out over `split` groups of lanes, each of which holds a row.
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(SharedArgs a, int f32, int split, int64_t total) {
@@ -487,43 +538,66 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(SharedArgs a, int f
 }
 
 struct SharedPlan {
-  int rg, step, row_tiles, chunk, chunks;
+  int rg;  // groups of 32 rows to a workgroup; 0: few rows
+  int step, row_tiles, chunk, chunks;
   AttnPlan own;
   int own_chunks;
   size_t ml_bytes, o_bytes, own_ml_bytes, own_o_bytes;
   size_t bytes() const { return ml_bytes + o_bytes + own_ml_bytes + own_o_bytes; }
 };
 
-static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t rows, int64_t max_prefix, int64_t max_len,
-                        SharedPlan* p) {
+// Tokens of a tile.
+constexpr int tile_tokens(bool f32, int dim, int rg) { return !f32 && dim <= 128 && rg == 4 ? 64 : 32; }
+
+// Waves of a SIMD that its registers leave room for.
+constexpr int tile_waves(bool f32, int dim, int rg) { return dim > 128 || (f32 && dim > 64 && rg == 2) ? 1 : 2; }
+
+static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t queries, int64_t group, int64_t max_prefix,
+                        int64_t max_len, SharedPlan* p) {
+  const int64_t rows = queries * group;
   const bool f32 = c->dtype == TALLAX_F32;
   const int64_t all = c->batch / prefixes * rows, units = prefixes * c->kv_heads;
-  p->rg = all <= 32 && !(f32 && c->dim > 128) ? 1 : all <= 64 ? 2 : 4;
-  const int tg = c->dim > 128 ? (f32 || p->rg == 4 ? 1 : 2) : f32 ? (c->dim > 64 ? 2 : p->rg == 4 ? 2 : 4) : p->rg == 4 ? 1 : p->rg == 2 ? 2 : 4;
-  const int wt = !f32 && c->dim <= 128 && p->rg >= 2 ? 64 : 32;
-  const int places = !f32 && c->dim <= 128 ? (p->rg == 4 ? 512 : p->rg == 2 ? 256 : 256) : 256;
-  p->step = tg * wt;
-  p->row_tiles = (int)((all + 32 * p->rg - 1) / (32 * p->rg));
-  // Chunks, so that the workgroups take whole rounds of the card's 256 places: of one to four rounds that which leaves
-  // the fewest steps one after another, each round with some six more for its beginning and end.
-  const int64_t steps = (max_prefix + p->step - 1) / p->step, pieces = units * p->row_tiles;
-  int64_t best = INT64_MAX;
-  p->chunks = 1;
-  p->chunk = (int)(steps > 0 ? steps : 1) * p->step;
-  for (int rounds = 1; rounds <= 4; ++rounds) {
-    int64_t n = places * rounds / pieces;
-    if (n < 1) n = 1;
-    if (n > steps) n = steps;
-    if (n < 1) break;
-    const int64_t each = (steps + n - 1) / n;
-    const int64_t turns = (pieces * n + places - 1) / places, cost = turns * (each + 6);
-    if (cost < best) {
-      best = cost;
-      p->chunk = (int)(each * p->step);
-      p->chunks = (int)((steps + each - 1) / each);
+  const int most = f32 || c->dim <= 128 ? 2 : 1;  // sixteens of rows that the kernel for few takes
+  plan_attention(c->batch, c->kv_heads, rows, c->dim, c->dtype, max_len, false, &p->own);
+  if (all <= 16 * most) {
+    p->rg = 0;
+    p->own.mt = all <= 16 ? 1 : 2;
+    p->own.row_groups = 1;
+    AttnPlan front;
+    plan_attention(prefixes, c->kv_heads, all, c->dim, c->dtype, max_prefix, false, &front);
+    p->row_tiles = 1;
+    p->step = 1;
+    p->chunk = front.chunk;
+    p->chunks = front.chunks;
+  } else {
+    p->rg = all <= 64 && !(f32 && c->dim > 128) ? 2 : 4;  // float32 above dim 128 has no room for two groups' tiles
+    p->step = kAttnWaves / p->rg * tile_tokens(f32, c->dim, p->rg);
+    p->row_tiles = (int)((all + 32 * p->rg - 1) / (32 * p->rg));
+    // Chunks: of those that make one to eight workgroups to a CU, what takes the least by these measurements (bfloat16,
+    // dim 128): a workgroup alone on its CU takes 2.3 us a step, two of them 3.9, some two steps more for their beginning
+    // and end; and each chunk's parts are written and read, at some 5 TB/s.  64 sequences, 32 / 8 heads, behind 8192
+    // slots 31 us with 16 chunks, 33 with 32; 16 with 64 / 8 heads behind 131071 145 with 64 and 167 with 32.
+    const int64_t steps = (max_prefix + p->step - 1) / p->step, pieces = units * p->row_tiles;
+    const bool two = tile_waves(f32, c->dim, p->rg) == 2;
+    const double dims = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256, tokens = tile_tokens(f32, c->dim, p->rg);
+    const double step_us = (f32 ? 7.4 : 2.3) * dims / 128 * tokens / 64, part_us = (double)(units * all) * c->dim * 8 / 5e6;
+    double best = 1e300;
+    p->chunks = 1;
+    p->chunk = (int)(steps > 0 ? steps : 1) * p->step;
+    for (int k = 1; k <= 8; ++k) {
+      int64_t n = 256 * k / pieces;
+      n = n > steps ? steps : n;
+      n = n < 1 ? 1 : n;
+      const int64_t each = (steps + n - 1) / n, groups = pieces * n, room = two ? 512 : 256, rest = groups % room;
+      const double turns = groups / room * (two ? 1.7 : 1.0) + (rest > 256 ? 1.7 : rest ? 1.0 : 0.0);
+      const double cost = turns * (each + 2) * step_us + n * part_us;
+      if (steps > 0 && cost < best) {
+        best = cost;
+        p->chunk = (int)(each * p->step);
+        p->chunks = (int)((steps + each - 1) / each);
+      }
     }
   }
-  plan_attention(c->batch, c->kv_heads, rows, c->dim, c->dtype, max_len, false, &p->own);
   p->own_chunks = p->own.chunks > 1 ? p->own.chunks : 2;  // with one the kernel would write outputs, not parts
   p->ml_bytes = align_up((size_t)(units * p->chunks * all) * sizeof(float2), 256);
   p->o_bytes = align_up((size_t)(units * p->chunks * all) * c->dim * 4, 256);
@@ -532,49 +606,47 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t rows
   p->own_o_bytes = align_up((size_t)own * c->dim * 4, 256);
 }
 
-template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
-static int launch_prefix(const SharedArgs& a, int step, hipStream_t s) {
-  using P = Prefix<F32, DP, RG, TG, WT, WAVES>;
-  if (step != P::STEP) {  // the plan and the instance must agree
-    set_error("kv_decode_shared: no kernel for steps of %d", step);
-    return kUnsupported;
-  }
-  if (P::kBytes > 48 * 1024) {
-    const hipError_t e = set_dynamic_lds_limit((const void*)kv_prefix_kernel<F32, DP, RG, TG, WT, WAVES>, P::kBytes, s);
+template <class K>
+static int launch_shared(K kernel, const SharedArgs& a, int64_t groups, int bytes, hipStream_t s) {
+  if (bytes > 48 * 1024) {
+    const hipError_t e = set_dynamic_lds_limit((const void*)kernel, bytes, s);
     if (e != hipSuccess) {
       set_error("kv_decode_shared: %s", hipGetErrorString(e));
       return kHipError;
     }
   }
-  const unsigned grid = (unsigned)((a.pieces + 7) / 8 * 8) * (unsigned)a.row_tiles;
-  kv_prefix_kernel<F32, DP, RG, TG, WT, WAVES><<<grid, P::kThreads, P::kBytes, s>>>(a);
+  kernel<<<(unsigned)groups, kAttnThreads, bytes, s>>>(a);
   return launch_status("kv_decode_shared");
 }
 
-static int launch_prefix_any(const SharedArgs& a, int rg, int step, bool f32, hipStream_t s) {
-  const int dim = a.own.c.dim;
-  if (f32) {
-    if (dim <= 64)
-      return rg == 1   ? launch_prefix<true, 64, 1, 4, 32, 1>(a, step, s)
-             : rg == 2 ? launch_prefix<true, 64, 2, 4, 32, 2>(a, step, s)
-                       : launch_prefix<true, 64, 4, 2, 32, 2>(a, step, s);
-    if (dim <= 128)
-      return rg == 1   ? launch_prefix<true, 128, 1, 2, 32, 1>(a, step, s)
-             : rg == 2 ? launch_prefix<true, 128, 2, 2, 32, 1>(a, step, s)
-                       : launch_prefix<true, 128, 4, 2, 32, 2>(a, step, s);
-    return rg == 2 ? launch_prefix<true, 256, 2, 1, 32, 1>(a, step, s) : launch_prefix<true, 256, 4, 1, 32, 1>(a, step, s);
-  }
-  if (dim <= 64)
-    return rg == 1   ? launch_prefix<false, 64, 1, 4, 32, 1>(a, step, s)
-           : rg == 2 ? launch_prefix<false, 64, 2, 2, 64, 1>(a, step, s)
-                     : launch_prefix<false, 64, 4, 1, 64, 2>(a, step, s);
-  if (dim <= 128)
-    return rg == 1   ? launch_prefix<false, 128, 1, 4, 32, 1>(a, step, s)
-           : rg == 2 ? launch_prefix<false, 128, 2, 2, 64, 1>(a, step, s)
-                     : launch_prefix<false, 128, 4, 1, 64, 2>(a, step, s);
-  return rg == 1   ? launch_prefix<false, 256, 1, 2, 32, 1>(a, step, s)
-         : rg == 2 ? launch_prefix<false, 256, 2, 2, 32, 1>(a, step, s)
-                   : launch_prefix<false, 256, 4, 1, 32, 1>(a, step, s);
+template <bool F32, int DP, int RG>
+static int launch_tiles(const SharedArgs& a, int64_t groups, hipStream_t s) {
+  constexpr int TG = kAttnWaves / RG, WT = tile_tokens(F32, DP, RG), WAVES = tile_waves(F32, DP, RG);
+  return launch_shared(kv_shared_tiles_kernel<F32, DP, RG, TG, WT, WAVES>, a, groups, Prefix<F32, DP, RG, TG, WT, WAVES>::kBytes, s);
+}
+
+template <bool F32, int DP, int MT>
+static int launch_rows(const SharedArgs& a, int64_t groups, hipStream_t s) {
+  constexpr int WAVES = F32 && DP > 128 ? 1 : 2;
+  if (a.own.queries > 1)
+    return launch_shared(kv_shared_rows_kernel<F32, DP, MT, true, WAVES>, a, groups, decode_lds_bytes<F32, DP, MT, true>(), s);
+  return launch_shared(kv_shared_rows_kernel<F32, DP, MT, false, WAVES>, a, groups, decode_lds_bytes<F32, DP, MT, false>(), s);
+}
+
+template <bool F32, int DP>
+static int launch_dim(const SharedArgs& a, const SharedPlan& p, int64_t groups, hipStream_t s) {
+  if (p.rg == 4) return launch_tiles<F32, DP, 4>(a, groups, s);
+  if constexpr (!F32 || DP <= 128)
+    if (p.rg == 2) return launch_tiles<F32, DP, 2>(a, groups, s);
+  if constexpr (F32 || DP <= 128)
+    if (p.own.mt == 2) return launch_rows<F32, DP, 2>(a, groups, s);
+  return launch_rows<F32, DP, 1>(a, groups, s);
+}
+
+template <bool F32>
+static int launch_prefix(const SharedArgs& a, const SharedPlan& p, int64_t groups, hipStream_t s) {
+  if (a.own.c.dim <= 64) return launch_dim<F32, 64>(a, p, groups, s);
+  return a.own.c.dim <= 128 ? launch_dim<F32, 128>(a, p, groups, s) : launch_dim<F32, 256>(a, p, groups, s);
 }
 
 }  // namespace tx
@@ -594,7 +666,7 @@ size_t tallax_kv_decode_shared_workspace_size(const tallax_kv_cache* cache, int6
   const int64_t most = prefix_width * cache->page_size;
   if (max_prefix < 0 || max_prefix > most) max_prefix = most;
   SharedPlan p;
-  plan_shared(cache, prefixes, queries * (heads / cache->kv_heads), max_prefix, max_len, &p);
+  plan_shared(cache, prefixes, queries, heads / cache->kv_heads, max_prefix, max_len, &p);
   return p.bytes();
 }
 
@@ -645,15 +717,15 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
     return kInvalidArgument;
   }
   SharedPlan p;
-  plan_shared(cache, prefixes, rows, max_prefix, max_len, &p);
+  plan_shared(cache, prefixes, queries, group, max_prefix, max_len, &p);
   st = check_workspace("kv_decode_shared", workspace, workspace_bytes, p.bytes());
   if (st != kOk) return st;
   st = pool_offsets(cache, o.c, "kv_decode_shared", &o.at);
   if (st != kOk) return st;
   const int64_t units = cache->batch * cache->kv_heads, pieces = prefixes * cache->kv_heads * p.chunks;
   const int64_t all = cache->batch * queries * heads;
-  if (units * p.own.row_groups > INT32_MAX || p.own.chunks > 65535 || cache->batch * rows > INT32_MAX / 64 ||
-      (pieces + 8) * p.row_tiles > INT32_MAX || all > INT32_MAX) {
+  if (units * p.own.row_groups * p.own.chunks + (pieces + 8) * p.row_tiles > INT32_MAX ||
+      cache->batch * rows > INT32_MAX / 64 || all > INT32_MAX) {
     set_error("kv_decode_shared: too many workgroups");
     return kUnsupported;
   }
@@ -694,24 +766,27 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
   a.row_tiles = p.row_tiles;
   a.chunk = p.chunk;
   a.chunks = p.chunks;
-  a.pieces = (int)pieces;
   a.flip = scale < 0 ? (es == 4 ? 0x80000000u : 0x80008000u) : 0u;
   a.scale2 = fmaxf(fabsf(o.scale2), 1.1754944e-38f);
   hipStream_t s = (hipStream_t)stream;
   const bool f32 = cache->dtype == TALLAX_F32;
-  if (a.max_len > 0) {
-    st = launch_prefix_any(a, p.rg, p.step, f32, s);
+  a.pieces = a.max_len > 0 ? (int)pieces : 0;
+  a.own_units = (int)(units * p.own.row_groups);
+  const int64_t own = max_len > 0 ? (int64_t)a.own_units * p.own.chunks : 0;
+  const int64_t groups = p.rg ? ((int64_t)a.pieces + 7) / 8 * 8 * p.row_tiles : a.pieces + own;
+  if (groups > 0) {
+    st = f32 ? launch_prefix<true>(a, p, groups, s) : launch_prefix<false>(a, p, groups, s);
     if (st != kOk) return st;
   }
-  if (max_len > 0) {
+  if (p.rg && own > 0) {
     st = launch_attention(o, p.own, units, f32, s);
     if (st != kOk) return st;
   }
-  const int groups = o.c.dim <= 64 ? 16 : o.c.dim <= 128 ? 8 : 4;
+  const int slots = o.c.dim <= 64 ? 16 : o.c.dim <= 128 ? 8 : 4;
   const int64_t parts = p.chunks + p.own.chunks;
   int split = 1;  // enough workgroups for the card, and no more groups of lanes to a row than parts
-  while (split < groups && split < parts && all * split / groups < 1024) split *= 2;
-  const int64_t each = groups / split;
+  while (split < slots && split < parts && all * split / slots < 1024) split *= 2;
+  const int64_t each = slots / split;
   kv_shared_join_kernel<<<(unsigned)((all + each - 1) / each), 256, 0, s>>>(a, f32, split, all);
   return launch_status("kv_decode_shared");
 }
