@@ -172,3 +172,32 @@ def test_refusals(gpu):
     for y in (x.half(), x.int(), torch.zeros((4, 1025), device=gpu)):
         with pytest.raises(NotImplementedError):
             experts.route(y, 4)
+
+
+def test_zeros_of_both_signs_tie(gpu):
+    rng = np.random.default_rng(7)
+    x = rng.choice([0.0, -0.0, 1e-30, -1.0], (50, 64)).astype(np.float32)
+    for dtype in ("f32", "bf16"):
+        for score in ("softmax", "sigmoid"):
+            _check(gpu, x, 8, dtype, None, score=score)
+            _check(gpu, x, 8, dtype, None, score=score, groups=8, top_groups=3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_large_logits_and_biases(gpu, dtype):
+    """Scores that saturate, that vanish, and biases far larger than them."""
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((40, 128)) * 30
+    for score in ("softmax", "sigmoid"):
+        for bias in (None, rng.standard_normal(128) * 100, rng.integers(-3, 4, 128) * 0.5):
+            for groups, top in ((1, 1), (16, 4), (4, 1)):
+                for how in ("max", "top2"):
+                    kw = dict(score=score, groups=groups, top_groups=top, group_score=how)
+                    values = host_values(x.astype(np.float32), dtype).astype(np.float64)
+                    b = None if bias is None else np.asarray(bias, np.float32).astype(np.float64)
+                    want, ids, margin = L.route(values, 8, bias=b, **kw)
+                    w, got = _run(gpu, x.astype(np.float32), 8, dtype, bias, **kw)
+                    if margin > 1e-13:
+                        assert np.array_equal(got, ids), kw
+                        assert (np.abs(w - want) <= np.abs(want) * 32 * L.F32 + 2.0 ** -148).all()
+                    assert np.isfinite(w).all()
