@@ -2,8 +2,6 @@
 // experts and their weights, a wave for each token.
 #include <math.h>
 
-#include <type_traits>
-
 #include "tx_common.h"
 #include "tx_host.h"
 
@@ -18,7 +16,7 @@ struct RouteArgs {
   const void* logits;
   int64_t tokens, row_stride;
   int experts, k, groups, per_group, top_groups, group_top, sigmoid, renormalise;
-  int shift, vectors;  // a group's lanes are 1 << shift; logits may be read four at a time
+  int shift, each, places, vectors;  // a group's lanes are 1 << shift, with `each` experts; logits may be read four at a time
   const float* bias;
   double scale;
   float* weights;
@@ -174,40 +172,22 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_exactly_kernel(Rout
   if (token < a.tokens) route_exactly<BF16, NJ>(a, token, lds + wave * a.experts);
 }
 
-// Comparators of Batcher's odd-even merge sort of N values.
-template <int N>
-struct SortNet {
-  int lo[80] = {}, hi[80] = {}, n = 0;
-  constexpr SortNet() {
-    for (int p = 1; p < N; p *= 2)
-      for (int k = p; k >= 1; k /= 2)
-        for (int j = k % p; j + k < N; j += 2 * k)
-          for (int i = 0; i < k && i + j + k < N; ++i)
-            if ((i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-              lo[n] = i + j;
-              hi[n++] = i + j + k;
-            }
-  }
-};
-
 __device__ __forceinline__ void larger_first(int& x, int& y) {
   const int m = max(x, y);
   y = min(x, y);
   x = m;
 }
 
-template <int N>
-__device__ __forceinline__ void sort_down(int* v) {
-  constexpr SortNet<N> net;
-#pragma unroll
-  for (int i = 0; i < net.n; ++i) larger_first(v[net.lo[i]], v[net.hi[i]]);
-}
-
-// The L largest of two descending lists of L, descending, in the first.
+// The L largest of a descending list of L and four values, descending.
 template <int L>
-__device__ __forceinline__ void keep_largest(int* x, const int* y) {
+__device__ __forceinline__ void insert_four(int (&x)[L], int (&y)[4]) {
+  larger_first(y[0], y[1]);
+  larger_first(y[2], y[3]);
+  larger_first(y[0], y[2]);
+  larger_first(y[1], y[3]);
+  larger_first(y[1], y[2]);
 #pragma unroll
-  for (int i = 0; i < L; ++i) x[i] = max(x[i], y[L - 1 - i]);
+  for (int i = 0; i < 4; ++i) x[L - 1 - i] = max(x[L - 1 - i], y[i]);
 #pragma unroll
   for (int d = L / 2; d >= 1; d /= 2)
 #pragma unroll
@@ -257,61 +237,27 @@ __device__ __forceinline__ double row_sum_d(double v) {
   return v + lane_xor_d(v, 1);
 }
 
-// A group's rank, the same in all of its lanes.
-struct Rank {
-  int whole;          // where it is exact
-  float value, room;  // else, and how far any two of the token may be off
-};
+__device__ __forceinline__ uint32_t from_lane(uint32_t x, int lane) {
+  return (uint32_t)__builtin_amdgcn_ds_bpermute(lane << 2, (int)x);
+}
+__device__ __forceinline__ double from_lane_d(double x, int lane) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = from_lane((uint32_t)u, lane), hi = from_lane((uint32_t)(u >> 32), lane);
+  return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
 
-// Compares it with that of the group N lanes before: counts those that come first, and sees whether any is too near to
-// tell.
-template <int N>
-__device__ __forceinline__ void count_before(const Rank& r, bool exact, int l, int shift, int& before, bool& near) {
-  if (N & ((1 << shift) - 1)) return;
-  const bool lower = (((l - N) & 15) >> shift) < (l >> shift);
-  if (exact) {
-    const int o = row_ror<N>(r.whole);
-    before += (o > r.whole) | ((o == r.whole) & lower);
-  } else {
-    const float o = row_ror_f<N>(r.value);
-    before += (o > r.value) | ((o == r.value) & lower);
-    near = near | (fabsf(o - r.value) <= r.room);
+// How many of lanes l + step, l + 2 step, .. (mod 16) of the same 16, below n, come before this one: by the larger key,
+// of equal ones by the lower number.
+__device__ __forceinline__ int count_before(double key, int number, int l, int step, int n) {
+  int before = 0;
+#pragma unroll 1
+  for (int r = step; r < 16; r += step) {
+    const int from = (l + r) & 15, lane = (lane_id() & 48) | from;
+    const double o = from_lane_d(key, lane);
+    const int i = (int)from_lane((uint32_t)number, lane);
+    before += (from < n) & ((o > key) | ((o == key) & (i < number)));
   }
-}
-
-// Whether it matters: one of the two is chosen and the other is not.
-template <int N>
-__device__ __forceinline__ void across(const Rank& r, int open, int shift, bool& near) {
-  if (N & ((1 << shift) - 1)) return;
-  near = near | ((fabsf(row_ror_f<N>(r.value) - r.value) <= r.room) & (row_ror<N>(open) != open));
-}
-
-template <int N>
-__device__ __forceinline__ void count_larger(double key, int at, int l, int k, int& before) {
-  const uint64_t u = (uint64_t)__double_as_longlong(key);
-  const uint32_t lo = (uint32_t)row_ror<N>((int)(uint32_t)u), hi = (uint32_t)row_ror<N>((int)(uint32_t)(u >> 32));
-  const double o = __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
-  const int i = row_ror<N>(at);
-  before += (((l - N) & 15) < k) & ((o > key) | ((o == key) & (i < at)));
-}
-
-template <class F>
-__device__ __forceinline__ void for_rotations(F f) {  // of 16 lanes
-  f(std::integral_constant<int, 1>());
-  f(std::integral_constant<int, 2>());
-  f(std::integral_constant<int, 3>());
-  f(std::integral_constant<int, 4>());
-  f(std::integral_constant<int, 5>());
-  f(std::integral_constant<int, 6>());
-  f(std::integral_constant<int, 7>());
-  f(std::integral_constant<int, 8>());
-  f(std::integral_constant<int, 9>());
-  f(std::integral_constant<int, 10>());
-  f(std::integral_constant<int, 11>());
-  f(std::integral_constant<int, 12>());
-  f(std::integral_constant<int, 13>());
-  f(std::integral_constant<int, 14>());
-  f(std::integral_constant<int, 15>());
+  return before;
 }
 
 constexpr int kNone = INT32_MIN;
@@ -336,146 +282,217 @@ __device__ __forceinline__ double reciprocal(double x) {
   return fma(fma(-x, r, 1.0), r, r);
 }
 
-// Four tokens a wave, 16 lanes each, a lane with up to EPL neighbouring experts
-// of one group; 1 << shift lanes hold a group.  Keys (scores plus bias, or
-// logits) are 32 bits, in the order of integers, their last bits the expert's
-// place in the lane.  Each lane sorts its keys and keeps the L largest; the
-// largest head of 16 lanes is the next choice, and the lane it is from moves on.
-// Where two choices lie within their keys' rounding, their order is found in 64
-// bits; where the last choice and the next, or a group that is chosen and one
-// that is not, do, or there are not enough experts, the token goes to the whole
-// wave in 64 bits.  bfloat16 logits without a bias have room for the whole
-// expert's number in the key, which then is exact.
-template <bool BF16, int EPL, int L>
+// Four tokens a wave, 16 lanes each, a lane with a.each neighbouring experts of
+// one group; 1 << shift lanes hold a group.  Keys (scores plus bias, or logits)
+// are 32 bits, in the order of integers, their last bits the expert's place in
+// the lane.  Each lane keeps its L largest, sorted; the largest head of 16 lanes
+// is the next choice, and the lane it is from moves on.
+// Where two choices, or the last and the next, lie within their keys' rounding,
+// those are compared in 64 bits, and where a group that is chosen and one that is
+// not do, the groups are.  Where the one after the next is as near, or there are
+// not enough experts, the token goes to the whole wave in 64 bits.  bfloat16 logits
+// without a bias have room for the whole expert's number in the key, which then is
+// exact.
+//
+// Every wave runs through here once, and what it waits for is its instructions, at
+// some 16 cycles each when they are new to the CU: hence the loops, which hold
+// little code (16384 tokens of 256 experts in 8 groups took 17.2 us with everything
+// unrolled).
+template <bool BF16, int L, int NJ>
 __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a) {
   extern __shared__ double lds[];  // [waves][experts], where there are groups
-  constexpr int kPlace = EPL - 1;
   constexpr float kLog2e = 1.44269504088896340736f;
-  // How far apart two keys must lie: the place takes up to EPL - 1 last bits of 24 of each; a score is off by the rounding
-  // of its exponent (at most .3 of 2^-23 of the largest score, since s |x| has a maximum), of its exponential, sum and
-  // reciprocal (2^-23 of itself each) and of the sum with the bias: by less than 2^-21 of the largest, two by 2^-20.
-  constexpr float kCut = EPL / 8388608.0f, kOff = 9.5367432e-7f;
+  // How far apart two keys must lie: the place takes the last bits of 24 of each, so that both are too small, by up to
+  // `cut` of themselves; a score is off by the rounding of its exponent (at most .3 of 2^-23 of the largest score, since
+  // s |x| has a maximum), of its exponential, sum and reciprocal (2^-23 of itself each) and of the sum with the bias: by
+  // less than 2^-21 of the largest, two by 2^-20.
+  const float cut = (a.places + 1) * 1.1920929e-7f;
+  constexpr float kOff = 9.5367432e-7f;
   const int wave = threadIdx.x / kWave, lane = lane_id(), l = lane & 15;
   const int64_t first = ((int64_t)blockIdx.x * kRouteWaves + wave) * 4, token = first + lane / 16;
   if (first >= a.tokens) return;
   const bool valid = token < a.tokens, exact = BF16 && !a.bias;
-  const int group = l >> a.shift, within = (l & ((1 << a.shift) - 1)) * EPL;
+  const int group = l >> a.shift, within = (l & ((1 << a.shift) - 1)) * a.each;
   const int e0 = group * a.per_group + within;
-  const int n = valid && group < a.groups ? a.per_group - within : 0;  // experts of this lane, if positive
-  float x[EPL], bias[EPL];
-  if (a.vectors) {
-#pragma unroll
-    for (int j = 0; j < EPL; j += 4) {
-      const bool some = j < n;
-      const int64_t at = some ? token * a.row_stride + e0 + j : 0;
+  const int n = valid && group < a.groups ? min(a.per_group - within, a.each) : 0;  // experts of this lane, if positive
+  const int64_t row = valid ? token * a.row_stride : 0;
+
+  // logits and biases of four experts; -inf where there are none
+  auto four = [&](int j, float (&x)[4], float (&b)[4]) {
+    if (a.vectors) {
+      const int at = j < n ? e0 + j : 0;
       if constexpr (BF16) {
-        const uint2 u = *(const uint2*)((const uint16_t*)a.logits + at);
-        x[j] = __uint_as_float(u.x << 16);
-        x[j + 1] = __uint_as_float(u.x & 0xffff0000u);
-        x[j + 2] = __uint_as_float(u.y << 16);
-        x[j + 3] = __uint_as_float(u.y & 0xffff0000u);
+        const uint2 u = *(const uint2*)((const uint16_t*)a.logits + row + at);
+        x[0] = __uint_as_float(u.x << 16);
+        x[1] = __uint_as_float(u.x & 0xffff0000u);
+        x[2] = __uint_as_float(u.y << 16);
+        x[3] = __uint_as_float(u.y & 0xffff0000u);
       } else {
-        const float4 u = *(const float4*)((const float*)a.logits + at);
-        x[j] = u.x;
-        x[j + 1] = u.y;
-        x[j + 2] = u.z;
-        x[j + 3] = u.w;
+        const float4 u = *(const float4*)((const float*)a.logits + row + at);
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
       }
-      const float4 u = a.bias ? *(const float4*)(a.bias + (some ? e0 + j : 0)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      bias[j] = u.x;
-      bias[j + 1] = u.y;
-      bias[j + 2] = u.z;
-      bias[j + 3] = u.w;
+      const float4 u = a.bias ? *(const float4*)(a.bias + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+      b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w;
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[j + i] = some ? x[j + i] : -INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        const int at = j + i < n ? e0 + j + i : 0;
+        x[i] = BF16 ? __uint_as_float((uint32_t)((const uint16_t*)a.logits)[row + at] << 16) : ((const float*)a.logits)[row + at];
+        b[i] = a.bias ? a.bias[at] : 0.0f;
+      }
     }
-  } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const bool some = j < n;
-      x[j] = logit_at<BF16>(a, some ? token : 0, some ? e0 + j : 0);
-      bias[j] = a.bias ? a.bias[some ? e0 + j : 0] : 0.0f;
-      x[j] = some ? x[j] : -INFINITY;
-    }
-  }
+    for (int i = 0; i < 4; ++i) x[i] = j + i < n ? x[i] : -INFINITY;
+  };
+
   // softmax: the sum over all experts, where scores are compared or given as they are
   const bool scores = a.bias || (a.groups > 1 && a.group_top == 2);
   float top = 0.0f, sum = 1.0f;  // top: 0 for sigmoid scores
   if (!a.sigmoid && (scores || !a.renormalise)) {
     top = -INFINITY;
+    sum = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < a.each; j += 4) {
+      float x[4], b[4];
+      four(j, x, b);
+      float m = top;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) top = x[j] > top ? fminf(x[j], kMost) : top;
-    top = row_max_f(top);
-    top = top == -INFINITY ? 0.0f : top;
-    float part = 0.0f;
+      for (int i = 0; i < 4; ++i) m = x[i] > m ? fminf(x[i], kMost) : m;
+      const float base = m == -INFINITY ? 0.0f : m;
+      sum *= __builtin_amdgcn_exp2f((top - base) * kLog2e);
+      top = m;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      part += x[j] > -INFINITY ? __builtin_amdgcn_exp2f((fminf(x[j], kMost) - top) * kLog2e) : 0.0f;
-    sum = row_sum_f(part);
+      for (int i = 0; i < 4; ++i)
+        sum += x[i] > -INFINITY ? __builtin_amdgcn_exp2f((fminf(x[i], kMost) - base) * kLog2e) : 0.0f;
+    }
+    const float m = row_max_f(top), base = m == -INFINITY ? 0.0f : m;
+    sum = row_sum_f(sum * __builtin_amdgcn_exp2f((top - base) * kLog2e));
+    top = base;
   }
   const float inverse = 1.0f / sum, largest = a.sigmoid ? 1.0f : inverse;  // of all scores
   auto score_of = [&](float v) {
     return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * kLog2e))
                      : __builtin_amdgcn_exp2f((v - top) * kLog2e) * inverse;
   };
-  int key[EPL];
+
+  int key[L];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    bool here = x[j] > -INFINITY;  // not NaN either
-    x[j] += 0.0f;  // -0 is 0
-    if (exact) {
-      key[j] = here ? (ordered(x[j]) & (int)0xffff0000) | (0xffff - (e0 + j)) : kNone;
-    } else {
-      float f = fminf(x[j], kMost);
-      if (a.bias) {
-        here = here & (bias[j] == bias[j]);
-        f = score_of(f) + fminf(fmaxf(bias[j], -kMost), kMost);
+  for (int i = 0; i < L; ++i) key[i] = kNone;
+#pragma unroll 1
+  for (int j = 0; j < a.each; j += 4) {
+    float x[4], b[4];
+    int k[4];
+    four(j, x, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool here = (x[i] > -INFINITY) & (b[i] == b[i]);  // not NaN either
+      const float v = x[i] + 0.0f;                            // -0 is 0
+      if (exact) {
+        k[i] = (ordered(v) & (int)0xffff0000) | (0xffff - (e0 + j + i));
+      } else {
+        float f = fminf(v, kMost);
+        if (a.bias) f = score_of(f) + __builtin_amdgcn_fmed3f(b[i], -kMost, kMost);
+        k[i] = (ordered(f) & ~a.places) | (a.places - (j + i));
       }
-      key[j] = here ? (ordered(f) & ~kPlace) | (kPlace - j) : kNone;
+      k[i] = here ? k[i] : kNone;
     }
-  }
-  constexpr int S = L < EPL ? L : EPL;
-#pragma unroll
-  for (int i = 0; i < EPL; i += S) {
-    sort_down<S>(key + i);
-    if (i > 0) keep_largest<S>(key, key + i);
+    insert_four<L>(key, k);
   }
   bool near = false;
-  auto value = [&](int k) { return from_ordered(k & (exact ? (int)0xffff0000 : ~kPlace)); };
+  auto value = [&](int k) { return from_ordered(k & (exact ? (int)0xffff0000 : ~a.places)); };
+  // in 64 bits, for the few tokens that need it
+  auto exact_sum = [&]() {
+    double all = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const float v = logit_at<BF16>(a, token, e0 + j);
+      all += v > -INFINITY ? exp((double)fminf(v, kMost) - (double)top) : 0.0;
+    }
+    return row_sum_d(all);
+  };
+  auto exact_key = [&](float v, float b, double all) {
+    const double e = exp(a.sigmoid ? -(double)v : (double)v - (double)top);
+    return (a.sigmoid ? 1.0 / (1.0 + e) : e / all) + (double)__builtin_amdgcn_fmed3f(b, -kMost, kMost);
+  };
+  // whether two keys, in this order, are too near to tell
+  auto close = [&](int larger, int smaller) {
+    const float p = value(larger), q = value(smaller);
+    return (smaller != kNone) & (a.bias ? p - q <= cut * fmaxf(fabsf(p), fabsf(q)) + kOff * largest : p == q);
+  };
+  auto expert_of = [&](int k, int lane_of) {
+    return exact ? 0xffff - (k & 0xffff)
+                 : (lane_of >> a.shift) * a.per_group + (lane_of & ((1 << a.shift) - 1)) * a.each + a.places - (k & a.places);
+  };
   if (a.groups > 1) {
     int k0 = key[0], k1 = key[1];
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-      if (d >> a.shift) continue;
-      const int o0 = (int)lane_xor((uint32_t)k0, d), o1 = (int)lane_xor((uint32_t)k1, d);
+#pragma unroll 1
+    for (int d = 1; d >> a.shift == 0; d <<= 1) {
+      const int o0 = (int)from_lane((uint32_t)k0, lane ^ d), o1 = (int)from_lane((uint32_t)k1, lane ^ d);
       k1 = max(min(k0, o0), max(k1, o1));
       k0 = max(k0, o0);
     }
-    Rank r;
-    const bool whole = a.group_top == 1 && exact;
-    r.whole = group < a.groups ? k0 : kNone;
-    float v0 = value(k0), v1 = value(k1);
-    if (a.group_top == 1) {
-      r.value = v0;
-      // logits, as they are but for their last bits
-      r.room = a.bias ? kCut * fabsf(v0) + kOff * largest : kCut * fabsf(v0);
-    } else if (a.bias) {
-      r.value = v0 + (k1 == kNone ? 0.0f : v1);
-      r.room = kCut * (fabsf(v0) + (k1 == kNone ? 0.0f : fabsf(v1))) + 2.0f * kOff * largest;
-    } else {
-      const float far = fmaxf(fabsf(v0), k1 == kNone ? 0.0f : fabsf(v1)) + fabsf(top);
-      r.value = score_of(v0) + (k1 == kNone ? 0.0f : score_of(v1));
-      r.room = (kCut + kOff) * r.value * (1.0f + far);
+    // the group's rank, and how far any two of the token may be off; whole: integers, which are exact
+    const bool whole = a.group_top == 1 && exact, two = a.group_top == 2 && k1 != kNone;
+    float rank = value(k0), room = cut * fabsf(rank);
+    const float v1 = two ? value(k1) : 0.0f;
+    if (a.bias) {
+      room += cut * fabsf(v1);
+      rank += v1;
+    } else if (a.group_top == 2) {
+      const float far = fmaxf(fabsf(rank), fabsf(v1)) + fabsf(top);
+      rank = score_of(rank) + (two ? score_of(v1) : 0.0f);
+      room = 2.0f * (cut + kOff) * rank * (1.0f + far);
     }
-    if (k0 == kNone || group >= a.groups) r.value = -INFINITY, r.room = 0.0f;
-    r.room = 2.0f * row_max_f(r.room);
+    const bool none = k0 == kNone || group >= a.groups;
+    if (whole) rank = __int_as_float(0);
+    rank = none ? -INFINITY : rank;
+    room = row_max_f(none ? 0.0f : room) + (a.bias ? a.group_top * kOff * largest : 0.0f);
+    const int number = none ? kNone : k0;
     int before = 0;
-    bool close = false;
-    for_rotations([&](auto i) { count_before<i.value>(r, whole, l, a.shift, before, close); });
-    if (__ballot(close)) for_rotations([&](auto i) { across<i.value>(r, before < a.top_groups, a.shift, near); });
+    float over = INFINITY, under = INFINITY;  // to the nearest group that comes before, and after
+#pragma unroll 1
+    for (int r = 1 << a.shift; r < 16; r += 1 << a.shift) {
+      const int from = (l + r) & 15, other = (lane & 48) | from;
+      const bool lower = from >> a.shift < group;
+      const float o = __uint_as_float(from_lane(__float_as_uint(rank), other));
+      const int i = (int)from_lane((uint32_t)number, other);
+      const bool first_ = whole ? (i > number) | ((i == number) & lower) : (o > rank) | ((o == rank) & lower);
+      before += first_;
+      const float d = fabsf(o - rank);  // NaN where both have none
+      over = first_ ? fminf(over, d) : over;
+      under = first_ ? under : fminf(under, d);
+    }
+    // too near: the last group that is chosen and the first that is not
+    const bool border = before == a.top_groups - 1 ? under <= room : before == a.top_groups && over <= room;
+    if (!whole && __ballot(border & valid)) {
+      // of each lane's first four: its two largest are among them, unless the second and the fifth are as near
+      const double all = a.sigmoid || !scores ? 1.0 : exact_sum();
+      double m0 = kGone, m1 = kGone;
+      near = near | close(key[1], key[4]);
+      int k[4] = {key[0], key[1], key[2], key[3]};
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const int e = expert_of(k[0], l);
+        const float v = k[0] != kNone ? fminf(logit_at<BF16>(a, token, e), kMost) : 0.0f;
+        const double y = !scores ? (double)v : exact_key(v, a.bias && k[0] != kNone ? a.bias[e] : 0.0f, all);
+        if (k[0] != kNone) {
+          m1 = fmax(m1, fmin(m0, y));
+          m0 = fmax(m0, y);
+        }
+        k[0] = k[1], k[1] = k[2], k[2] = k[3];
+      }
+#pragma unroll 1
+      for (int d = 1; d >> a.shift == 0; d <<= 1) {
+        const double o0 = from_lane_d(m0, lane ^ d), o1 = from_lane_d(m1, lane ^ d);
+        m1 = fmax(fmin(m0, o0), fmax(m1, o1));
+        m0 = fmax(m0, o0);
+      }
+      if (a.group_top == 2 && m1 > kGone) m0 += m1;
+      before = count_before(group < a.groups ? m0 : kTaken, group, l, 1 << a.shift, 16);
+    }
     if (before >= a.top_groups) {
 #pragma unroll
-      for (int i = 0; i < S; ++i) key[i] = kNone;
+      for (int i = 0; i < L; ++i) key[i] = kNone;
     }
   }
   int mine = kNone, from = 0;  // lane i: choice i, and the lane it is from
@@ -488,23 +505,31 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
     // by masks: of a choice between two places of an array the compiler makes a search through all of it
     const int pop = l == src ? -1 : 0;
 #pragma unroll
-    for (int j = 0; j < S; ++j) key[j] = (pop & (j + 1 < S ? key[j + 1 < S ? j + 1 : 0] : kNone)) | (~pop & key[j]);
+    for (int j = 0; j < L; ++j) key[j] = (pop & (j + 1 < L ? key[j + 1 < L ? j + 1 : 0] : kNone)) | (~pop & key[j]);
   }
   near = near | ((l < a.k) & (mine == kNone));
   bool order = false;  // of this choice and the one before it is open
+  int picks = a.k;     // lanes that hold one
   if (!exact) {
     const int next = row_max(key[0]);
-    auto close = [&](int larger, int smaller) {
-      const float p = value(larger), q = value(smaller);
-      return (smaller != kNone) & (a.bias ? p - q <= kCut * (fabsf(p) + fabsf(q)) + kOff * largest : p == q);
-    };
+    const bool edge = (l == a.k - 1) & close(mine, next);  // of the last choice and the next
     order = (l > 0) & (l < a.k) & close(row_ror<1>(mine), mine);
-    // 32 bits of a softmax's sum leave it open what a score adds to a bias
-    near = near | (order & (a.bias && !a.sigmoid)) | ((l == a.k - 1) & close(mine, next));
+    if (__ballot(edge & valid)) {  // then the next is a choice too, of which one is left out
+      if (a.k == 16) {
+        near = near | edge;
+      } else {
+        const int src = __ffs((int)(uint32_t)((__ballot(key[0] == next) >> (lane & 48)) & 0xffff)) - 1;
+        const int third = row_max(l == src ? key[1] : key[0]);
+        near = near | (edge & close(mine, third));
+        mine = l == a.k ? next : mine;
+        from = l == a.k ? src : from;
+        picks = a.k + (next != kNone);
+        order = order | edge;
+      }
+    }
   }
-  const int at = exact ? 0xffff - (mine & 0xffff)
-                       : (from >> a.shift) * a.per_group + (from & ((1 << a.shift) - 1)) * EPL + kPlace - (mine & kPlace);
-  const bool picked = valid & (l < a.k) & (mine != kNone);
+  const int at = expert_of(mine, from);
+  const bool picked = valid & (l < picks) & (mine != kNone);
   const float logit = picked ? fminf(logit_at<BF16>(a, token, at), kMost) : -INFINITY;
   // scores that 64 bits may not hold, and whose sum may be 0
   if (a.renormalise && (a.sigmoid || scores)) near = near | (picked & (logit - top < -700.0f));
@@ -518,30 +543,34 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
     w = power((double)logit - (double)base);
     if (!a.renormalise) w *= reciprocal((double)sum);
   }
-  w = chosen ? w : 0.0;
+  int place = chosen ? l : 16;
+  if (__ballot(order & chosen)) {
+    const double all = a.sigmoid || !a.bias ? 1.0 : exact_sum();
+    const double exactly = !a.bias ? (double)logit : exact_key(logit, picked ? a.bias[at] : 0.0f, all);
+    const int before = count_before(exactly, at, l, 1, picks);
+    place = chosen ? before : 16;
+  }
+  const bool kept = place < a.k;
+  w = kept ? w : 0.0;
   if (a.renormalise) {
     const double all = row_sum_d(w);
     w = all > 0.0 ? w * reciprocal(all) : 0.0;
   }
-  int place = l;
-  if (__ballot(order & chosen)) {
-    const double score = 1.0 / (1.0 + exp(-(double)logit));
-    const double exactly = !a.bias ? (double)logit : chosen ? score + (double)fminf(fmaxf(a.bias[at], -kMost), kMost) : 0.0;
-    place = 0;
-    for_rotations([&](auto i) { count_larger<i.value>(exactly, at, l, a.k, place); });
-  }
-  if (chosen) {
+  if (kept) {
     a.weights[token * a.k + place] = (float)(w * a.scale);
     a.ids[token * a.k + place] = at;
   }
+#pragma unroll 1
   for (int r = 0; r < 4; ++r)
-    if ((unsure >> (16 * r)) & 0xffff) route_exactly<BF16, EPL / 4>(a, first + r, lds + wave * a.experts);
+    if ((unsure >> (16 * r)) & 0xffff) route_exactly<BF16, NJ>(a, first + r, lds + wave * a.experts);
 }
 
-template <bool BF16, int EPL, int L>
+template <bool BF16, int L>
 static int launch_rows(const RouteArgs& a, size_t lds, hipStream_t s) {
-  constexpr int kTokens = kRouteWaves * 4;
-  route_kernel<BF16, EPL, L><<<(unsigned)((a.tokens + kTokens - 1) / kTokens), kRouteWaves * kWave, lds, s>>>(a);
+  constexpr int kTokens = kRouteWaves * 4, kThreads = kRouteWaves * kWave;
+  const unsigned grid = (unsigned)((a.tokens + kTokens - 1) / kTokens);
+  if (a.experts <= 256) route_kernel<BF16, L, 4><<<grid, kThreads, lds, s>>>(a);
+  else route_kernel<BF16, L, 16><<<grid, kThreads, lds, s>>>(a);
   return launch_status("route");
 }
 
@@ -551,16 +580,15 @@ static int launch_route(RouteArgs a, hipStream_t s) {
   // lanes of a group: a power of two, all groups in 16
   int shift = 4;
   while (shift > 0 && a.groups << shift > 16) --shift;
-  const int each = (a.per_group + (1 << shift) - 1) >> shift;
-  if (a.groups <= 16 && a.k <= 16 && each <= 32) {
+  if (a.groups <= 16 && a.k <= 16) {
     const int bytes = BF16 ? 2 : 4;
     a.shift = shift;
+    a.each = (((a.per_group + (1 << shift) - 1) >> shift) + 3) / 4 * 4;  // at most 64
+    a.places = 3;
+    while (a.places < a.each - 1) a.places = 2 * a.places + 1;
     a.vectors = ((uintptr_t)a.logits | (uintptr_t)(a.row_stride * bytes)) % (4 * bytes) == 0 && (uintptr_t)a.bias % 16 == 0 &&
                 a.per_group % 4 == 0;
-    if (each <= 4) return launch_rows<BF16, 4, 4>(a, lds, s);
-    if (each <= 8) return launch_rows<BF16, 8, 8>(a, lds, s);
-    if (each <= 16) return a.k <= 8 ? launch_rows<BF16, 16, 8>(a, lds, s) : launch_rows<BF16, 16, 16>(a, lds, s);
-    return a.k <= 8 ? launch_rows<BF16, 32, 8>(a, lds, s) : launch_rows<BF16, 32, 16>(a, lds, s);
+    return a.k <= 8 ? launch_rows<BF16, 8>(a, lds, s) : launch_rows<BF16, 16>(a, lds, s);
   }
   const unsigned grid = (unsigned)((a.tokens + kRouteWaves - 1) / kRouteWaves);
   const int threads = kRouteWaves * kWave;
