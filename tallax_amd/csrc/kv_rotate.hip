@@ -4,9 +4,11 @@
 //   y0 = x0 cos a - x1 sin a,   y1 = x1 cos a + x0 sin a,
 // in float32, rounded once to the tensors' type; values are only moved.
 //
-// A workgroup takes a few tokens of one sequence.  Its threads first work out
-// the tokens' places in the cache and the cosines and sines of all pairs, which
-// the heads share, into LDS; then each moves 16 bytes at a time.
+// A workgroup takes one to four tokens of one sequence, a whole number of waves
+// each.  Its threads first work out the tokens' places in the cache and the
+// cosines and sines of all pairs, which the heads share, into LDS; then each
+// moves 16 bytes of a head at a time, or 32.  A token's addresses are the same
+// in a wave: what is left to each vector is its head and its place in it.
 #include "tx_common.h"
 #include "tx_kv.h"
 
@@ -17,10 +19,11 @@ struct RotateArgs {
   const int32_t* lens;
   const int32_t* counts;
   const char* in[3];                       // q, k, v of the new tokens
-  int64_t batch_at[3], token_at[3], head_at[3];  // their strides in bytes
+  uint32_t batch_at[3], token_at[3];       // their strides, of heads in bytes, else in sixteens of them
+  uint32_t head_at[3];
   char* out_q;
   int tokens, heads, kv_heads, pairs, axes;
-  int per_wg;       // tokens of a workgroup
+  int log_tokens;   // 1 << log_tokens tokens a workgroup, 256 >> log_tokens threads each
   const float* frequencies;
   const int32_t* places;     // [batch, tokens, axes] or null
   const int32_t* pair_axes;  // [pairs] or null
@@ -28,7 +31,7 @@ struct RotateArgs {
   int32_t* positions;
   const int32_t* seen;
   int32_t* out_lens;
-  PageDiv per_token, per_head, per_value;  // items of a token, of a rotated head, of a value's head
+  PageDiv per_head, per_value, per_token;  // items of a rotated head, of a value's head; pairs of a token
 };
 
 constexpr int kRotateTokens = 4;  // of a workgroup, at most
@@ -64,8 +67,8 @@ template <bool F32>
 struct Vec {  // 16 bytes of elements as float32
   static constexpr int kE = F32 ? 4 : 8;
   float x[kE];
-  __device__ __forceinline__ void load(const char* p) {
-    const uint4 u = *(const uint4*)p;
+  __device__ __forceinline__ void load(const char* p) { unpack(*(const uint4*)p); }
+  __device__ __forceinline__ void unpack(uint4 u) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < kE; ++i) {
@@ -106,77 +109,72 @@ template <bool F32, int HOW>
 __global__ __launch_bounds__(256) void kv_rotate_kernel(RotateArgs a) {
   constexpr int E = Vec<F32>::kE;
   __shared__ float2 turn[kRotateTokens * kMostPairs];
-  __shared__ int64_t k_to[kRotateTokens], v_to[kRotateTokens];  // the token's slot in the pools, -1: in none
-  const int b = blockIdx.y, tid = threadIdx.x, t0 = blockIdx.x * a.per_wg;
-  const int n = min(a.per_wg, a.tokens - t0);
+  const int b = blockIdx.y, tid = threadIdx.x, t0 = blockIdx.x << a.log_tokens;
+  const int n = min(1 << a.log_tokens, a.tokens - t0);
   const int len = max(a.lens[b], 0);
   const int cnt = a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
   const int first = a.seen ? a.seen[b] : len;
   if (blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) a.out_lens[b] = (int)min((int64_t)len + cnt, (int64_t)a.c.capacity);
-  if (tid < n) {
-    const int64_t slot = (int64_t)len + t0 + tid;
-    int64_t k = -1, v = -1;
-    if (t0 + tid < cnt && slot < a.c.capacity) {
-      const int page = page_id(a.c, a.c.table + (int64_t)b * a.c.width, (int)slot);
-      if (page >= 0) {
-        const int off = (int)slot - (int)page_of(a.c.div, (uint32_t)slot) * a.c.div.size;
-        k = page * a.c.k_page + off * a.c.k_slot;
-        v = page * a.c.v_page + off * a.c.v_slot;
-      }
-    }
-    k_to[tid] = k;
-    v_to[tid] = v;
+  // this wave's token, and its slot in the pools
+  const int log_threads = 8 - a.log_tokens, t = __builtin_amdgcn_readfirstlane(tid >> log_threads), token = t0 + t;
+  const bool counts = token < cnt;
+  const int64_t slot = (int64_t)len + token;
+  int page = -1, off = 0;
+  if (counts && slot < a.c.capacity) {
+    const uint32_t in_row = page_of(a.c.div, (uint32_t)slot);
+    page = a.c.table[(uint64_t)(uint32_t)b * (uint32_t)a.c.width + in_row];
+    page = (uint32_t)page < (uint32_t)a.c.pages ? page : -1;
+    off = (int)slot - (int)in_row * a.c.div.size;
   }
   for (int i = tid; i < n * a.pairs; i += 256) {
-    const int t = i / a.pairs, pair = i - t * a.pairs;
-    const int axis = a.pair_axes ? min(max(a.pair_axes[pair], 0), a.axes - 1) : 0;
-    const int64_t p = a.places ? a.places[((int64_t)b * a.tokens + t0 + t) * a.axes + axis] : (int64_t)first + t0 + t;
-    turn[t * a.pairs + pair] = cos_sin_turns((double)p * ((double)a.frequencies[pair] * 0.15915494309189533577));
+    const int u = (int)page_of(a.per_token, (uint32_t)i), pair = i - u * a.pairs;
+    int64_t p = (int64_t)first + t0 + u;
+    if (a.places) {
+      const int axis = a.pair_axes ? min(max(a.pair_axes[pair], 0), a.axes - 1) : 0;
+      p = a.places[((int64_t)b * a.tokens + t0 + u) * a.axes + axis];
+    }
+    turn[i] = cos_sin_turns((double)p * ((double)a.frequencies[pair] * 0.15915494309189533577));
   }
   __syncthreads();
-  const int dim = a.c.dim, vecs = dim / E, rotated = a.heads + a.kv_heads;
-  const int from_values = rotated * a.per_head.size;
-  const int items = n * a.per_token.size;
-  for (int i = blockIdx.z * 256 + tid; i < items; i += gridDim.z * 256) {
-    const int t = (int)page_of(a.per_token, i);
-    int r = i - t * a.per_token.size;
-    const int64_t k_slot = k_to[t], v_slot = v_to[t];
-    if (r >= from_values) {
-      r -= from_values;
-      const int head = (int)page_of(a.per_value, r), v = r - head * a.per_value.size;
-      if (v_slot >= 0)
-        *(uint4*)(a.c.v + v_slot + head * a.c.v_head + v * 16) =
-            *(const uint4*)(a.in[2] + b * a.batch_at[2] + (t0 + t) * a.token_at[2] + head * a.head_at[2] + v * 16);
+  if (t >= n) return;
+  const int dim = a.c.dim, vecs = a.per_value.size, half = a.pairs / E;
+  const int from_values = (a.heads + a.kv_heads) * a.per_head.size, items = from_values + a.kv_heads * vecs;
+  const char* in[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    in[i] = a.in[i] + (((uint64_t)(uint32_t)b * a.batch_at[i] + (uint64_t)(uint32_t)token * a.token_at[i]) << 4);
+  char* out_q = a.out_q + ((uint64_t)(uint32_t)b * (uint32_t)a.tokens + (uint32_t)token) * (uint32_t)(a.heads * vecs) * 16;
+  char* k_to = a.c.k + (uint64_t)(uint32_t)page * (uint64_t)a.c.k_page + (uint32_t)off * a.c.k_slot;
+  char* v_to = a.c.v + (uint64_t)(uint32_t)page * (uint64_t)a.c.v_page + (uint32_t)off * a.c.v_slot;
+  const float2* tr = turn + t * a.pairs;
+  for (int i = (blockIdx.z << log_threads) + (tid & ((1 << log_threads) - 1)); i < items; i += gridDim.z << log_threads) {
+    if (i >= from_values) {
+      const int r = i - from_values, head = (int)page_of(a.per_value, r), v = r - head * vecs;
+      if (page >= 0)
+        *(uint4*)(v_to + head * a.c.v_head + v * 16) = *(const uint4*)(in[2] + (uint64_t)(uint32_t)head * a.head_at[2] + v * 16);
       continue;
     }
-    int head = (int)page_of(a.per_head, r);
-    const int v = r - head * a.per_head.size;
+    int head = (int)page_of(a.per_head, i);
+    const int v = i - head * a.per_head.size;
     const bool key = head >= a.heads;
     head -= key ? a.heads : 0;
-    char* to;
-    if (key) {
-      if (k_slot < 0) continue;
-      to = a.c.k + k_slot + head * a.c.k_head;
-      if (a.scores && v == 0) {
-        const int64_t at = ((int64_t)b * a.kv_heads + head) * a.c.capacity + len + t0 + t;
-        a.scores[at] = 0.0f;
-        a.positions[at] = a.seen[b] + t0 + t;
-      }
-    } else {
-      to = a.out_q + (((int64_t)b * a.tokens + t0 + t) * a.heads + head) * dim * (F32 ? 4 : 2);
-      if (t0 + t >= cnt) {  // a token that does not count
-        const int half = HOW == kHalves ? a.pairs / E : 0;
-        if (v < half) *(uint4*)(to + v * 16) = make_uint4(0, 0, 0, 0);
-        *(uint4*)(to + (v + half) * 16) = make_uint4(0, 0, 0, 0);
-        continue;
-      }
+    if (key && page < 0) continue;
+    char* to = key ? k_to + head * a.c.k_head : out_q + (uint32_t)(head * vecs) * 16;
+    if (!counts) {  // a token that does not count: its query is 0, its key has no slot
+      const uint4 none = make_uint4(0, 0, 0, 0);
+      if (HOW == kHalves && v < half) *(uint4*)(to + v * 16) = none;
+      *(uint4*)(to + (HOW == kHalves ? v + half : v) * 16) = none;
+      continue;
     }
-    const char* from = a.in[key] + b * a.batch_at[key] + (t0 + t) * a.token_at[key] + head * a.head_at[key];
-    const float2* tr = turn + t * a.pairs;
+    if (key && v == 0 && a.scores) {
+      const int64_t s = ((int64_t)b * a.kv_heads + head) * a.c.capacity + slot;
+      a.scores[s] = 0.0f;
+      a.positions[s] = a.seen[b] + token;
+    }
+    const char* from = key ? in[1] + (uint64_t)(uint32_t)head * a.head_at[1] : in[0] + (uint64_t)(uint32_t)head * a.head_at[0];
     Vec<F32> x;
     if constexpr (HOW == kHalves) {
       // the first pairs / E items are vectors of both halves, the others what is not rotated
-      const int half = a.pairs / E;
       if (v < half) {
         Vec<F32> y;
         x.load(from + v * 16);
@@ -193,25 +191,43 @@ __global__ __launch_bounds__(256) void kv_rotate_kernel(RotateArgs a) {
       } else {
         *(uint4*)(to + (v + half) * 16) = *(const uint4*)(from + (v + half) * 16);
       }
-    } else {
+    } else if constexpr (HOW == kNeighbours) {
       x.load(from + v * 16);
-      if (v * E < 2 * a.pairs) {
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const int pair = (v * E + e) / 2;
+        if (pair < a.pairs) {
+          const float2 cs = tr[pair];
+          const float x0 = x.x[e], x1 = x.x[e + 1];
+          x.x[e] = x0 * cs.x - x1 * cs.y;
+          x.x[e + 1] = x1 * cs.x + x0 * cs.y;
+        }
+      }
+      *(uint4*)(to + v * 16) = x.bits();
+    } else {
+      // the partners of a vector's elements are as many elements before or after it, at any alignment
+      x.load(from + v * 16);
+      const int d = v * E;
+      Vec<F32> y;
+      const bool low = d + E <= a.pairs && d + a.pairs + E <= dim, high = d >= a.pairs && d + E <= 2 * a.pairs;
+      if (low || high) {
+        uint4 u;
+        __builtin_memcpy(&u, from + (low ? d + a.pairs : d - a.pairs) * (F32 ? 4 : 2), 16);
+        y.unpack(u);
+      } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const int d = v * E + e;
-          if constexpr (HOW == kNeighbours) {
-            if (e & 1 || d >= 2 * a.pairs) continue;
-            const float2 cs = tr[d / 2];
-            const float x0 = x.x[e], x1 = x.x[e | 1];
-            x.x[e] = x0 * cs.x - x1 * cs.y;
-            x.x[e | 1] = x1 * cs.x + x0 * cs.y;
-          } else if (d < a.pairs) {
-            const float2 cs = tr[d];
-            x.x[e] = x.x[e] * cs.x - element<F32>(from, d + a.pairs) * cs.y;
-          } else if (d < 2 * a.pairs) {
-            const float2 cs = tr[d - a.pairs];
-            x.x[e] = x.x[e] * cs.x + element<F32>(from, d - a.pairs) * cs.y;
-          }
+          const int p = d + e < a.pairs ? d + e + a.pairs : d + e < 2 * a.pairs ? d + e - a.pairs : d + e;
+          y.x[e] = element<F32>(from, p);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int pair = d + e < a.pairs ? d + e : d + e - a.pairs;
+        if (pair < a.pairs) {
+          const float2 cs = tr[pair];
+          const float other = y.x[e] * cs.y;
+          x.x[e] = x.x[e] * cs.x + (d + e < a.pairs ? -other : other);
         }
       }
       *(uint4*)(to + v * 16) = x.bits();
@@ -262,15 +278,16 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
   bool ok = ((uintptr_t)out_q & 15) == 0;
   for (int i = 0; i < 3; ++i) {
     const int64_t s[3] = {fresh->stride_batch[i], fresh->stride_token[i], fresh->stride_head[i]};
-    for (int64_t x : s) ok = ok && x >= 0 && x * es % 16 == 0 && x < ((int64_t)1 << 40);
+    for (int64_t x : s) ok = ok && x >= 0 && x < ((int64_t)1 << 35) && x * es % 16 == 0 && x * es / 16 <= UINT32_MAX;
+    ok = ok && s[2] * es <= UINT32_MAX;
     ok = ok && ((uintptr_t)in[i] & 15) == 0;
     a.in[i] = (const char*)in[i];
-    a.batch_at[i] = s[0] * es;
-    a.token_at[i] = s[1] * es;
-    a.head_at[i] = s[2] * es;
+    a.batch_at[i] = (uint32_t)(s[0] * es / 16);
+    a.token_at[i] = (uint32_t)(s[1] * es / 16);
+    a.head_at[i] = (uint32_t)(s[2] * es);
   }
   if (!ok) {
-    set_error("kv_append_rotated: q, k, v, their strides and out_q must be multiples of 16 bytes");
+    set_error("kv_append_rotated: q, k, v, their strides and out_q must be multiples of 16 bytes, below 2^36, of heads 2^32");
     return kUnsupported;
   }
   a.lens = lens;
@@ -291,16 +308,16 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
   const int e = 16 / (int)es, vecs = cache->dim / e;
   const PairsAre how = turn->neighbours ? kNeighbours : turn->pairs % e == 0 ? kHalves : kHalvesAny;
   const int per_head = how == kHalves ? vecs - a.pairs / e : vecs;
-  const int64_t per_token = (int64_t)(a.heads + a.kv_heads) * per_head + (int64_t)a.kv_heads * vecs;
+  const int64_t items = (int64_t)(a.heads + a.kv_heads) * per_head + (int64_t)a.kv_heads * vecs;
   a.per_head = make_page_div(per_head);
   a.per_value = make_page_div(vecs);
-  a.per_token = make_page_div(per_token);
-  // One token a workgroup while that gives the card no more than it has room for, and then several workgroups to a
-  // token's heads.
+  // A token's threads: 256 unless it has fewer items than that; and several workgroups to one where they are few.
   const int64_t all = (int64_t)cache->batch * a.tokens;
-  a.per_wg = all >= 8192 ? kRotateTokens : 1;
-  const int64_t blocks = a.tokens > 0 ? (a.tokens + a.per_wg - 1) / a.per_wg : 1;
-  int64_t split = (per_token * a.per_wg + 255) / 256;
+  a.per_token = make_page_div(a.pairs);
+  a.log_tokens = items <= 192 ? 2 : items <= 300 ? 1 : 0;
+  while (a.log_tokens > 0 && 1 << (a.log_tokens - 1) >= a.tokens) --a.log_tokens;
+  const int64_t blocks = a.tokens > 0 ? (a.tokens + (1 << a.log_tokens) - 1) >> a.log_tokens : 1;
+  int64_t split = ((items << a.log_tokens) + 255) / 256;
   const int64_t room = all > 0 ? 512 / all : 1;
   split = split < room ? split : room;
   const dim3 grid((unsigned)blocks, (unsigned)cache->batch, (unsigned)(split < 1 ? 1 : split));
