@@ -159,7 +159,14 @@ struct Prefix {
     };
     hand_over(0);
     uint4 kv[2][GROUP][NB];
+    // float32: products of elements past dim, all zeros, are left out in blocks, where the instance has such.  64
+    // sequences x 4 rows of dim 80 behind 8192 slots 53 us, with them 60; in bfloat16 they cost nothing (25.5, 25.6).
+    const int dim = a.own.c.dim;
+    constexpr int SPAN = GROUP * 32 / ES;  // elements of a group of the first product
+    auto in_keys = [&](int g) { return !F32 || g * SPAN <= DP / 2 || g * SPAN < dim; };
+    auto in_values = [&](int j) { return !F32 || 32 * j <= DP / 2 || 32 * j < dim; };
     auto read_keys = [&](int g) {
+      if (!in_keys(g)) return;
 #pragma unroll
       for (int i = 0; i < GROUP; ++i)
 #pragma unroll
@@ -173,6 +180,7 @@ struct Prefix {
       if (g + 1 < QV / GROUP) read_keys(g + 1);
       pass_on(g);
       __builtin_amdgcn_sched_barrier(0);
+      if (!in_keys(g)) continue;
 #pragma unroll
       for (int i = 0; i < GROUP; ++i)
 #pragma unroll
@@ -234,7 +242,7 @@ struct Prefix {
           }
 #pragma unroll
           for (int j = 0; j < ACC; ++j)
-            acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+            if (in_values(j)) acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(
                 lds_read<float>((values ^ (8 * j << 4)) + (32 * u + 8 * (r / 4) + r % 4) * ROW), s[u][r], acc[j], 0, 0, 0);
         }
     } else {
@@ -449,6 +457,39 @@ struct PrefixRows {
   __device__ __forceinline__ float* part_o() const { return a.part_o; }
 };
 
+// A sequence's own slots in one chunk, joined with the parts of its prefix: what comes out are the outputs.
+struct LastRows : OwnRows {
+  const SharedArgs& s;
+  __device__ __forceinline__ LastRows(const SharedArgs& args, int u) : OwnRows(args.own, u), s(args) {}
+  __device__ __forceinline__ bool parts() const { return false; }
+  __device__ __forceinline__ void merge(int row, int d, float4& x, float& m, float& l) const {
+    if (row / a.group >= seen.cnt) return;
+    const int p = b / s.per, len = min(max(s.lens[p], 0), s.max_len), chunks = (len + s.chunk - 1) / s.chunk;
+    const int64_t first = ((int64_t)(p * a.kv_heads + kvh) * s.chunks) * s.rows + (b - p * s.per) * a.rows + row;
+#pragma unroll 4
+    for (int c = 0; c < chunks; ++c) {
+      const int64_t i = first + (int64_t)c * s.rows;
+      const float2 y = s.part_ml[i];
+      const float4 z = *(const float4*)(s.part_o + i * a.c.dim + d);
+      const float top = fmaxf(m, y.x), base = top == -INFINITY ? 0.0f : top;
+      const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(y.x - base);
+      m = top;
+      l = l * f + y.y * g;
+      x.x = x.x * f + z.x * g;
+      x.y = x.y * f + z.y * g;
+      x.z = x.z * f + z.z * g;
+      x.w = x.w * f + z.w * g;
+    }
+  }
+};
+
+template <bool F32, int DP, int MT, bool MANY, int WAVES>
+__global__ __launch_bounds__(kAttnThreads, WAVES) void kv_shared_last_kernel(SharedArgs a) {
+  extern __shared__ float lds[];
+  const int rg = blockIdx.x % a.own.row_groups, unit = blockIdx.x / a.own.row_groups;
+  decode_chunk<F32, DP, MT, MANY>(a.own, LastRows(a, unit), rg, 0, lds);
+}
+
 // Many rows behind a prefix.
 template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
 __global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_shared_tiles_kernel(SharedArgs a) {
@@ -541,6 +582,7 @@ struct SharedPlan {
   int rg;  // groups of 32 rows to a workgroup; 0: few rows
   int step, row_tiles, chunk, chunks;
   AttnPlan own;
+  bool last;  // the sequences' own slots are one chunk each, whose workgroup makes the outputs
   int own_chunks;
   size_t ml_bytes, o_bytes, own_ml_bytes, own_o_bytes;
   size_t bytes() const { return ml_bytes + o_bytes + own_ml_bytes + own_o_bytes; }
@@ -598,10 +640,18 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t quer
       }
     }
   }
-  p->own_chunks = p->own.chunks > 1 ? p->own.chunks : 2;  // with one the kernel would write outputs, not parts
+  // A sequence's own slots in one chunk spare the join's launch and their parts' way, where there are enough of them to
+  // fill the card: 128 sequences x 5 queries with up to 700 slots, 8 kv heads, 134 us, in chunks 157; 64 x 8 kv heads with
+  // up to 1024 60.5 and 64.4; but 8 x 8 with up to 500 44.0 and 40.6, 100 x 1 33.8 and 31.7, and 160 the same.
+  p->last = p->rg && max_len > 0 && c->batch * c->kv_heads * p->own.row_groups >= 256;
+  if (p->last) {
+    p->own.chunk = (int)max_len;
+    p->own.chunks = 1;
+  }
+  p->own_chunks = p->last ? 1 : p->own.chunks > 1 ? p->own.chunks : 2;  // with one the kernel would write outputs, not parts
   p->ml_bytes = align_up((size_t)(units * p->chunks * all) * sizeof(float2), 256);
   p->o_bytes = align_up((size_t)(units * p->chunks * all) * c->dim * 4, 256);
-  const int64_t own = max_len > 0 ? c->batch * c->kv_heads * p->own_chunks * rows : 0;
+  const int64_t own = max_len > 0 && !p->last ? c->batch * c->kv_heads * p->own_chunks * rows : 0;
   p->own_ml_bytes = align_up((size_t)own * sizeof(float2), 256);
   p->own_o_bytes = align_up((size_t)own * c->dim * 4, 256);
 }
@@ -641,6 +691,21 @@ static int launch_dim(const SharedArgs& a, const SharedPlan& p, int64_t groups, 
   if constexpr (F32 || DP <= 128)
     if (p.own.mt == 2) return launch_rows<F32, DP, 2>(a, groups, s);
   return launch_rows<F32, DP, 1>(a, groups, s);
+}
+
+template <bool F32, int DP, int MT>
+static int launch_last_mt(const SharedArgs& a, int64_t groups, hipStream_t s) {
+  constexpr int W1 = F32 && DP > 128 ? 1 : 2, W3 = DP == 128 && MT == 1 ? 3 : W1;
+  if (a.own.queries > 1)
+    return launch_shared(kv_shared_last_kernel<F32, DP, MT, true, W1>, a, groups, decode_lds_bytes<F32, DP, MT, true>(), s);
+  return launch_shared(kv_shared_last_kernel<F32, DP, MT, false, W3>, a, groups, decode_lds_bytes<F32, DP, MT, false>(), s);
+}
+
+template <bool F32, int DP>
+static int launch_last(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
+  if constexpr (F32 || DP <= 128)
+    if (p.own.mt == 2) return launch_last_mt<F32, DP, 2>(a, a.own_units, s);
+  return launch_last_mt<F32, DP, 1>(a, a.own_units, s);
 }
 
 template <bool F32>
@@ -777,6 +842,11 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
   if (groups > 0) {
     st = f32 ? launch_prefix<true>(a, p, groups, s) : launch_prefix<false>(a, p, groups, s);
     if (st != kOk) return st;
+  }
+  if (p.last) {
+    if (o.c.dim <= 64) return f32 ? launch_last<true, 64>(a, p, s) : launch_last<false, 64>(a, p, s);
+    if (o.c.dim <= 128) return f32 ? launch_last<true, 128>(a, p, s) : launch_last<false, 128>(a, p, s);
+    return f32 ? launch_last<true, 256>(a, p, s) : launch_last<false, 256>(a, p, s);
   }
   if (p.rg && own > 0) {
     st = launch_attention(o, p.own, units, f32, s);

@@ -210,6 +210,8 @@ struct OwnRows {
     const int t = row / a.group;
     return ((int64_t)b * a.queries + t) * a.heads + kvh * a.group + (row - t * a.group);
   }
+  // what belongs to an output beside these slots: elements d .. d + 3, maximum and sum of a row
+  __device__ __forceinline__ void merge(int, int, float4&, float&, float&) const {}
   __device__ __forceinline__ int64_t part(int c) const { return ((int64_t)unit * a.chunks + c) * a.rows; }
   __device__ __forceinline__ float2* part_ml() const { return a.part_ml; }
   __device__ __forceinline__ float* part_o() const { return a.part_o; }
@@ -484,12 +486,13 @@ __device__ __forceinline__ void decode_chunk(const AttnArgs& a, const Rows& rows
         o.z += x.z;
         o.w += x.w;
       }
-      const float rm = ml[kAttnWaves * 32 + 2 * rn], rl = ml[kAttnWaves * 32 + 2 * rn + 1];
+      float rm = ml[kAttnWaves * 32 + 2 * rn], rl = ml[kAttnWaves * 32 + 2 * rn + 1];
       if (rows.parts()) {
         const int64_t at = rows.part(chunk) + row;
         *(float4*)(rows.part_o() + at * a.c.dim + d) = o;
         if (d == 0) rows.part_ml()[at] = make_float2(rm, rl);
       } else if constexpr (Rows::kOutputs) {
+        rows.merge(row, d, o, rm, rl);
         const float inv = rl == 0.0f ? 0.0f : 1.0f / rl;
         const int64_t head = rows.output(row);
         const bool none = rl == 0.0f;

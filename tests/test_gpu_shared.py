@@ -252,3 +252,38 @@ def test_refusals(gpu):
     for i, bad in ((0, q), (3, d[3].repeat(1, 2)[:, ::2]), (4, begins), (5, table), (0, None)):
         with pytest.raises(ValueError):
             kvcache.decode_shared(*d[:i], bad, *d[i + 1:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,queries,group", [(64, 1, 3), (128, 1, 2), (128, 3, 2), (128, 5, 4), (256, 1, 2), (80, 2, 12),
+                                               (192, 2, 3), (64, 1, 18)])
+def test_many_sequences(gpu, dtype, dim, queries, group):
+    """Enough of them that the workgroup of a sequence's own slots makes the outputs: lengths of zero, tables of several
+    pages, counts of none and too many, pages that are missing, a prefix that is empty."""
+    rng = np.random.default_rng(dim + queries)
+    batch, kv_heads = 132, 2
+    lens = [0 if i % 11 == 5 else queries + (i * 7) % 150 for i in range(batch)]
+    args = _make(rng, lens, [333, 0, 70], queries, kv_heads * group, kv_heads, dim, 16, dtype, fill=math.nan)
+    q, k, v, prefix, begins, table, own = args
+    counts = torch.from_numpy(rng.integers(-1, queries + 3, batch).astype(np.int32))
+    _both(gpu, args, counts=counts)
+    table, prefix = table.clone(), prefix.clone()
+    table[3], table[7, 0], prefix[0, [1, 5]] = -1, 99999, -1
+    out, lse = _both(gpu, (q, k, v, prefix, begins, table, own))
+    _both(gpu, (q, k, v, prefix, begins * 0, table, own))
+    _both(gpu, (q, k, v, prefix, begins, table, own * 0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_many_sequences_with_values_that_are_not_finite(gpu, dtype):
+    rng = np.random.default_rng(14)
+    q, k, v, prefix, begins, table, lens = _make(rng, [20] * 140, [100, 90], 2, 4, 2, 64, 16, dtype)
+    v[int(prefix[1, 2]), 1, 3, 5] = math.inf  # seen by the second prefix's sequences, by kv head 1
+    v[int(table[1, 1]), 0, 3, 9] = math.nan   # slot 19: seen by the last query alone
+    v[int(table[2, 0]), 0, 3, 7] = -math.inf
+    out, _ = _run(gpu, (q, k, v, prefix, begins, table, lens))
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    bad[70:, :, 2:, 5] = True
+    bad[1, 1, :2, 9] = True
+    bad[2, :, :2, 7] = True
+    assert torch.equal(~torch.isfinite(out.cpu().float()), bad)
