@@ -379,7 +379,8 @@ int tallax_kv_decode(const tallax_kv_cache* cache, const void* q, int64_t q_stri
  * seen[b] + t (seen null: lens[b] + t).  Angles are computed in 64 bits.
  * The turned keys and the values go to the cache as tallax_kv_append's do,
  * the turned queries to out_q [batch, tokens, heads, dim] (dense), 0 for
- * tokens from counts[b] on.  seen may be given without scores.
+ * tokens from counts[b] on.  seen may be given without scores.  Up to 2^23
+ * tokens of a sequence; strides of q, k and v below 2^36 bytes, of heads 2^32.
  * ---------------------------------------------------------------------- */
 typedef struct tallax_kv_tokens {
   const void* q;
@@ -411,8 +412,8 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
  * b / (batch / prefixes) = p.  Query t < counts[b] sees the whole prefix and
  * what it sees in tallax_kv_decode of its sequence's own slots (block_table,
  * lens); queries from counts[b] on see nothing.  max_prefix bounds prefix_lens
- * as max_len bounds lens.  Workspace: tallax_kv_decode_shared_workspace_size
- * bytes, on a multiple of 16.
+ * as max_len bounds lens.  batch * queries * heads is below 2^24.  Workspace:
+ * tallax_kv_decode_shared_workspace_size bytes, on a multiple of 16.
  * ---------------------------------------------------------------------- */
 size_t tallax_kv_decode_shared_workspace_size(const tallax_kv_cache* cache, int64_t prefixes, int64_t prefix_width,
                                               int64_t queries, int64_t heads, int64_t max_prefix, int64_t max_len);
@@ -487,7 +488,8 @@ int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, in
  * nothing to a group, and are chosen after all others of the chosen groups,
  * lowest first, with weight 0.  +inf logits and infinite biases count as the
  * largest finite ones.  experts up to 1024, groups up to 64, k up to 64 and to
- * top_groups * experts / groups.  out_weights f32, out_ids int32 [tokens, k].
+ * top_groups * experts / groups, tokens up to 2^25.  out_weights f32, out_ids
+ * int32 [tokens, k].
  * ---------------------------------------------------------------------- */
 int tallax_route(const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t row_stride, int64_t k,
                  int sigmoid, const float* bias, int64_t groups, int64_t top_groups, int group_top, int renormalise,

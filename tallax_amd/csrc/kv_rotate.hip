@@ -252,9 +252,9 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
     set_error("kv_append_rotated: null tokens or rotation");
     return kInvalidArgument;
   }
-  if (fresh->tokens < 0 || fresh->tokens > (1 << 24) || fresh->heads < 1 || turn->pairs < 1 ||
+  if (fresh->tokens < 0 || fresh->tokens > (1 << 23) || fresh->heads < 1 || turn->pairs < 1 ||
       2 * turn->pairs > cache->dim || turn->axes < 1) {
-    set_error("kv_append_rotated: %lld tokens (0 to 2^24), %lld heads, %lld pairs of %d elements, %lld axes",
+    set_error("kv_append_rotated: %lld tokens (0 to 2^23), %lld heads, %lld pairs of %d elements, %lld axes",
               (long long)fresh->tokens, (long long)fresh->heads, (long long)turn->pairs, cache->dim,
               (long long)turn->axes);
     return kInvalidArgument;

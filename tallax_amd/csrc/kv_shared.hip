@@ -789,8 +789,8 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
   if (st != kOk) return st;
   const int64_t units = cache->batch * cache->kv_heads, pieces = prefixes * cache->kv_heads * p.chunks;
   const int64_t all = cache->batch * queries * heads;
-  if (units * p.own.row_groups * p.own.chunks + (pieces + 8) * p.row_tiles > INT32_MAX ||
-      cache->batch * rows > INT32_MAX / 64 || all > INT32_MAX) {
+  const int64_t most = (1 << 24) - 1;  // workgroups of 256 threads, of which HIP counts below 2^32
+  if (units * p.own.row_groups * p.own.chunks + (pieces + 8) * p.row_tiles > most || all > most || p.own.chunks > 65535) {
     set_error("kv_decode_shared: too many workgroups");
     return kUnsupported;
   }

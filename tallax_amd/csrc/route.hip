@@ -620,9 +620,9 @@ int tallax_route(const void* logits, int logits_dtype, int64_t tokens, int64_t e
     set_error("route: scale must be finite in float32");
     return kInvalidArgument;
   }
-  if (experts > kMostExperts || groups > kMostGroups || k > kMostChosen || tokens > ((int64_t)1 << 31) ||
+  if (experts > kMostExperts || groups > kMostGroups || k > kMostChosen || tokens > (1 << 25) ||
       row_stride > ((int64_t)1 << 31)) {
-    set_error("route: up to %d experts, %d groups, %d chosen, 2^31 tokens", kMostExperts, kMostGroups, kMostChosen);
+    set_error("route: up to %d experts, %d groups, %d chosen, 2^25 tokens", kMostExperts, kMostGroups, kMostChosen);
     return kUnsupported;
   }
   if (tokens == 0) return kOk;

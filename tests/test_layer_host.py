@@ -35,7 +35,8 @@ def test_append_rotated_refuses_on_the_host():
                    (dict(scores=4), inv), (dict(positions=4), inv), (dict(scores=4, positions=4), inv),
                    (dict(q=24), uns), (dict(k=24), uns), (dict(v=17), uns), (dict(out_q=24), uns),
                    (dict(head_at=(60, 64, 64)), uns), (dict(token_at=(256, -128, 128)), uns),
-                   (dict(batch_at=(256, 128, 4)), uns)):
+                   (dict(batch_at=(256, 128, 4)), uns), (dict(tokens=(1 << 23) + 1), inv),
+                   (dict(head_at=(1 << 31, 64, 64)), uns), (dict(token_at=(1 << 35, 128, 128)), uns)):
         assert _rotate(c, **kw) == st, kw
         assert _lib.LIB.tallax_last_error()
     assert _lib.LIB.tallax_kv_append_rotated(ctypes.byref(c), 4, None, None, None, None, None, None, 16, 8, None) == inv
@@ -71,6 +72,9 @@ def test_decode_shared_refuses_on_the_host():
     far = dict(dim=8, page_size=1, kv_heads=1, k_stride_page=24, v_stride_page=24, k_stride_slot=8, v_stride_slot=8)
     assert _shared(_cache(pages=2 ** 31 - 1, **far), heads=1, max_len=4, max_prefix=4) == uns
     assert b"2^32" in _lib.LIB.tallax_last_error()
+    many = _cache(batch=65535, pages=1 << 20)
+    assert _shared(many, queries=256, heads=2, qt=128, nws=1 << 62) == uns
+    assert b"workgroups" in _lib.LIB.tallax_last_error()
     assert _shared(_cache(batch=0), prefixes=0) == _lib.OK
     size = _lib.LIB.tallax_kv_decode_shared_workspace_size
     assert size(ctypes.byref(c), 2, 4, 1, 4, 64, 64) == 0 == size(ctypes.byref(c), 1, 4, 0, 4, 64, 64)
@@ -94,7 +98,8 @@ def test_route_refuses_on_the_host():
                    (dict(k=0), inv), (dict(k=33), inv), (dict(group_top=3), inv), (dict(stride=-1), inv),
                    (dict(scale=math.nan), inv), (dict(scale=math.inf), inv), (dict(scale=1e39), inv),
                    (dict(experts=2048), uns), (dict(experts=1024, groups=128, top_groups=128), uns),
-                   (dict(experts=1024, groups=1, top_groups=1, k=65), uns), (dict(logits=None), inv),
+                   (dict(experts=1024, groups=1, top_groups=1, k=65), uns), (dict(tokens=(1 << 25) + 1), uns),
+                   (dict(logits=None), inv),
                    (dict(weights=None), inv), (dict(ids=None), inv)):
         assert _route(**kw) == st, kw
         assert _lib.LIB.tallax_last_error()
