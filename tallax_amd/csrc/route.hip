@@ -495,6 +495,8 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
       for (int i = 0; i < L; ++i) key[i] = kNone;
     }
   }
+  // the lists' ends: what a lane had no room for comes after its own
+  const int end = n > L ? key[L - 1] : kNone;
   int mine = kNone, from = 0;  // lane i: choice i, and the lane it is from
 #pragma unroll 1
   for (int i = 0; i < a.k; ++i) {
@@ -513,6 +515,8 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
   if (!exact) {
     const int next = row_max(key[0]);
     const bool edge = (l == a.k - 1) & close(mine, next);  // of the last choice and the next
+    // where a lane's whole list may be chosen, or next: whether the last choice is as near to what it had no room for
+    if (a.k >= L - 1) near = near | ((l == a.k - 1) & close(mine, row_max(end)));
     order = (l > 0) & (l < a.k) & close(row_ror<1>(mine), mine);
     if (__ballot(edge & valid)) {  // then the next is a choice too, of which one is left out
       if (a.k == 16) {

@@ -201,3 +201,16 @@ def test_large_logits_and_biases(gpu, dtype):
                         assert np.array_equal(got, ids), kw
                         assert (np.abs(w - want) <= np.abs(want) * 32 * L.F32 + 2.0 ** -148).all()
                     assert np.isfinite(w).all()
+
+
+@pytest.mark.parametrize("k", [6, 7, 8, 15, 16])
+@pytest.mark.parametrize("bias", [False, True])
+def test_neighbours_that_rise_by_the_smallest_steps(gpu, k, bias):
+    """The largest experts lie next to each other, and more of them than are chosen differ in their last bits alone."""
+    x = np.full((9, 512), -3.0, np.float32)
+    for t in range(9):
+        x[t, 32 * t:32 * t + 32] = 1.0 + np.arange(32) * 2.0 ** -23
+    b = np.zeros(512) if bias else None
+    for groups, top in ((1, 1), (8, 2)):
+        for score in ("softmax", "sigmoid"):
+            _check(gpu, x, k, "f32", b, score=score, groups=groups, top_groups=top)
