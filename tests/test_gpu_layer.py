@@ -145,3 +145,36 @@ def test_inputs_are_left_as_they_were(gpu):
     step()
     now = (step.qkv, step.table, step.prefix, step.lens, step.begins, step.f, step.logits, step.bias)
     assert all(torch.equal(a, b) for a, b in zip(kept, now, strict=True))
+
+
+@pytest.mark.parametrize("heads_first", [False, True])
+@pytest.mark.parametrize("batch", [3, 20, 70])
+def test_pools_of_more_than_32_bits(gpu, batch, heads_first):
+    """The last pages of pools of 6.5 GB, page after page or head after head, against a pool of their own."""
+    step = Step(gpu, batch, 16, 8, 128, torch.bfloat16, seed=7)
+    pages, kv_heads, page, dim = step.k.shape
+    start = step.k.clone(), step.v.clone()
+    want = [x.clone() for x in step()]
+    kept = step.k, step.v
+    many = 6_500_000_000 // (kv_heads * page * dim * 2)
+    shape = (kv_heads, many, page, dim) if heads_first else (many, kv_heads, page, dim)
+    far = [torch.empty(shape, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    step.k, step.v = [x.transpose(0, 1) if heads_first else x for x in far]
+    for pool, first in zip((step.k, step.v), start, strict=True):
+        pool[-pages:] = first
+    for table in (step.table, step.prefix):
+        table[table >= 0] += many - pages
+    got = step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+    assert torch.equal(step.k[-pages:], kept[0]) and torch.equal(step.v[-pages:], kept[1])
+
+
+@pytest.mark.parametrize("batch", [2, 40, 70])
+def test_pools_without_a_page(gpu, batch):
+    """Every token is dropped and nothing is seen."""
+    step = Step(gpu, batch, 8, 4, 128, torch.bfloat16, seed=8)
+    q = step()[1]
+    step.k, step.v = step.k[:0], step.v[:0]
+    lens, turned, out, lse, _, _ = step()
+    assert torch.equal(q, turned) and torch.equal(lens, step.lens + 1)
+    assert not bool(out.any()) and bool((lse == -float("inf")).all())
