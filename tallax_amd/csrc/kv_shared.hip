@@ -29,6 +29,7 @@ struct SharedArgs {
   int row_tiles, chunk, chunks;
   int pieces;            // chunks of all kv heads of all prefixes
   int own_units;         // workgroups of a chunk of the sequences' own slots
+  int own_from;          // the first of them, where the prefix's are tiles
   uint32_t flip;         // sign bits of q, where the scale is negative
   float scale2;          // its size, above 0: -inf, of what is not seen, stays -inf
   float2* part_ml;       // [prefixes * kv_heads][chunks][rows]: maximum (base 2), sum
@@ -57,7 +58,7 @@ __device__ __forceinline__ T lds_read(uint32_t at) {
   return *(const __attribute__((address_space(3))) T*)(lds_char*)at;
 }
 
-template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
+template <bool F32, int DP, int RG, int TG, int WT>
 struct Prefix {
   static constexpr int ES = F32 ? 4 : 2, NW = RG * TG, kThreads = NW * kWave;
   static constexpr int VECS = DP * ES / 16;               // 16-byte vectors of a token's key
@@ -286,9 +287,9 @@ struct Prefix {
 };
 
 // Rows 32 RG times the tile's number and on of a prefix's kv head, over one chunk: workgroup f of those for prefixes.
-template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
+template <bool F32, int DP, int RG, int TG, int WT>
 __device__ __forceinline__ void prefix_chunk(const SharedArgs& a, int f, uint4* tiles) {
-  using P = Prefix<F32, DP, RG, TG, WT, WAVES>;
+  using P = Prefix<F32, DP, RG, TG, WT>;
   constexpr int NW = P::NW, PAD = P::PAD, STEP = P::STEP;
 
   // The row tiles of a piece (chunk of a prefix's kv head) are workgroups of one XCD, that follow one another: their
@@ -494,7 +495,20 @@ __global__ __launch_bounds__(kAttnThreads, WAVES) void kv_shared_last_kernel(Sha
 template <bool F32, int DP, int RG, int TG, int WT, int WAVES>
 __global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_shared_tiles_kernel(SharedArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint4 tiles[];  // [2][TG][keys, values][WT * VECS]
-  prefix_chunk<F32, DP, RG, TG, WT, WAVES>(a, blockIdx.x, tiles);
+  prefix_chunk<F32, DP, RG, TG, WT>(a, blockIdx.x, tiles);
+}
+
+// The same, and the sequences' own slots in the same launch.
+template <bool F32, int DP, int RG, int TG, int WT, int MT, int WAVES>
+__global__ __launch_bounds__(RG * TG * kWave, WAVES) void kv_shared_both_kernel(SharedArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) uint4 tiles[];
+  const int i = (int)blockIdx.x - a.own_from;
+  if (i < 0) {
+    prefix_chunk<F32, DP, RG, TG, WT>(a, blockIdx.x, tiles);
+  } else {
+    const int chunk = i / a.own_units, k = i - chunk * a.own_units, unit = k / a.own.row_groups;
+    decode_chunk<F32, DP, MT, true>(a.own, OwnRows(a.own, unit), k - unit * a.own.row_groups, chunk, (float*)tiles);
+  }
 }
 
 // Few rows behind a prefix, and the sequences' own slots in the same launch.
@@ -582,6 +596,7 @@ struct SharedPlan {
   int rg;  // groups of 32 rows to a workgroup; 0: few rows
   int step, row_tiles, chunk, chunks;
   AttnPlan own;
+  bool both;  // tiles, and the sequences' own slots in the same launch
   bool last;  // the sequences' own slots are one chunk each, whose workgroup makes the outputs
   int own_chunks;
   size_t ml_bytes, o_bytes, own_ml_bytes, own_o_bytes;
@@ -640,14 +655,21 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t quer
       }
     }
   }
-  // A sequence's own slots in one chunk spare the join's launch and their parts' way, where there are enough of them to
-  // fill the card: 128 sequences x 5 queries with up to 700 slots, 8 kv heads, 134 us, in chunks 157; 64 x 8 kv heads with
-  // up to 1024 60.5 and 64.4; but 8 x 8 with up to 500 44.0 and 40.6, 100 x 1 33.8 and 31.7, and 160 the same.
-  p->last = p->rg && max_len > 0 && c->batch * c->kv_heads * p->own.row_groups >= 256;
+  // The sequences' own slots, behind tiles.  In the same launch, where the tiles' workgroups are all on the card at once:
+  // both take each other's time (32 / 8 heads of 128 behind 2048 slots, up to 512 of their own: 31 sequences 27.8 us, one
+  // launch after the other 33.8; 64 behind 8192 42.9 and 45.3 in one chunk each, 128 66.4 and 75.9), but not where a
+  // workgroup has a CU for itself and there is one on each (64 sequences, 4 / 2 heads of 256: 47.7 and 44.7).
+  // Or each sequence in one chunk after the tiles, where there are enough of them to fill the card: their workgroups make
+  // the outputs, which spares the join and their parts' way.  So where the prefix is short next to its rows (128 sequences
+  // behind 512: 49.6 and 56.0), or the decode kernel needs the registers that tiles leave it less of: two sixteens of
+  // rows (128 x 5 queries behind 4099: 137 and 162), float32 (50 x 8 heads, one a kv head, behind 1024: 55 and 65).
+  p->last = p->rg && max_len > 0 && c->batch * c->kv_heads * p->own.row_groups >= 256 &&
+            (f32 || p->own.mt == 2 || max_prefix < 4 * all);
   if (p->last) {
     p->own.chunk = (int)max_len;
     p->own.chunks = 1;
   }
+  p->both = p->rg && max_len > 0 && !p->last && units * p->row_tiles * p->chunks <= (tile_waves(f32, c->dim, p->rg) == 2 ? 512 : 255);
   p->own_chunks = p->last ? 1 : p->own.chunks > 1 ? p->own.chunks : 2;  // with one the kernel would write outputs, not parts
   p->ml_bytes = align_up((size_t)(units * p->chunks * all) * sizeof(float2), 256);
   p->o_bytes = align_up((size_t)(units * p->chunks * all) * c->dim * 4, 256);
@@ -670,9 +692,17 @@ static int launch_shared(K kernel, const SharedArgs& a, int64_t groups, int byte
 }
 
 template <bool F32, int DP, int RG>
-static int launch_tiles(const SharedArgs& a, int64_t groups, hipStream_t s) {
+static int launch_tiles(const SharedArgs& a, const SharedPlan& p, int64_t groups, hipStream_t s) {
   constexpr int TG = kAttnWaves / RG, WT = tile_tokens(F32, DP, RG), WAVES = tile_waves(F32, DP, RG);
-  return launch_shared(kv_shared_tiles_kernel<F32, DP, RG, TG, WT, WAVES>, a, groups, Prefix<F32, DP, RG, TG, WT, WAVES>::kBytes, s);
+  constexpr int kBytes = Prefix<F32, DP, RG, TG, WT>::kBytes;
+  if (!p.both) return launch_shared(kv_shared_tiles_kernel<F32, DP, RG, TG, WT, WAVES>, a, groups, kBytes, s);
+  constexpr int kOwn = decode_lds_bytes<F32, DP, 1, true>(), kMost = kBytes > kOwn ? kBytes : kOwn;
+  if constexpr (F32 || DP <= 128) {
+    constexpr int kOwn2 = decode_lds_bytes<F32, DP, 2, true>();
+    if (p.own.mt == 2)
+      return launch_shared(kv_shared_both_kernel<F32, DP, RG, TG, WT, 2, WAVES>, a, groups, kBytes > kOwn2 ? kBytes : kOwn2, s);
+  }
+  return launch_shared(kv_shared_both_kernel<F32, DP, RG, TG, WT, 1, WAVES>, a, groups, kMost, s);
 }
 
 template <bool F32, int DP, int MT>
@@ -685,9 +715,9 @@ static int launch_rows(const SharedArgs& a, int64_t groups, hipStream_t s) {
 
 template <bool F32, int DP>
 static int launch_dim(const SharedArgs& a, const SharedPlan& p, int64_t groups, hipStream_t s) {
-  if (p.rg == 4) return launch_tiles<F32, DP, 4>(a, groups, s);
+  if (p.rg == 4) return launch_tiles<F32, DP, 4>(a, p, groups, s);
   if constexpr (!F32 || DP <= 128)
-    if (p.rg == 2) return launch_tiles<F32, DP, 2>(a, groups, s);
+    if (p.rg == 2) return launch_tiles<F32, DP, 2>(a, p, groups, s);
   if constexpr (F32 || DP <= 128)
     if (p.own.mt == 2) return launch_rows<F32, DP, 2>(a, groups, s);
   return launch_rows<F32, DP, 1>(a, groups, s);
@@ -838,7 +868,8 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
   a.pieces = a.max_len > 0 ? (int)pieces : 0;
   a.own_units = (int)(units * p.own.row_groups);
   const int64_t own = max_len > 0 ? (int64_t)a.own_units * p.own.chunks : 0;
-  const int64_t groups = p.rg ? ((int64_t)a.pieces + 7) / 8 * 8 * p.row_tiles : a.pieces + own;
+  a.own_from = (int)(((int64_t)a.pieces + 7) / 8 * 8 * p.row_tiles);
+  const int64_t groups = !p.rg ? a.pieces + own : p.both ? a.own_from + own : a.own_from;
   if (groups > 0) {
     st = f32 ? launch_prefix<true>(a, p, groups, s) : launch_prefix<false>(a, p, groups, s);
     if (st != kOk) return st;
@@ -848,7 +879,7 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
     if (o.c.dim <= 128) return f32 ? launch_last<true, 128>(a, p, s) : launch_last<false, 128>(a, p, s);
     return f32 ? launch_last<true, 256>(a, p, s) : launch_last<false, 256>(a, p, s);
   }
-  if (p.rg && own > 0) {
+  if (p.rg && !p.both && own > 0) {
     st = launch_attention(o, p.own, units, f32, s);
     if (st != kOk) return st;
   }
