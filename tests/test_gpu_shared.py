@@ -287,3 +287,40 @@ def test_many_sequences_with_values_that_are_not_finite(gpu, dtype):
     bad[1, 1, :2, 9] = True
     bad[2, :, :2, 7] = True
     assert torch.equal(~torch.isfinite(out.cpu().float()), bad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,queries,group", [(64, 1, 5), (64, 1, 20), (64, 3, 3), (128, 1, 6), (128, 3, 2), (128, 5, 4),
+                                               (256, 1, 5), (256, 2, 12), (80, 2, 12), (192, 2, 3)])
+def test_one_launch(gpu, dtype, dim, queries, group):
+    """Too few sequences to make the outputs, too many rows for the kernel of few, and tiles that fill less than the card:
+    a prefix's tiles and the sequences' own slots side by side, in one chunk of these and in several."""
+    rng = np.random.default_rng(dim + queries)
+    batch, kv_heads = 39, 2
+    for longest in (150, 900):
+        lens = [0 if i % 11 == 5 else queries + (i * 7) % longest for i in range(batch)]
+        lens[0] = longest
+        args = _make(rng, lens, [333, 0, 1070], queries, kv_heads * group, kv_heads, dim, 16, dtype, fill=math.nan)
+        q, k, v, prefix, begins, table, own = args
+        counts = torch.from_numpy(rng.integers(-1, queries + 3, batch).astype(np.int32))
+        _both(gpu, args, counts=counts)
+        table, prefix = table.clone(), prefix.clone()
+        table[3], table[7, 0], prefix[0, [1, 5]] = -1, 99999, -1
+        _both(gpu, (q, k, v, prefix, begins, table, own))
+        _both(gpu, (q, k, v, prefix, begins * 0, table, own))
+    _both(gpu, (q, k, v, prefix, begins, table, own * 0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_launch_with_values_that_are_not_finite(gpu, dtype):
+    rng = np.random.default_rng(15)
+    q, k, v, prefix, begins, table, lens = _make(rng, [20] * 40, [100, 90], 2, 4, 2, 64, 16, dtype)
+    v[int(prefix[1, 2]), 1, 3, 5] = math.inf  # seen by the second prefix's sequences, by kv head 1
+    v[int(table[1, 1]), 0, 3, 9] = math.nan   # slot 19: seen by the last query alone
+    v[int(table[2, 0]), 0, 3, 7] = -math.inf
+    out, _ = _run(gpu, (q, k, v, prefix, begins, table, lens))
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    bad[20:, :, 2:, 5] = True
+    bad[1, 1, :2, 9] = True
+    bad[2, :, :2, 7] = True
+    assert torch.equal(~torch.isfinite(out.cpu().float()), bad)
