@@ -1,18 +1,36 @@
-// Attention of the newest tokens of sequences that begin with a shared prefix.
+// Attention of the newest tokens of sequences that begin with a shared prefix:
+// x = scale q.k over the prefix's slots and the sequence's own, w = exp(x - lse),
+// out = sum w v.  A chunk of either gives its rows' maximum m, l = sum 2^(x - m)
+// and sum 2^(x - m) v (x in base 2); two of them join as m = max, l = l1 2^(m1 - m)
+// + l2 2^(m2 - m), and so the outputs.
 //
 // The prefix's slots are taken for all its sequences at once: the rows of a kv
 // head (sequence, query and head of the group, in this order) are the columns
 // of two matrix products,
-//   S^T = K Q^T   (tokens x rows),   O^T = V^T P^T   (dim x rows),
-// of which a workgroup computes 32 * RG rows over a chunk of the prefix.  The
-// sequences' own slots are kv_attention.hip's; the join puts both together.
+//   S^T = K Q^T   (tokens x rows),   O^T = V^T P^T   (dim x rows).
+// Up to 32 rows (16 in bfloat16 above dim 128): kv_shared_rows_kernel, by the
+// products of tx_decode.h.  More: kv_shared_tiles_kernel, of which a workgroup
+// computes 32 * RG rows over a chunk of the prefix.  The sequences' own slots are
+// always tx_decode.h's: in the same launch (kv_shared_rows_kernel,
+// kv_shared_both_kernel), or after the prefix's (kv_shared_last_kernel, which makes
+// the outputs, and kv_decode_kernel); plan_shared has the rules.  Where nothing
+// else does, kv_shared_join_kernel makes the outputs.
 //
-// A workgroup has RG * TG waves: wave (rg, tg) takes 32 rows and every TG-th
-// tile of WT tokens, which its RG waves bring into LDS together, through
+// A workgroup of tiles has RG * TG waves: wave (rg, tg) takes 32 rows and every
+// TG-th tile of WT tokens, which its RG waves bring into LDS together, through
 // registers and one tile ahead.  In S^T a lane holds one row's scores, so that
 // weights are the second operand of the second product as they lie; its first
 // operand, values by dim, is read transposed from LDS (bfloat16), or in single
 // elements (float32).
+//
+// Up to some 100 rows the bytes bound it, beyond that the products, whose weights
+// take as many cycles of the vector units (an exponential of 16, and some eight
+// operations of 4, to each 64 scores): 20 rows of each of 128 sequences behind 4099
+// slots of 8 heads of 128, 43 GFLOP, 72 us in the tiles, 600 TFLOP/s, the matrix
+// units busy a quarter of the cycles; 16 x 64 / 8 heads behind 131071 slots with up
+// to 300 of their own, 69 GFLOP and 550 MB, 114 us and 10.5 in the join (reading
+// alone 115); 64 x 32 / 8 heads behind 8192 with up to 1024, 203 MB, 51 and 10.5;
+// float32, 3 x 12 heads of 80 behind three times 2050 slots with up to 333, 18 and 5.
 #include "tx_decode.h"
 
 namespace tx {

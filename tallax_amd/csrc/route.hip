@@ -1,5 +1,16 @@
-// Routing tokens to experts: scores, the choice of groups, the choice of
-// experts and their weights, a wave for each token.
+// Routing tokens to experts: scores s = softmax(x) or 1 / (1 + exp(-x)), keys
+// s + bias, the choice of groups by their largest key or the sum of two, the choice
+// of the k largest keys in them, and the weights s (over their sum) times scale.
+// What is chosen is what 64-bit keys choose.
+//
+// Four tokens a wave and 32-bit keys, for up to 16 chosen of up to 16 groups
+// (route_kernel); a wave for each token, all in 64 bits, for others and for the
+// tokens whose 32-bit keys leave a choice open (route_exactly).  A row of logits is
+// read once or twice, the second time from the cache, and little else: 16384 tokens
+// of 256 float32 experts in 8 groups, sigmoid with a bias, the two largest, 17.8 MB,
+// take 13.1 us, where reading them takes 3.7.  What bounds it is its instructions:
+// some 10 us are a wave's way through the code, new to the CU, and 2.3 the few waves
+// with a comparison in 64 bits.  130 tokens take 6.8 us, one of 64 experts 3.1.
 #include <math.h>
 
 #include "tx_common.h"
