@@ -8,6 +8,7 @@
 // head (sequence, query and head of the group, in this order) are the columns
 // of two matrix products,
 //   S^T = K Q^T   (tokens x rows),   O^T = V^T P^T   (dim x rows).
+// Short prefixes are read by each sequence (kv_shared_whole_kernel): one launch.
 // Up to 32 rows (16 in bfloat16 above dim 128): kv_shared_rows_kernel, by the
 // products of tx_decode.h.  More: kv_shared_tiles_kernel, of which a workgroup
 // computes 32 * RG rows over a chunk of the prefix.  The sequences' own slots are
@@ -465,6 +466,8 @@ struct PrefixRows {
   __device__ __forceinline__ int limit(int) const { return length; }
   __device__ __forceinline__ int open() const { return length; }
   __device__ __forceinline__ const int32_t* table() const { return a.table + (int64_t)p * a.width; }
+  __device__ __forceinline__ const int32_t* table_of(const int32_t* own, int) const { return own; }
+  __device__ __forceinline__ int slot_of(int t) const { return t; }
   __device__ __forceinline__ const char* query(int row) const {
     const AttnArgs& o = a.own;
     const int seq = row / o.rows, rr = row - seq * o.rows, t = rr / o.group;
@@ -501,6 +504,35 @@ struct LastRows : OwnRows {
     }
   }
 };
+
+// A sequence's prefix and its own slots, one after the other, as its queries' rows see them.
+struct WholeRows : OwnRows {
+  const int32_t* front;
+  int first;  // slots of the prefix
+  __device__ __forceinline__ WholeRows(const SharedArgs& s, int u) : OwnRows(s.own, u) {
+    const int p = b / s.per;
+    front = s.table + (int64_t)p * s.width;
+    first = min(max(s.lens[p], 0), s.max_len);
+  }
+  __device__ __forceinline__ int len() const { return first + seen.len; }
+  __device__ __forceinline__ int chunk() const { return first + seen.len; }
+  __device__ __forceinline__ bool parts() const { return false; }
+  __device__ __forceinline__ int limit(int row) const {
+    const int t = row / a.group;
+    return t < seen.cnt ? first + max(seen.limit(t), 0) : 0;
+  }
+  __device__ __forceinline__ int open() const { return first + max(seen.first, 0); }
+  __device__ __forceinline__ const int32_t* table_of(const int32_t* own, int t) const { return t < first ? front : own; }
+  __device__ __forceinline__ int slot_of(int t) const { return t < first ? t : t - first; }
+};
+
+// Short prefixes and lengths: each sequence reads all of its own.
+template <bool F32, int DP, int MT, bool MANY, int WAVES>
+__global__ __launch_bounds__(kAttnThreads, WAVES) void kv_shared_whole_kernel(SharedArgs a) {
+  extern __shared__ float lds[];
+  const int rg = blockIdx.x % a.own.row_groups, unit = blockIdx.x / a.own.row_groups;
+  decode_chunk<F32, DP, MT, MANY>(a.own, WholeRows(a, unit), rg, 0, lds);
+}
 
 template <bool F32, int DP, int MT, bool MANY, int WAVES>
 __global__ __launch_bounds__(kAttnThreads, WAVES) void kv_shared_last_kernel(SharedArgs a) {
@@ -614,6 +646,7 @@ struct SharedPlan {
   int rg;  // groups of 32 rows to a workgroup; 0: few rows
   int step, row_tiles, chunk, chunks;
   AttnPlan own;
+  bool whole;  // each sequence's prefix and own slots in one chunk: of the others own.mt and own.row_groups count alone
   bool both;  // tiles, and the sequences' own slots in the same launch
   bool last;  // the sequences' own slots are one chunk each, whose workgroup makes the outputs
   int own_chunks;
@@ -634,6 +667,21 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t quer
   const int64_t all = c->batch / prefixes * rows, units = prefixes * c->kv_heads;
   const int most = f32 || c->dim <= 128 ? 2 : 1;  // sixteens of rows that the kernel for few takes
   plan_attention(c->batch, c->kv_heads, rows, c->dim, c->dtype, max_len, false, &p->own);
+  // One workgroup for a sequence's prefix and own slots, without parts and their join, takes some 5.4 us and 1 us for 100
+  // slots in bfloat16 at dim 128 (0.7 at 64, 2 at 256; two to three times that in float32), and longer where there are more of
+  // them than the card holds; the other ways take 10 to 11 us with few rows and 14 and more with tiles.  Sequences of 32 / 8
+  // heads of 128 behind 250 slots with up to 60 of their own: 4 of them 8.6 us, else 11.4, 32 8.9 and 15.8, 128 20.4 and 25.4;
+  // behind 1000 with up to 100: 4 16.4 and 10.9, 16 16.6 and 15.5; 16 in float32 behind 250 15.7 and 19.7, 500 25.4 and 20.4.
+  const int64_t units_all = c->batch * c->kv_heads * p->own.row_groups;
+  const double most_slots = (all <= 16 * most ? 105e3 : 210e3) / (c->dim + 64) / (f32 ? 3 : 1) / (1 + units_all / 1024.0);
+  p->whole = (double)(max_prefix + max_len) <= most_slots;
+  if (p->whole) {
+    const AttnPlan own = p->own;
+    *p = SharedPlan{};
+    p->own = own;
+    p->whole = true;
+    return;
+  }
   if (all <= 16 * most) {
     p->rg = 0;
     p->own.mt = all <= 16 ? 1 : 2;
@@ -742,8 +790,12 @@ static int launch_dim(const SharedArgs& a, const SharedPlan& p, int64_t groups, 
 }
 
 template <bool F32, int DP, int MT>
-static int launch_last_mt(const SharedArgs& a, int64_t groups, hipStream_t s) {
+static int launch_last_mt(const SharedArgs& a, const SharedPlan& p, int64_t groups, hipStream_t s) {
   constexpr int W1 = F32 && DP > 128 ? 1 : 2, W3 = DP == 128 && MT == 1 ? 3 : W1;
+  if (p.whole && a.own.queries > 1)
+    return launch_shared(kv_shared_whole_kernel<F32, DP, MT, true, W1>, a, groups, decode_lds_bytes<F32, DP, MT, true>(), s);
+  if (p.whole)
+    return launch_shared(kv_shared_whole_kernel<F32, DP, MT, false, W3>, a, groups, decode_lds_bytes<F32, DP, MT, false>(), s);
   if (a.own.queries > 1)
     return launch_shared(kv_shared_last_kernel<F32, DP, MT, true, W1>, a, groups, decode_lds_bytes<F32, DP, MT, true>(), s);
   return launch_shared(kv_shared_last_kernel<F32, DP, MT, false, W3>, a, groups, decode_lds_bytes<F32, DP, MT, false>(), s);
@@ -752,8 +804,8 @@ static int launch_last_mt(const SharedArgs& a, int64_t groups, hipStream_t s) {
 template <bool F32, int DP>
 static int launch_last(const SharedArgs& a, const SharedPlan& p, hipStream_t s) {
   if constexpr (F32 || DP <= 128)
-    if (p.own.mt == 2) return launch_last_mt<F32, DP, 2>(a, a.own_units, s);
-  return launch_last_mt<F32, DP, 1>(a, a.own_units, s);
+    if (p.own.mt == 2) return launch_last_mt<F32, DP, 2>(a, p, a.own_units, s);
+  return launch_last_mt<F32, DP, 1>(a, p, a.own_units, s);
 }
 
 template <bool F32>
@@ -887,12 +939,12 @@ int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_
   a.own_units = (int)(units * p.own.row_groups);
   const int64_t own = max_len > 0 ? (int64_t)a.own_units * p.own.chunks : 0;
   a.own_from = (int)(((int64_t)a.pieces + 7) / 8 * 8 * p.row_tiles);
-  const int64_t groups = !p.rg ? a.pieces + own : p.both ? a.own_from + own : a.own_from;
+  const int64_t groups = p.whole ? 0 : !p.rg ? a.pieces + own : p.both ? a.own_from + own : a.own_from;
   if (groups > 0) {
     st = f32 ? launch_prefix<true>(a, p, groups, s) : launch_prefix<false>(a, p, groups, s);
     if (st != kOk) return st;
   }
-  if (p.last) {
+  if (p.last || p.whole) {
     if (o.c.dim <= 64) return f32 ? launch_last<true, 64>(a, p, s) : launch_last<false, 64>(a, p, s);
     if (o.c.dim <= 128) return f32 ? launch_last<true, 128>(a, p, s) : launch_last<false, 128>(a, p, s);
     return f32 ? launch_last<true, 256>(a, p, s) : launch_last<false, 256>(a, p, s);

@@ -202,6 +202,9 @@ struct OwnRows {
   __device__ __forceinline__ int limit(int row) const { return seen.limit(row / a.group); }
   __device__ __forceinline__ int open() const { return seen.first; }
   __device__ __forceinline__ const int32_t* table() const { return a.c.table + (int64_t)b * a.c.width; }
+  // where token t of the list lies: in which table's row (of the one above, or another), and in which slot of it
+  __device__ __forceinline__ const int32_t* table_of(const int32_t* own, int) const { return own; }
+  __device__ __forceinline__ int slot_of(int t) const { return t; }
   __device__ __forceinline__ const char* query(int row) const {
     const int t = row / a.group;
     return a.q + b * a.q_batch + t * a.q_query + (int64_t)(kvh * a.group + row - t * a.group) * a.q_head;
@@ -243,7 +246,10 @@ __device__ __forceinline__ void decode_chunk(const AttnArgs& a, const Rows& rows
   const char* vbase = a.c.v + rows.kvh * a.c.v_head;
   const int32_t* table = rows.table();
   const int mine = lane & (T::kTokens - 1);
-  auto page_at = [&](int t0) { return t0 + mine < end ? page_id(a.c, table, t0 + mine) : -1; };
+  auto page_at = [&](int t0) {
+    const int t = t0 + mine;
+    return t < end ? page_id(a.c, rows.table_of(table, t), rows.slot_of(t)) : -1;
+  };
   int t0 = start + wave * T::kTokens;
   // Each lane works out the place of one token and hands it to those that load
   // from it.  Tokens past the end or in no page are read from a query.
@@ -253,7 +259,7 @@ __device__ __forceinline__ void decode_chunk(const AttnArgs& a, const Rows& rows
     uint32_t k, v;
   };
   auto places_of = [&](int t, int page) {
-    const int off = t + mine - (int)page_of(a.c.div, (uint32_t)(t + mine)) * a.c.div.size;
+    const int slot = rows.slot_of(t + mine), off = slot - (int)page_of(a.c.div, (uint32_t)slot) * a.c.div.size;
     return Places{page, (uint32_t)page * a.at.k_page + (uint32_t)off * a.at.k_slot,
                   (uint32_t)page * a.at.v_page + (uint32_t)off * a.at.v_slot};
   };

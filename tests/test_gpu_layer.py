@@ -21,13 +21,13 @@ def example():
     return module
 
 
-@pytest.mark.parametrize("samples", [3, 40])
-def test_a_prompt_kept_once_changes_no_token(gpu, example, samples):
+@pytest.mark.parametrize("samples,length", [(3, 67), (40, 67), (3, 1111), (20, 1111)])
+def test_a_prompt_kept_once_changes_no_token(gpu, example, samples, length):
     """In float32 and greedily, samples behind shared prompts decode what they decode with prompts of their own."""
     model = example.Model(vocab=1500, hidden=256, heads=6, kv_heads=3, dim=40, n_experts=24, dtype=torch.float32)
     gen = torch.Generator(device=gpu)
     gen.manual_seed(10)
-    prompts = torch.randint(0, 1500, (2, 67), generator=gen, device=gpu, dtype=torch.int32)
+    prompts = torch.randint(0, 1500, (2, length), generator=gen, device=gpu, dtype=torch.int32)
     own = example.generate(model, prompts, samples, 24, shared=False)
     once = example.generate(model, prompts, samples, 24)
     assert torch.equal(own, once)
@@ -87,10 +87,11 @@ SHAPES = [(3, 4, 2, 64, torch.bfloat16), (20, 8, 4, 128, torch.bfloat16), (70, 8
           (70, 4, 4, 80, torch.float32), (9, 4, 2, 256, torch.float32)]
 
 
+@pytest.mark.parametrize("prefix", [300, 2500])
 @pytest.mark.parametrize("shape", SHAPES)
-def test_a_captured_step(gpu, shape):
+def test_a_captured_step(gpu, shape, prefix):
     """Captured without a run before; each replay, with new inputs and eager work between them, is the eager result."""
-    step = Step(gpu, *shape, seed=1)
+    step = Step(gpu, *shape, seed=1, prefix=prefix)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         held = step()
@@ -104,9 +105,10 @@ def test_a_captured_step(gpu, shape):
         assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True)), i
 
 
-def test_two_captured_steps_of_one_workspace(gpu):
+@pytest.mark.parametrize("prefix", [300, 2500])
+def test_two_captured_steps_of_one_workspace(gpu, prefix):
     """Two graphs, replayed one after the other in turn, whose calls use the same workspace."""
-    steps = [Step(gpu, *SHAPES[2], seed=2), Step(gpu, *SHAPES[1], seed=3)]
+    steps = [Step(gpu, *SHAPES[2], seed=2, prefix=prefix), Step(gpu, *SHAPES[1], seed=3, prefix=prefix)]
     steps[1].ws = steps[0].ws
     graphs, held = [], []
     for s in steps:
@@ -123,8 +125,9 @@ def test_two_captured_steps_of_one_workspace(gpu):
         assert all(torch.equal(a, b) for a, b in zip(held[i], want[i], strict=True)), i
 
 
-def test_two_streams_at_once(gpu):
-    steps = [Step(gpu, *SHAPES[2], seed=4), Step(gpu, *SHAPES[3], seed=5)]
+@pytest.mark.parametrize("prefix", [300, 2500])
+def test_two_streams_at_once(gpu, prefix):
+    steps = [Step(gpu, *SHAPES[2], seed=4, prefix=prefix), Step(gpu, *SHAPES[3], seed=5, prefix=prefix)]
     want = [[x.clone() for x in s()] for s in steps]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(gpu) for _ in steps]
@@ -148,10 +151,10 @@ def test_inputs_are_left_as_they_were(gpu):
 
 
 @pytest.mark.parametrize("heads_first", [False, True])
-@pytest.mark.parametrize("batch", [3, 20, 70])
-def test_pools_of_more_than_32_bits(gpu, batch, heads_first):
+@pytest.mark.parametrize("batch,prefix", [(3, 300), (3, 2500), (20, 300), (20, 2500), (70, 2500)])
+def test_pools_of_more_than_32_bits(gpu, batch, prefix, heads_first):
     """The last pages of pools of 6.5 GB, page after page or head after head, against a pool of their own."""
-    step = Step(gpu, batch, 16, 8, 128, torch.bfloat16, seed=7)
+    step = Step(gpu, batch, 16, 8, 128, torch.bfloat16, seed=7, prefix=prefix)
     pages, kv_heads, page, dim = step.k.shape
     start = step.k.clone(), step.v.clone()
     want = [x.clone() for x in step()]
@@ -169,10 +172,11 @@ def test_pools_of_more_than_32_bits(gpu, batch, heads_first):
     assert torch.equal(step.k[-pages:], kept[0]) and torch.equal(step.v[-pages:], kept[1])
 
 
+@pytest.mark.parametrize("prefix", [300, 2500])
 @pytest.mark.parametrize("batch", [2, 40, 70])
-def test_pools_without_a_page(gpu, batch):
+def test_pools_without_a_page(gpu, batch, prefix):
     """Every token is dropped and nothing is seen."""
-    step = Step(gpu, batch, 8, 4, 128, torch.bfloat16, seed=8)
+    step = Step(gpu, batch, 8, 4, 128, torch.bfloat16, seed=8, prefix=prefix)
     q = step()[1]
     step.k, step.v = step.k[:0], step.v[:0]
     lens, turned, out, lse, _, _ = step()

@@ -324,3 +324,68 @@ def test_one_launch_with_values_that_are_not_finite(gpu, dtype):
     bad[1, 1, :2, 9] = True
     bad[2, :, :2, 7] = True
     assert torch.equal(~torch.isfinite(out.cpu().float()), bad)
+
+
+def _wide(args, slots=6000):
+    """The same with room for many slots in the tables, by which both parts are split."""
+    q, k, v, prefix, begins, table, lens = args
+    pad = torch.full((prefix.shape[0], -(-slots // k.shape[2])), -1, dtype=torch.int32)
+    return q, k, v, torch.cat([prefix, pad], 1).contiguous(), begins, table, lens
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [1, 16, 17, 31, 32, 33, 64, 65, 129, 260])
+def test_wide_tables_rows_around_the_tiles(gpu, dtype, rows):
+    rng = np.random.default_rng(rows)
+    for slots in (2000, 20000):
+        _both(gpu, _wide(_make(rng, [3] * rows, [150], 1, 1, 1, 64, 16, dtype), slots))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("batch", [4, 40, 80])
+def test_wide_tables_prefixes_around_the_tiles(gpu, dtype, dim, batch):
+    rng = np.random.default_rng(dim + batch)
+    for prefix in (1, 31, 33, 64, 65, 127, 129, 257, 513):
+        _both(gpu, _wide(_make(rng, [2] * batch, [prefix], 1, 1, 1, dim, 16, dtype)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("batch", [3, 40, 130])
+@pytest.mark.parametrize("dim", [40, 64, 128, 256])
+def test_wide_tables_unused_slots_and_pages(gpu, dtype, batch, dim):
+    rng = np.random.default_rng(5)
+    args = _wide(_make(rng, [20 + i % 3 for i in range(batch)], [77], 1, 2, 1, dim, 16, dtype, fill=math.nan))
+    _both(gpu, args)
+    q, k, v, prefix, begins, table, lens = args
+    prefix, table = prefix.clone(), table.clone()
+    prefix[0, [0, 3]] = torch.tensor([-1, 99999], dtype=torch.int32)
+    table[0] = -1
+    _both(gpu, (q, k, v, prefix, begins, table, lens))
+    _both(gpu, (q, k, v, prefix, begins * 0, table, lens))
+    _both(gpu, (q, k, v, prefix, begins, table, lens * 0))
+    out, lse = _both(gpu, (q, k, v, prefix * 0 - 1, begins, table * 0 - 1, lens))
+    assert not bool(out.any()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("batch", [3, 40, 130])
+@pytest.mark.parametrize("wide", [False, True])
+def test_queries_in_front_of_their_first_slot(gpu, dtype, batch, wide):
+    """More queries than own slots: the first see the prefix alone, those from counts on nothing; values that are not
+    finite reach those that see them."""
+    rng = np.random.default_rng(16)
+    lens = [i % 5 for i in range(2 * batch)]
+    q, k, v, prefix, begins, table, own = _make(rng, lens, [100, 90], 4, 4, 2, 64, 16, dtype, fill=math.nan)
+    args = q, k, v, prefix, begins, table, own
+    args = _wide(args) if wide else args
+    _both(gpu, args)
+    counts = torch.tensor([(3 * i) % 7 - 1 for i in range(2 * batch)], dtype=torch.int32)
+    _both(gpu, args, counts=counts)
+    v[int(table[4, 0]), 0, 3, 9] = math.inf  # sequence 4's newest slot: its last query's alone
+    v[int(prefix[0, 2]), 1, 3, 5] = math.nan
+    out, _ = _run(gpu, args)
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    bad[:batch, :, 2:, 5] = True
+    bad[4, 3, :2, 9] = True
+    assert torch.equal(~torch.isfinite(out.cpu().float()), bad)
