@@ -15,8 +15,7 @@
 // of 80, float32, three axes, 173 MB, 30 us by itself and 42 among other calls, whose
 // data then are in the caches.  A token each of 64 sequences takes 4.6 us, the launch
 // and a chain of loads (length, table, tokens); 65 pairs of 192 elements, partners
-// off the vectors' alignment, 395 MB in 125 us (3.2 TB/s): each vector is read as
-// itself and as its partner, and looks up twice the angles of aligned ones.
+// off the vectors' alignment, 395 MB in 101 us (3.9 TB/s).
 #include "tx_common.h"
 #include "tx_kv.h"
 
@@ -110,12 +109,21 @@ __device__ __forceinline__ float element(const char* p, int i) {
   return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
 }
 
-// How pairs lie: (i, i + pairs) in whole vectors, in any number, or (2i, 2i + 1).
-enum PairsAre { kHalves = 0, kHalvesAny = 1, kNeighbours = 2 };
+// 16 bytes at any address.
+__device__ __forceinline__ uint4 load_any(const char* p) {
+  uint4 u;
+  __builtin_memcpy(&u, p, 16);
+  return u;
+}
+__device__ __forceinline__ void store_any(char* p, uint4 u) { __builtin_memcpy(p, &u, 16); }
+
+// How pairs lie: (i, i + pairs) in whole vectors, in any number, or (2i, 2i + 1); kHalvesOver: in any number that fills a
+// vector, and so does what is not rotated, or there is nothing.
+enum PairsAre { kHalves = 0, kHalvesAny = 1, kNeighbours = 2, kHalvesOver = 3 };
 
 template <bool F32, int HOW>
 __global__ __launch_bounds__(256) void kv_rotate_kernel(RotateArgs a) {
-  constexpr int E = Vec<F32>::kE;
+  constexpr int E = Vec<F32>::kE, ES = F32 ? 4 : 2;
   __shared__ float2 turn[kRotateTokens * kMostPairs];
   const int b = blockIdx.y, tid = threadIdx.x, t0 = blockIdx.x << a.log_tokens;
   const int n = min(1 << a.log_tokens, a.tokens - t0);
@@ -170,8 +178,8 @@ __global__ __launch_bounds__(256) void kv_rotate_kernel(RotateArgs a) {
     char* to = key ? k_to + head * a.c.k_head : out_q + (uint32_t)(head * vecs) * 16;
     if (!counts) {  // a token that does not count: its query is 0, its key has no slot
       const uint4 none = make_uint4(0, 0, 0, 0);
-      if (HOW == kHalves && v < half) *(uint4*)(to + v * 16) = none;
-      *(uint4*)(to + (HOW == kHalves ? v + half : v) * 16) = none;
+      *(uint4*)(to + v * 16) = none;
+      if (v + a.per_head.size < vecs) *(uint4*)(to + (v + a.per_head.size) * 16) = none;
       continue;
     }
     if (key && v == 0 && a.scores) {
@@ -212,6 +220,28 @@ __global__ __launch_bounds__(256) void kv_rotate_kernel(RotateArgs a) {
         }
       }
       *(uint4*)(to + v * 16) = x.bits();
+    } else if constexpr (HOW == kHalvesOver) {
+      // both halves, then what is not rotated, each in whole vectors at any alignment; the last of them begins inside the
+      // one before it, and writes the same there
+      const int low = (a.pairs + E - 1) / E, rest = 2 * a.pairs;
+      if (v < low) {
+        const int d = min(v * E, a.pairs - E);
+        Vec<F32> y;
+        x.unpack(load_any(from + d * ES));
+        y.unpack(load_any(from + (d + a.pairs) * ES));
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float2 cs = tr[d + e];
+          const float x0 = x.x[e], x1 = y.x[e];
+          x.x[e] = x0 * cs.x - x1 * cs.y;
+          y.x[e] = x1 * cs.x + x0 * cs.y;
+        }
+        store_any(to + d * ES, x.bits());
+        store_any(to + (d + a.pairs) * ES, y.bits());
+      } else {
+        const int d = min(rest + (v - low) * E, dim - E);
+        store_any(to + d * ES, load_any(from + d * ES));
+      }
     } else {
       // the partners of a vector's elements are as many elements before or after it, at any alignment
       x.load(from + v * 16);
@@ -219,9 +249,7 @@ __global__ __launch_bounds__(256) void kv_rotate_kernel(RotateArgs a) {
       Vec<F32> y;
       const bool low = d + E <= a.pairs && d + a.pairs + E <= dim, high = d >= a.pairs && d + E <= 2 * a.pairs;
       if (low || high) {
-        uint4 u;
-        __builtin_memcpy(&u, from + (low ? d + a.pairs : d - a.pairs) * (F32 ? 4 : 2), 16);
-        y.unpack(u);
+        y.unpack(load_any(from + (low ? d + a.pairs : d - a.pairs) * ES));
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -314,8 +342,16 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
   a.seen = seen;
   a.out_lens = out_lens;
   const int e = 16 / (int)es, vecs = cache->dim / e;
-  const PairsAre how = turn->neighbours ? kNeighbours : turn->pairs % e == 0 ? kHalves : kHalvesAny;
-  const int per_head = how == kHalves ? vecs - a.pairs / e : vecs;
+  // Halves that are no whole vectors: in vectors over each other in bfloat16 (4 x 4096 tokens of 32 + 2 x 8 heads of 128, 33
+  // pairs 96 us, each vector as itself and as a partner 121; of 80, 36 pairs 44 and 61), not in float32, whose vectors hold
+  // half as many elements and whose other way is at the memory's rate (35 of 128 83 and 80.5), nor where single elements are
+  // left (63 of 128 109 and 103, 5 121 and 108).
+  const int left = cache->dim - 2 * a.pairs;
+  const bool over = es == 2 && a.pairs >= e && (left == 0 || left >= e);
+  const PairsAre how = turn->neighbours ? kNeighbours : a.pairs % e == 0 ? kHalves : over ? kHalvesOver : kHalvesAny;
+  const int per_head = how == kHalves       ? vecs - a.pairs / e
+                       : how == kHalvesOver ? (a.pairs + e - 1) / e + (left + e - 1) / e
+                                            : vecs;
   const int64_t items = (int64_t)(a.heads + a.kv_heads) * per_head + (int64_t)a.kv_heads * vecs;
   a.per_head = make_page_div(per_head);
   a.per_value = make_page_div(vecs);
@@ -336,6 +372,7 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
     else kv_rotate_kernel<true, kNeighbours><<<grid, 256, 0, s>>>(a);
   } else {
     if (how == kHalves) kv_rotate_kernel<false, kHalves><<<grid, 256, 0, s>>>(a);
+    else if (how == kHalvesOver) kv_rotate_kernel<false, kHalvesOver><<<grid, 256, 0, s>>>(a);
     else if (how == kHalvesAny) kv_rotate_kernel<false, kHalvesAny><<<grid, 256, 0, s>>>(a);
     else kv_rotate_kernel<false, kNeighbours><<<grid, 256, 0, s>>>(a);
   }

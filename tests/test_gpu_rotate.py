@@ -230,3 +230,23 @@ def test_refusals(gpu):
         a = {**good, **over}
         with pytest.raises(ValueError):
             kvcache.append_rotated(k, v, table, lens, a.pop("q"), a.pop("k_new"), a.pop("v_new"), a.pop("frequencies"), **a)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,pairs", [(128, 33), (80, 20), (80, 36), (192, 65), (96, 9), (128, 60), (24, 8), (40, 16),
+                                       (128, 63), (24, 9), (256, 124), (16, 5)])
+def test_halves_off_the_vectors(gpu, dtype, dim, pairs):
+    """Halves of any number of pairs, also with tokens that do not count and tokens that have no slot."""
+    rng = np.random.default_rng(dim + pairs)
+    for tokens, heads, kv_heads in ((1, 4, 2), (9, 8, 8), (3, 40, 20)):
+        counts = torch.tensor([tokens, 0, tokens - 1], dtype=torch.int32)
+        _case(gpu, rng, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, pairs=pairs, dtype=dtype)
+        out = _case(gpu, rng, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, pairs=pairs, dtype=dtype, counts=counts)
+        assert not bool(out[1].any()) and not bool(out[2, -1].any())
+
+        def cut(table):
+            table = table.clone()
+            table[:, 1] = -1
+            return table
+
+        _case(gpu, rng, tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, pairs=pairs, dtype=dtype, table=cut)
