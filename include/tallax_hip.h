@@ -413,7 +413,8 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
  * what it sees in tallax_kv_decode of its sequence's own slots (block_table,
  * lens); queries from counts[b] on see nothing.  max_prefix bounds prefix_lens
  * as max_len bounds lens.  batch * queries * heads is below 2^24.  Workspace:
- * tallax_kv_decode_shared_workspace_size bytes, on a multiple of 16.
+ * tallax_kv_decode_shared_workspace_size bytes (0 where lengths are short), on a
+ * multiple of 16.
  * ---------------------------------------------------------------------- */
 size_t tallax_kv_decode_shared_workspace_size(const tallax_kv_cache* cache, int64_t prefixes, int64_t prefix_width,
                                               int64_t queries, int64_t heads, int64_t max_prefix, int64_t max_len);

@@ -65,8 +65,9 @@ def test_decode_shared_refuses_on_the_host():
                      (dict(out=None), inv), (dict(prefix_lens=None), inv), (dict(table=None), inv), (dict(q=18), uns),
                      (dict(qh=63), uns), (dict(qb=-256), uns), (dict(out=24), uns), (dict(max_len=65), inv),
                      (dict(max_len=-1), inv), (dict(max_prefix=65), inv), (dict(max_prefix=-1), inv),
-                     (dict(ws=None), _lib.WORKSPACE_TOO_SMALL), (dict(nws=64), _lib.WORKSPACE_TOO_SMALL),
-                     (dict(ws=264), inv)):
+                     (dict(width=512, max_prefix=8192, ws=None), _lib.WORKSPACE_TOO_SMALL),
+                     (dict(width=512, max_prefix=8192, nws=64), _lib.WORKSPACE_TOO_SMALL),
+                     (dict(width=512, max_prefix=8192, ws=264), inv)):
         assert _shared(c, **over) == st, over
         assert _lib.LIB.tallax_last_error()
     far = dict(dim=8, page_size=1, kv_heads=1, k_stride_page=24, v_stride_page=24, k_stride_slot=8, v_stride_slot=8)
@@ -78,8 +79,9 @@ def test_decode_shared_refuses_on_the_host():
     assert _shared(_cache(batch=0), prefixes=0) == _lib.OK
     size = _lib.LIB.tallax_kv_decode_shared_workspace_size
     assert size(ctypes.byref(c), 2, 4, 1, 4, 64, 64) == 0 == size(ctypes.byref(c), 1, 4, 0, 4, 64, 64)
-    assert size(ctypes.byref(c), 3, 4, 1, 4, 64, 64) > 0
-    assert size(ctypes.byref(c), 1, 4, 1, 4, -1, -1) == size(ctypes.byref(c), 1, 4, 1, 4, 64, 64)
+    assert size(ctypes.byref(c), 3, 4, 1, 4, 64, 64) == 0  # short ones need none
+    assert size(ctypes.byref(c), 3, 512, 1, 4, 8192, 64) > 0
+    assert size(ctypes.byref(c), 1, 512, 1, 4, -1, -1) == size(ctypes.byref(c), 1, 512, 1, 4, 8192, 64) > 0
 
 
 def _route(**over):
