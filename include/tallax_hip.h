@@ -406,7 +406,8 @@ int tallax_kv_append_rotated(const tallax_kv_cache* cache, const int32_t* lens, 
 
 /* ------------------------------------------------------------------------
  * tallax_kv_decode (without scores) for sequences that begin with a shared
- * prefix, whose keys and values are read once for all of them.  prefix_table
+ * prefix, whose keys and values are read once for all of them, or by each where
+ * prefix and lengths are short.  prefix_table
  * [prefixes, prefix_width] int32 and prefix_lens [prefixes] int32 are a block
  * table and lengths in the same pools; sequences b of prefix p are those with
  * b / (batch / prefixes) = p.  Query t < counts[b] sees the whole prefix and

@@ -111,7 +111,7 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                   scale: float | None = None, counts: torch.Tensor | None = None, max_prefix: int | None = None,
                   max_len: int | None = None,
                   workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """decode, for sequences that begin with a shared prefix, which is read once for all of them.
+    """decode, for sequences that begin with a shared prefix, which is read once for all of them (a short one by each).
 
     prefix_table [prefixes, prefix_width] int32 and prefix_lens [prefixes]
     int32: the pages, in the same pools, and the slots of each prefix.  batch

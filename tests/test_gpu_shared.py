@@ -389,3 +389,40 @@ def test_queries_in_front_of_their_first_slot(gpu, dtype, batch, wide):
     bad[:batch, :, 2:, 5] = True
     bad[4, 3, :2, 9] = True
     assert torch.equal(~torch.isfinite(out.cpu().float()), bad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0, 1e-30])
+def test_wide_tables_scales(gpu, dtype, scale):
+    rng = np.random.default_rng(17)
+    for batch in (2, 40, 140):
+        args = _wide(_make(rng, [7] * batch, [130], 1, 4, 2, 64, 16, dtype, q_scale=1.0))
+        _both(gpu, args, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("batch", [2, 40, 140])
+def test_wide_tables_scores_that_grow_and_shrink(gpu, dtype, batch):
+    rng = np.random.default_rng(18)
+    for slope in (0.5, -0.5):
+        q, k, v, prefix, begins, table, lens = _make(rng, [40] * batch, [1500], 1, 4, 2, 64, 8, dtype)
+        q[..., 0] = 8.0
+        for i in range(1500):
+            k[int(prefix[0, i // 8]), 0, i % 8, 0] = slope * i
+        _both(gpu, (q, k, v, prefix, begins, table, lens))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("batch", [3, 30, 130])
+def test_wide_tables_layouts(gpu, dtype, batch):
+    from tallax_amd import kvcache
+    rng = np.random.default_rng(19)
+    args = _wide(_make(rng, [9 + i % 9 for i in range(batch)], [500], 2, 4, 2, 48, 8, dtype))
+    want = _both(gpu, args)
+    q, k, v, *rest = (x.to(gpu) for x in args)
+    k2, v2 = (y.transpose(1, 2).contiguous().transpose(1, 2) for y in (k, v))
+    big = torch.zeros((batch, 2, 12, 48), dtype=dtype, device=gpu)
+    big[:, :, 4:8] = q
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)
+    for qq, kk, vv in ((q, k2, v2), (big[:, :, 4:8], k, v), (turned, k2, v)):
+        assert all(torch.equal(a, b) for a, b in zip(kvcache.decode_shared(qq, kk, vv, *rest), want, strict=True))
