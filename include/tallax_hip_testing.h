@@ -68,6 +68,17 @@ int tallax_testing_verify_steps(const int32_t* draft, const void* logits, int lo
                                 int32_t* out_tokens, int32_t* out_accepted, void* workspace, size_t workspace_bytes,
                                 tallax_stream_t stream, int stat_steps, int race_steps);
 
+/* How tallax_kv_decode_shared runs a call of these arguments (max_prefix and
+ * max_len -1: what the tables hold): out[0] 0 each sequence its whole list in
+ * one launch, 1 few rows, 2 tiles and the sequences' own slots in one launch,
+ * 3 tiles, then own slots in one chunk each that make the outputs, 4 tiles,
+ * then tallax_kv_decode's kernel, then the join; out[1] groups of 32 rows to a
+ * workgroup of tiles, out[2] sixteens of rows to one of the own slots, out[3]
+ * workgroups that share those rows, out[4] chunks of a prefix, out[5] of a
+ * sequence's own slots.  Host only: no device work. */
+int tallax_testing_shared_plan(const tallax_kv_cache* cache, int64_t prefixes, int64_t prefix_width, int64_t queries,
+                               int64_t heads, int64_t max_prefix, int64_t max_len, int32_t* out);
+
 /* Reads nbytes of src with `width`-byte loads (4, 8 or 16; src aligned to it,
  * nbytes a multiple of it) and writes one word per workgroup to out (2048
  * words): the calibration launch for the FETCH_SIZE counter. */

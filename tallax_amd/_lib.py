@@ -105,6 +105,7 @@ _SIGNATURES = {
     "tallax_testing_lds_atomic_order": ([_c_p, _c_i64, _c_int, _c_p, _c_p], _c_int),
     "tallax_testing_select_plan": ([_c_i64, _c_i64, _c_int, _c_p], _c_int),
     "tallax_testing_select_route": ([_c_i64, _c_i64, _c_int, _c_int, _c_p], _c_int),
+    "tallax_testing_shared_plan": ([_c_kv, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p], _c_int),
     "tallax_testing_top_dynamic_k_path": ([_c_p, _c_int, _c_i64, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_int,
                                            _c_int, _c_int, _c_d, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p, _c_int],
                                           _c_int),

@@ -32,6 +32,7 @@
 // to 300 of their own, 69 GFLOP and 550 MB, 114 us and 10.5 in the join (reading
 // alone 115); 64 x 32 / 8 heads behind 8192 with up to 1024, 203 MB, 51 and 10.5;
 // float32, 3 x 12 heads of 80 behind three times 2050 slots with up to 333, 18 and 5.
+#include "tallax_hip_testing.h"
 #include "tx_decode.h"
 
 namespace tx {
@@ -744,6 +745,21 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t quer
   p->own_o_bytes = align_up((size_t)own * c->dim * 4, 256);
 }
 
+// The plan of a call; false where its arguments are not those of one.
+static bool plan_call(const tallax_kv_cache* cache, int64_t prefixes, int64_t prefix_width, int64_t queries, int64_t heads,
+                      int64_t max_prefix, int64_t max_len, SharedPlan* p) {
+  KvView v;
+  if (make_kv_view(cache, "kv_decode_shared", &v) != kOk || cache->batch < 1 || queries < 1 || queries > 1024 ||
+      heads < 1 || heads % cache->kv_heads || prefixes < 1 || cache->batch % prefixes || prefix_width < 0 ||
+      prefix_width > (1 << 25) / cache->page_size)
+    return false;
+  if (max_len < 0 || max_len > v.capacity) max_len = v.capacity;
+  const int64_t most = prefix_width * cache->page_size;
+  if (max_prefix < 0 || max_prefix > most) max_prefix = most;
+  plan_shared(cache, prefixes, queries, heads / cache->kv_heads, max_prefix, max_len, p);
+  return true;
+}
+
 template <class K>
 static int launch_shared(K kernel, const SharedArgs& a, int64_t groups, int bytes, hipStream_t s) {
   if (bytes > 48 * 1024) {
@@ -822,17 +838,24 @@ extern "C" {
 
 size_t tallax_kv_decode_shared_workspace_size(const tallax_kv_cache* cache, int64_t prefixes, int64_t prefix_width,
                                               int64_t queries, int64_t heads, int64_t max_prefix, int64_t max_len) {
-  KvView v;
-  if (make_kv_view(cache, "kv_decode_shared", &v) != kOk || cache->batch < 1 || queries < 1 || queries > 1024 ||
-      heads < 1 || heads % cache->kv_heads || prefixes < 1 || cache->batch % prefixes || prefix_width < 0 ||
-      prefix_width > (1 << 25) / cache->page_size)
-    return 0;
-  if (max_len < 0 || max_len > v.capacity) max_len = v.capacity;
-  const int64_t most = prefix_width * cache->page_size;
-  if (max_prefix < 0 || max_prefix > most) max_prefix = most;
   SharedPlan p;
-  plan_shared(cache, prefixes, queries, heads / cache->kv_heads, max_prefix, max_len, &p);
-  return p.bytes();
+  return plan_call(cache, prefixes, prefix_width, queries, heads, max_prefix, max_len, &p) ? p.bytes() : 0;
+}
+
+int tallax_testing_shared_plan(const tallax_kv_cache* cache, int64_t prefixes, int64_t prefix_width, int64_t queries,
+                               int64_t heads, int64_t max_prefix, int64_t max_len, int32_t* out) {
+  SharedPlan p;
+  if (!out || !plan_call(cache, prefixes, prefix_width, queries, heads, max_prefix, max_len, &p)) {
+    set_error("bad arguments");
+    return kInvalidArgument;
+  }
+  out[0] = p.whole ? 0 : !p.rg ? 1 : p.both ? 2 : p.last ? 3 : 4;
+  out[1] = p.rg;
+  out[2] = p.own.mt;
+  out[3] = p.own.row_groups;
+  out[4] = p.whole ? 1 : p.chunks;
+  out[5] = p.whole ? 1 : p.own.chunks;
+  return kOk;
 }
 
 int tallax_kv_decode_shared(const tallax_kv_cache* cache, const int32_t* prefix_table, int64_t prefixes,
