@@ -410,7 +410,9 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
     insert_four<L>(key, k);
   }
   bool near = false;
-  auto value = [&](int k) { return from_ordered(k & (exact ? (int)0xffff0000 : ~a.places)); };
+  // A key's logit, or score plus bias, without the expert's place: as it is where bfloat16 left its bits free (a negative
+  // number's are ones in its order), else the end of what the key stands for.
+  auto value = [&](int k) { return from_ordered(!exact ? k & ~a.places : k < 0 ? k | 0xffff : k & (int)0xffff0000); };
   // in 64 bits, for the few tokens that need it
   auto exact_sum = [&]() {
     double all = 0.0;

@@ -1,0 +1,48 @@
+"""GPU: experts.route where its 32-bit keys, ranks and sums leave a choice open, and where scores are far from 1."""
+import numpy as np
+import pytest
+import torch
+
+from tests import layer_ref as L
+from tests.gpu_util import host_values
+from tests.test_gpu_route import _check, _run
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(gpu, x, k, dtype="f32", bias=None, least=1.0, **kw):
+    """As _check, row by row: those whose border leaves nothing open (a share of `least` of them, at least)."""
+    values = host_values(x.astype(np.float32), dtype).astype(np.float64)
+    b = None if bias is None else np.asarray(bias, np.float32).astype(np.float64)
+    w, got = _run(gpu, x.astype(np.float32), k, dtype, bias, **kw)
+    assert np.isfinite(w).all()
+    checked = 0
+    for t in range(len(x)):
+        want, ids, margin = L.route(values[t:t + 1], k, bias=b, **kw)
+        if margin <= 1e-13:  # the device's 64-bit scores are off by less
+            continue
+        checked += 1
+        assert np.array_equal(got[t], ids[0]), (t, got[t], ids[0])
+        assert (np.abs(w[t] - want[0]) <= np.abs(want[0]) * 32 * L.F32 + 2.0 ** -148).all(), t
+    assert checked >= least * len(x), checked
+    return w, got
+
+
+# --- bfloat16 keys that hold the expert's number ---------------------------------------------------------------
+@pytest.mark.parametrize("logits,groups,top_groups,k,want", [
+    ([-1.0, -1.0, 149 / 1024, -10.0], 2, 1, 2, [0, 1]),  # ranks .5379 and .5364
+    ([-1.40625, 1.0546875, -0.31835938, -1.9609375, 1.7890625, -1.0625, 0.578125, -0.859375], 4, 2, 3, [4, 1, 5])])
+def test_ranks_of_negative_logits_by_hand(gpu, logits, groups, top_groups, k, want):
+    x = np.tile(np.asarray(logits, np.float32), (5, 1))
+    _, ids = _check(gpu, x, k, "bf16", score="sigmoid", groups=groups, top_groups=top_groups, group_score="top2")
+    assert (ids == want).all()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("mean,spread", [(-3.0, 0.5), (-3.0, 1.5), (-8.0, 1.0), (0.0, 1.5)])
+@pytest.mark.parametrize("experts,groups,top_groups,k", [(16, 8, 4, 3), (32, 16, 5, 6), (24, 8, 3, 4), (256, 8, 4, 8),
+                                                         (60, 4, 2, 6), (48, 3, 1, 10)])
+def test_ranks_of_negative_logits(gpu, score, mean, spread, experts, groups, top_groups, k):
+    rng = np.random.default_rng(experts + groups)
+    x = rng.standard_normal((1500, experts)) * spread + mean
+    _rows(gpu, x, k, "bf16", score=score, groups=groups, top_groups=top_groups, group_score="top2", least=0.99)
