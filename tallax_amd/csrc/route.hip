@@ -451,6 +451,7 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
     if (a.bias) {
       room += cut * fabsf(v1);
       rank += v1;
+      if (!(fabsf(rank) <= kMost)) room = INFINITY;  // past float32: only 64 bits tell it from others
     } else if (a.group_top == 2) {
       const float far = fmaxf(fabsf(rank), fabsf(v1)) + fabsf(top);
       rank = score_of(rank) + (two ? score_of(v1) : 0.0f);

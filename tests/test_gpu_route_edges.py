@@ -46,3 +46,34 @@ def test_ranks_of_negative_logits(gpu, score, mean, spread, experts, groups, top
     rng = np.random.default_rng(experts + groups)
     x = rng.standard_normal((1500, experts)) * spread + mean
     _rows(gpu, x, k, "bf16", score=score, groups=groups, top_groups=top_groups, group_score="top2", least=0.99)
+
+
+# --- ranks past float32 -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("order", [0, 1, 2])
+def test_ranks_past_float32(gpu, dtype, score, sign, order):
+    """Biases whose sum of two leaves float32 (an infinite one counts as the largest number): ranks still differ."""
+    rng = np.random.default_rng(order)
+    x = rng.standard_normal((40, 16))
+    small = np.asarray([3.0e38, 3.2e38, 2.1e38, 2.0e38])[np.roll(np.arange(4), order)]
+    bias = np.zeros((4, 4)) if sign > 0 else np.full((4, 4), -np.inf)
+    bias[:, 2], bias[:, 1] = sign * np.inf, sign * small
+    for top_groups in (1, 2, 3):
+        _check(gpu, x, 4 * top_groups, dtype, bias.reshape(-1), score=score, groups=4, top_groups=top_groups,
+               group_score="top2")
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_masked_group_before_one_that_is_not_there(gpu, score):
+    """A group whose biases are -inf ranks before one without an expert, whatever their numbers."""
+    x = np.random.default_rng(1).standard_normal((24, 32))
+    x[:, :8] = -np.inf
+    bias = np.zeros(32)
+    bias[8:16] = -np.inf
+    bias[16:24] = -3.0e38
+    for top_groups in (2, 3):
+        for how in ("max", "top2"):
+            _check(gpu, x, 8, "f32", bias, score=score, groups=4, top_groups=top_groups, group_score=how)
+            _check(gpu, x, 8 * top_groups, "f32", bias, score=score, groups=4, top_groups=top_groups, group_score=how)
