@@ -549,8 +549,8 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
   const int at = expert_of(mine, from);
   const bool picked = valid & (l < picks) & (mine != kNone);
   const float logit = picked ? fminf(logit_at<BF16>(a, token, at), kMost) : -INFINITY;
-  // scores that 64 bits may not hold, and whose sum may be 0
-  if (a.renormalise && (a.sigmoid || scores)) near = near | (picked & (logit - top < -700.0f));
+  // scores that 64 bits may not hold, and whose sum may be 0, or that power() does not reach (2^-1000 is e^-693.1)
+  if (a.renormalise && (a.sigmoid || scores)) near = near | (picked & (logit - top < -690.0f));
   const uint64_t unsure = __ballot(near & valid);
   const bool chosen = picked && ((unsure >> (lane & 48)) & 0xffff) == 0;
   double w = 0.0;

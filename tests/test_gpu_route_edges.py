@@ -77,3 +77,28 @@ def test_a_masked_group_before_one_that_is_not_there(gpu, score):
         for how in ("max", "top2"):
             _check(gpu, x, 8, "f32", bias, score=score, groups=4, top_groups=top_groups, group_score=how)
             _check(gpu, x, 8 * top_groups, "f32", bias, score=score, groups=4, top_groups=top_groups, group_score=how)
+
+
+# --- scores far from 1 ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("low,high", [(-692.0, -680.0), (-699.9, -691.0), (-720.0, -695.0), (-745.0, -690.0)])
+def test_sigmoids_that_64_bits_just_hold(gpu, dtype, low, high):
+    """Weights of scores of 1e-300: a power's range is not left where scores still have a sum."""
+    rng = np.random.default_rng(2)
+    x = np.full((50, 64), -900.0)
+    for t in range(50):
+        x[t, rng.choice(64, 12, replace=False)] = rng.uniform(low, high, 12)
+    _check(gpu, x, 8, dtype, score="sigmoid")
+
+
+def test_softmax_weights_far_below_the_largest(gpu):
+    """The largest logit is not chosen; the chosen ones are e^-690 and less of it."""
+    rng = np.random.default_rng(3)
+    x = np.full((30, 64), -800.0)
+    bias = np.zeros(64)
+    bias[0] = -2.0
+    bias[8:16] = 1.0 + np.arange(8) / 8
+    x[:, 0] = 0.0
+    for low, high in ((-680.0, -600.0), (-699.0, -691.0), (-703.0, -685.0)):
+        x[:, 8:16] = rng.uniform(low, high, (30, 8))
+        _check(gpu, x, 8, "f32", bias)
