@@ -314,11 +314,14 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
   extern __shared__ double lds[];  // [waves][experts], where there are groups
   constexpr float kLog2e = 1.44269504088896340736f;
   // How far apart two keys must lie: the place takes the last bits of 24 of each, so that both are too small, by up to
-  // `cut` of themselves; a score is off by the rounding of its exponent (at most .3 of 2^-23 of the largest score, since
-  // s |x| has a maximum), of its exponential, sum and reciprocal (2^-23 of itself each) and of the sum with the bias: by
-  // less than 2^-21 of the largest, two by 2^-20.
+  // `cut` of themselves; a score is off by the rounding of its exponent (at most .6 of 2^-23 of the largest score, since
+  // s |x| has a maximum), of its exponential and reciprocal (2^-23 of itself each) and of the sum with the bias: by less
+  // than 2^-21 of the largest, two by 2^-20.  A softmax's sum is off by up to `each` half steps for as many additions of a
+  // lane, by three for each of its rescalings, of which there is one in four experts at most, and by less than 13 steps
+  // for its terms' exponents (of up to 7, where 1024 of them make half of the sum), the lanes' join and the quotient.  That
+  // moves all scores alike, two of them apart by as much of the largest.
   const float cut = (a.places + 1) * 1.1920929e-7f;
-  constexpr float kOff = 9.5367432e-7f;
+  const float off = 9.5367432e-7f + (a.sigmoid ? 0.0f : (a.each + 16) * 1.1920929e-7f);
   const int wave = threadIdx.x / kWave, lane = lane_id(), l = lane & 15;
   const int64_t first = ((int64_t)blockIdx.x * kRouteWaves + wave) * 4, token = first + lane / 16;
   if (first >= a.tokens) return;
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
   // whether two keys, in this order, are too near to tell
   auto close = [&](int larger, int smaller) {
     const float p = value(larger), q = value(smaller);
-    return (smaller != kNone) & (a.bias ? p - q <= cut * fmaxf(fabsf(p), fabsf(q)) + kOff * largest : p == q);
+    return (smaller != kNone) & (a.bias ? p - q <= cut * fmaxf(fabsf(p), fabsf(q)) + off * largest : p == q);
   };
   auto expert_of = [&](int k, int lane_of) {
     return exact ? 0xffff - (k & 0xffff)
@@ -455,12 +458,12 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
     } else if (a.group_top == 2) {
       const float far = fmaxf(fabsf(rank), fabsf(v1)) + fabsf(top);
       rank = score_of(rank) + (two ? score_of(v1) : 0.0f);
-      room = 2.0f * (cut + kOff) * rank * (1.0f + far);
+      room = 2.0f * (cut + off) * rank * (1.0f + far);
     }
     const bool none = k0 == kNone || group >= a.groups;
     if (whole) rank = __int_as_float(0);
     rank = none ? -INFINITY : rank;
-    room = row_max_f(none ? 0.0f : room) + (a.bias ? a.group_top * kOff * largest : 0.0f);
+    room = row_max_f(none ? 0.0f : room) + (a.bias ? a.group_top * off * largest : 0.0f);
     const int number = none ? kNone : k0;
     int before = 0;
     float over = INFINITY, under = INFINITY;  // to the nearest group that comes before, and after

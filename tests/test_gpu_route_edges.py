@@ -102,3 +102,22 @@ def test_softmax_weights_far_below_the_largest(gpu):
     for low, high in ((-680.0, -600.0), (-699.0, -691.0), (-703.0, -685.0)):
         x[:, 8:16] = rng.uniform(low, high, (30, 8))
         _check(gpu, x, 8, "f32", bias)
+
+
+# --- the softmax's sum ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("experts,groups,group_score", [(1024, 1, "max"), (1017, 9, "max"), (1017, 9, "top2"), (1023, 3, "max"),
+                                                        (512, 1, "max"), (256, 1, "max")])
+def test_a_sum_whose_small_terms_are_lost(gpu, dtype, experts, groups, group_score):
+    """Terms of less than half a step of a float32 sum, as many as a lane holds: their scores' order hangs on them."""
+    size = experts // groups
+    x = np.full((9, experts), -200.0)
+    lane = 116 if groups == 9 else 88 if groups == 3 else experts // 16
+    x[:, 1:min(lane, size)] = -16.75  # e^-16.75 = 5.3e-8, which 1 in float32 does not feel
+    x[:, 0] = 0.0
+    other = size if groups > 1 else experts - 1
+    lost = (min(lane, size) - 1) * np.exp(-16.75)  # the first expert's score is 1 less this
+    for part in (0.3, 0.6, 0.9, 1.1, 1.5):
+        bias = np.full(experts, -5.0)
+        bias[0], bias[other] = -1.0, -part * lost
+        _check(gpu, x, 1, dtype, bias, groups=groups, top_groups=1, group_score=group_score)
