@@ -562,7 +562,7 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
   } else {
     const float base = a.renormalise ? row_max_f(logit) : top;
     w = power((double)logit - (double)base);
-    if (!a.renormalise) w *= reciprocal((double)sum);
+    if (!a.renormalise) w *= reciprocal(exact_sum());  // of 32 bits it would be off by some steps of the weight
   }
   int place = chosen ? l : 16;
   if (__ballot(order & chosen)) {

@@ -121,3 +121,22 @@ def test_a_sum_whose_small_terms_are_lost(gpu, dtype, experts, groups, group_sco
         bias = np.full(experts, -5.0)
         bias[0], bias[other] = -1.0, -part * lost
         _check(gpu, x, 1, dtype, bias, groups=groups, top_groups=1, group_score=group_score)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("experts,k,groups", [(64, 6, 1), (256, 8, 8), (1024, 16, 1), (700, 5, 4), (60, 20, 1)])
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_weights_are_rounded_once(gpu, dtype, experts, k, groups, renormalise):
+    """A weight is its score in 64 bits, rounded to float32: by which way a token goes its bits do not differ by more."""
+    rng = np.random.default_rng(experts)
+    for spread in (0.2, 1.5, 6.0):
+        x = rng.standard_normal((60, experts)) * spread
+        for bias in (None, rng.standard_normal(experts) * 0.05):
+            kw = dict(renormalise=renormalise, groups=groups, top_groups=max(1, groups // 2))
+            values = host_values(x.astype(np.float32), dtype).astype(np.float64)
+            want, ids, margin = L.route(values, k, bias=None if bias is None else bias.astype(np.float32).astype(np.float64), **kw)
+            assert margin > 1e-13
+            w, got = _run(gpu, x.astype(np.float32), k, dtype, bias, **kw)
+            assert np.array_equal(got, ids)
+            # half a step of float32, and 2^-30 for an exponential of 2^-32, a sum of those and a quotient of 2^-40
+            assert (np.abs(w - want) <= np.abs(want) * (L.F32 + 2.0 ** -30) + 2.0 ** -149).all()
