@@ -535,16 +535,18 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
     // where a lane's whole list may be chosen, or next: whether the last choice is as near to what it had no room for
     if (a.k >= L - 1) near = near | ((l == a.k - 1) & close(mine, row_max(end)));
     order = (l > 0) & (l < a.k) & close(row_ror<1>(mine), mine);
-    if (__ballot(edge & valid)) {  // then the next is a choice too, of which one is left out
+    const uint64_t edges = __ballot(edge & valid);
+    if (edges) {  // then the next is a choice too, of which one is left out; of other tokens of the wave it is not
       if (a.k == 16) {
         near = near | edge;
       } else {
         const int src = __ffs((int)(uint32_t)((__ballot(key[0] == next) >> (lane & 48)) & 0xffff)) - 1;
         const int third = row_max(l == src ? key[1] : key[0]);
         near = near | (edge & close(mine, third));
-        mine = l == a.k ? next : mine;
-        from = l == a.k ? src : from;
-        picks = a.k + (next != kNone);
+        const bool here = (edges >> (lane & 48)) & 0xffff;
+        mine = here & (l == a.k) ? next : mine;
+        from = here & (l == a.k) ? src : from;
+        picks = a.k + (here & (next != kNone));
         order = order | edge;
       }
     }

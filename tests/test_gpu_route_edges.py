@@ -140,3 +140,24 @@ def test_weights_are_rounded_once(gpu, dtype, experts, k, groups, renormalise):
             assert np.array_equal(got, ids)
             # half a step of float32, and 2^-30 for an exponential of 2^-32, a sum of those and a quotient of 2^-40
             assert (np.abs(w - want) <= np.abs(want) * (L.F32 + 2.0 ** -30) + 2.0 ** -149).all()
+
+
+# --- rows, and what is beside them ----------------------------------------------------------------------------------
+def test_a_row_is_what_it_is_alone(gpu):
+    """A token whose last choice is open beside others changes no bit of theirs."""
+    from tallax_amd import experts
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((16000, 256)).astype(np.float32)
+    bias = np.zeros(256, np.float32)
+    biased = rng.choice(255, 8, replace=False)
+    bias[biased] = 0.3
+    # every fourth token: expert 255's score is the others' and 0.3, as near as float32 comes: (e^v - 1) / (e^v + 255) = .3
+    near = np.zeros(256, np.float32)
+    b = float(np.float32(0.3))
+    near[255] = np.log((1 + 255 * b) / (1 - b))
+    x[::4] = near
+    d, bias_d = torch.from_numpy(x).to(gpu), torch.from_numpy(bias).to(gpu)
+    w, ids = experts.route(d, 8, bias=bias_d)
+    rest = torch.arange(16000, device=gpu) % 4 != 0
+    alone = experts.route(d[rest].contiguous(), 8, bias=bias_d)
+    assert torch.equal(ids[rest], alone[1]) and torch.equal(w[rest], alone[0])
