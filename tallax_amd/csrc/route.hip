@@ -606,7 +606,7 @@ static int launch_route(RouteArgs a, hipStream_t s) {
   if (a.groups <= 16 && a.k <= 16) {
     const int bytes = BF16 ? 2 : 4;
     a.shift = shift;
-    a.each = (((a.per_group + (1 << shift) - 1) >> shift) + 3) / 4 * 4;  // at most 64
+    a.each = (((a.per_group + (1 << shift) - 1) >> shift) + 3) / 4 * 4;  // at most 116: 9 groups of 113, with 127 places
     a.places = 3;
     while (a.places < a.each - 1) a.places = 2 * a.places + 1;
     a.vectors = ((uintptr_t)a.logits | (uintptr_t)(a.row_stride * bytes)) % (4 * bytes) == 0 && (uintptr_t)a.bias % 16 == 0 &&

@@ -104,6 +104,59 @@ def test_softmax_weights_far_below_the_largest(gpu):
         _check(gpu, x, 8, "f32", bias)
 
 
+def test_large_logits_and_biases_row_by_row(gpu):
+    """Scores that saturate, that vanish, and biases far larger than them: each row whose border is not open."""
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((40, 128)) * 30
+    for dtype in ("f32", "bf16"):
+        for score in ("softmax", "sigmoid"):
+            for bias in (None, rng.standard_normal(128) * 100, rng.integers(-3, 4, 128) * 0.5):
+                for groups, top in ((1, 1), (16, 4), (4, 1)):
+                    for how in ("max", "top2"):
+                        _border(gpu, x, 8, dtype, bias, score=score, groups=groups, top_groups=top, group_score=how)
+
+
+def _border(gpu, x, k, dtype, bias, **kw):
+    """Rows by what decides: the last group that is open against the first that is not, and each choice against the
+    next.  Those apart by more than 1e-13, or equal, have to come out; of others what comes out is as good to 1e-12."""
+    values = host_values(x.astype(np.float32), dtype).astype(np.float64)
+    b = None if bias is None else np.asarray(bias, np.float32).astype(np.float64)
+    w, got = _run(gpu, x.astype(np.float32), k, dtype, bias, **kw)
+    want, ids, _ = L.route(values, k, bias=b, **kw)
+    size, closed = x.shape[1] // kw["groups"], 0
+    for t in range(len(x)):
+        v = values[t]
+        s = np.exp(v - v.max()) / np.exp(v - v.max()).sum() if kw["score"] == "softmax" else 1.0 / (1.0 + np.exp(-v))
+        key = s if b is None else s + b
+        element = v if b is None else key
+        use = element if kw["group_score"] == "max" and b is None else key
+        n = 2 if kw["group_score"] == "top2" else 1
+        rank = np.sort(use.reshape(-1, size), -1)[:, ::-1][:, :n].sum(-1)
+        order = np.argsort(-rank, kind="stable")
+        gap = rank[order[kw["top_groups"] - 1]] - rank[order[kw["top_groups"]]] if kw["top_groups"] < kw["groups"] else 1.0
+        open_ = np.isin(np.arange(x.shape[1]) // size, order[:kw["top_groups"]])
+        # equal ranks: of scores and biases that are the same numbers, or of scores that are 1 (e^-40 is below 2^-54)
+        both = order[kw["top_groups"] - 1:kw["top_groups"] + 1]
+        ones = np.sort(v.reshape(-1, size)[both], -1)[:, ::-1][:, :n].min() > 40.0
+        sure = (gap == 0.0 and (b is not None or ones)) or gap > 1e-13
+        if b is not None:
+            d = -np.diff(np.sort(-np.where(open_, element, -np.inf))[:k + 1])
+            d = np.abs(d[np.isfinite(d)])
+            sure = sure and bool(((d == 0) | (d > 1e-13)).all())
+        if sure:
+            closed += 1
+            assert np.array_equal(got[t], ids[t]), (t, kw)
+            assert (np.abs(w[t] - want[t]) <= np.abs(want[t]) * 32 * L.F32 + 2.0 ** -148).all(), (t, kw)
+            continue
+        taken = sorted({int(g) for g in got[t] // size})
+        assert len(taken) <= kw["top_groups"] and len(set(got[t].tolist())) == k
+        assert all(rank[g] >= rank[order[kw["top_groups"] - 1]] - 1e-12 for g in taken)
+        assert (np.diff(element[got[t]]) <= 1e-12).all()
+        share = s[got[t]] / max(s[got[t]].sum(), 1e-300)
+        assert (np.abs(w[t] - share) <= 32 * L.F32 * share + 2.0 ** -40).all()
+    assert closed >= 6, (closed, kw)  # of 40: sums of two that saturate leave the most open
+
+
 # --- the softmax's sum ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("experts,groups,group_score", [(1024, 1, "max"), (1017, 9, "max"), (1017, 9, "top2"), (1023, 3, "max"),
@@ -161,3 +214,15 @@ def test_a_row_is_what_it_is_alone(gpu):
     rest = torch.arange(16000, device=gpu) % 4 != 0
     alone = experts.route(d[rest].contiguous(), 8, bias=bias_d)
     assert torch.equal(ids[rest], alone[1]) and torch.equal(w[rest], alone[0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups,k", [(1017, 9, 2, 16), (1017, 9, 5, 7), (1023, 3, 1, 8), (1023, 3, 2, 16),
+                                                         (1020, 5, 2, 8), (1015, 7, 3, 16)])
+def test_groups_of_many_experts_to_a_lane(gpu, dtype, score, experts, groups, top_groups, k):
+    rng = np.random.default_rng(experts + top_groups)
+    x = rng.standard_normal((37, experts)) * 1.5
+    for bias in (None, rng.standard_normal(experts) * 0.05):
+        for how in ("max", "top2"):
+            _rows(gpu, x, k, dtype, bias, score=score, groups=groups, top_groups=top_groups, group_score=how, least=0.9)
