@@ -490,8 +490,8 @@ int tallax_verify(const int32_t* draft, const void* logits, int logits_dtype, in
  * nothing to a group, and are chosen after all others of the chosen groups,
  * lowest first, with weight 0.  +inf logits and infinite biases count as the
  * largest finite ones.  experts up to 1024, groups up to 64, k up to 64 and to
- * top_groups * experts / groups, tokens up to 2^25.  out_weights f32, out_ids
- * int32 [tokens, k].
+ * top_groups * experts / groups, tokens up to 2^25, row strides up to 2^37.
+ * out_weights f32, out_ids int32 [tokens, k].
  * ---------------------------------------------------------------------- */
 int tallax_route(const void* logits, int logits_dtype, int64_t tokens, int64_t experts, int64_t row_stride, int64_t k,
                  int sigmoid, const float* bias, int64_t groups, int64_t top_groups, int group_top, int renormalise,

@@ -644,8 +644,9 @@ int tallax_route(const void* logits, int logits_dtype, int64_t tokens, int64_t e
     return kInvalidArgument;
   }
   if (experts > kMostExperts || groups > kMostGroups || k > kMostChosen || tokens > (1 << 25) ||
-      row_stride > ((int64_t)1 << 31)) {
-    set_error("route: up to %d experts, %d groups, %d chosen, 2^25 tokens", kMostExperts, kMostGroups, kMostChosen);
+      row_stride > ((int64_t)1 << 37)) {  // the logits' addresses are 64 bits wide
+    set_error("route: up to %d experts, %d groups, %d chosen, 2^25 tokens, rows up to 2^37 elements apart", kMostExperts,
+              kMostGroups, kMostChosen);
     return kUnsupported;
   }
   if (tokens == 0) return kOk;

@@ -226,3 +226,18 @@ def test_groups_of_many_experts_to_a_lane(gpu, dtype, score, experts, groups, to
     for bias in (None, rng.standard_normal(experts) * 0.05):
         for how in ("max", "top2"):
             _rows(gpu, x, k, dtype, bias, score=score, groups=groups, top_groups=top_groups, group_score=how, least=0.9)
+
+
+def test_rows_that_lie_far_apart(gpu):
+    """Rows more than 2^31 elements from each other, and one row of a stride that is never taken."""
+    from tallax_amd import experts
+    rng = np.random.default_rng(11)
+    stride = 2 ** 31 + 40
+    x = torch.from_numpy(rng.standard_normal((2, 64)).astype(np.float32)).to(gpu).bfloat16()
+    far = torch.empty(stride + 64, dtype=torch.bfloat16, device=gpu)
+    rows = far.as_strided((2, 64), (stride, 1))
+    rows.copy_(x)
+    want = experts.route(x, 6)
+    assert all(torch.equal(a, b) for a, b in zip(experts.route(rows, 6), want, strict=True))
+    one = x[:1].as_strided((1, 64), (2 ** 35, 1))
+    assert all(torch.equal(a, b[:1]) for a, b in zip(experts.route(one, 6), want, strict=True))
