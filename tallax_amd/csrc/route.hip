@@ -359,10 +359,10 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
     for (int i = 0; i < 4; ++i) x[i] = j + i < n ? x[i] : -INFINITY;
   };
 
-  // softmax: the sum over all experts, where scores are compared or given as they are
+  // softmax: the sum over all experts, where scores are compared
   const bool scores = a.bias || (a.groups > 1 && a.group_top == 2);
   float top = 0.0f, sum = 1.0f;  // top: 0 for sigmoid scores
-  if (!a.sigmoid && (scores || !a.renormalise)) {
+  if (!a.sigmoid && scores) {
     top = -INFINITY;
     sum = 0.0f;
 #pragma unroll 1
@@ -562,9 +562,20 @@ __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a)
   if (a.sigmoid) {
     w = reciprocal(1.0 + power(-(double)logit));
   } else {
-    const float base = a.renormalise ? row_max_f(logit) : top;
+    // without a bias the largest logit of all is among the choices
+    const float base = a.renormalise || !scores ? row_max_f(logit) : top;
     w = power((double)logit - (double)base);
-    if (!a.renormalise) w *= reciprocal(exact_sum());  // of 32 bits it would be off by some steps of the weight
+    if (!a.renormalise) {  // a sum of 32 bits would be off by some steps of the weight
+      double all = 0.0;
+#pragma unroll 1
+      for (int j = 0; j < a.each; j += 4) {
+        float x[4], b[4];
+        four(j, x, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) all += x[i] > -INFINITY ? power((double)fminf(x[i], kMost) - (double)base) : 0.0;
+      }
+      w *= reciprocal(row_sum_d(all));
+    }
   }
   int place = chosen ? l : 16;
   if (__ballot(order & chosen)) {
