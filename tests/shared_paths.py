@@ -10,23 +10,23 @@ PAGE = 16
 
 
 class Case:
-    def __init__(self, path, rg, mt, dtype, dim, batch, prompts, queries, group, kv_heads, prefix_pages, own_pages):
+    def __init__(self, path, rg, mt, dtype, dim, batch, prompts, queries, group, kv_heads, prefix_pages, own_pages, page=PAGE):
         self.path, self.rg, self.mt, self.dtype, self.dim = path, rg, mt, dtype, dim
         self.batch, self.prompts, self.queries, self.group, self.kv_heads = batch, prompts, queries, group, kv_heads
-        self.prefix_pages, self.own_pages = prefix_pages, own_pages
+        self.prefix_pages, self.own_pages, self.page = prefix_pages, own_pages, page
 
     def __repr__(self):
         t = "bf16" if self.dtype == torch.bfloat16 else "f32"
         return (f"{NAMES[self.path]}-rg{self.rg}-mt{self.mt}-{t}-{self.dim}-{self.batch}x{self.queries}x{self.group}"
-                f"x{self.kv_heads}-{self.prompts}-{self.prefix_pages}-{self.own_pages}")
+                f"x{self.kv_heads}-{self.prompts}-{self.prefix_pages}-{self.own_pages}" + (f"-p{self.page}" if self.page != PAGE else ""))
 
     def plan(self):
         """What the library makes of it."""
         from tallax_amd import _lib
-        n = self.kv_heads * PAGE * self.dim
-        strides = {f"{x}_stride_{y}": s for x in "kv" for y, s in (("page", n), ("head", PAGE * self.dim), ("slot", self.dim))}
+        n = self.kv_heads * self.page * self.dim
+        strides = {f"{x}_stride_{y}": s for x in "kv" for y, s in (("page", n), ("head", self.page * self.dim), ("slot", self.dim))}
         c = _lib.KvCache(k=4096, v=4096, dtype=_lib.BF16 if self.dtype == torch.bfloat16 else _lib.F32, dim=self.dim,
-                         pages=4096, kv_heads=self.kv_heads, page_size=PAGE, block_table=4096, batch=self.batch,
+                         pages=4096, kv_heads=self.kv_heads, page_size=self.page, block_table=4096, batch=self.batch,
                          table_width=self.own_pages, **strides)
         out = (ctypes.c_int32 * 6)()
         _lib.check(_lib.LIB.tallax_testing_shared_plan(ctypes.byref(c), self.prompts, self.prefix_pages, self.queries,
@@ -86,4 +86,27 @@ def cases():
                 add(APART, 4, 2, 40, 1, 1, 20, 5, 60000, 60)
             if not f32 and dim == 128:
                 add(APART, 2, 1, 210, 70, 3, 4, 8, 60, 10)
+    return r
+
+
+def cases_of_pages():
+    """Pages of one slot, of sizes that are no power of two and end inside tiles, and of more than a chunk."""
+    r = []
+    for dtype in (torch.bfloat16, torch.float32):
+        for dim in (64, 128, 192):
+            f32 = dtype == torch.float32
+            mt, narrow = (2 if f32 or dim <= 128 else 1), (4 if f32 and dim > 128 else 2)
+            for page in (1, 7, 24, 100, 1000):
+                for path, rg, m, calls, slots, own in ((ROWS, 0, 1, (4, 2, 3, 2, 2), 1000, 1000), (BOTH, 4, 1, (24, 1, 3, 5, 2), 2100, 1000),
+                                                       (LAST, 4, mt, (132, 1, 5, 4, 2), 2000, 160), (APART, narrow, 1, (60, 10, 1, 6, 4), 960000, 200)):
+                    r.append(Case(path, rg, m, dtype, dim, *calls, -(-slots // page), -(-own // page), page))
+    return r
+
+
+def cases_of_many_rows():
+    """The most rows of a sequence's kv head."""
+    r = []
+    for dtype in (torch.bfloat16, torch.float32):
+        r.append(Case(BOTH, 4, 2, dtype, 64, 1, 1, 1024, 4, 1, 200, 90))
+        r.append(Case(LAST, 4, 2, dtype, 64, 2, 1, 1024, 4, 1, 200, 90))
     return r

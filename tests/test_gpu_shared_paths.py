@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 def _args(c, rng, lens, begins, fill=math.nan):
     """Inputs of the lengths, in tables of the case's width."""
     q, k, v, prefix, begins, table, lens = _make(rng, lens, begins, c.queries, c.group * c.kv_heads, c.kv_heads, c.dim,
-                                                 S.PAGE, c.dtype, fill=fill)
+                                                 c.page, c.dtype, fill=fill)
 
     def wide(t, width):
         pad = torch.full((t.shape[0], max(width - t.shape[1], 0)), -1, dtype=torch.int32)
@@ -27,17 +27,17 @@ def _args(c, rng, lens, begins, fill=math.nan):
 
 
 def _lens(c, most=150):
-    most = min(most, c.own_pages * S.PAGE - c.queries)
+    most = min(most, c.own_pages * c.page - c.queries)
     lens = [0 if i % 11 == 5 else c.queries + i * 37 % most for i in range(c.batch)]
     lens[0] = c.queries + most - 1
     return lens
 
 
 def _begins(c, most=333):
-    return [(min(most, c.prefix_pages * S.PAGE), 70, 0, 1, 129)[i % 5] for i in range(c.prompts)]
+    return [(min(most, c.prefix_pages * c.page), 70, 0, 1, 129)[i % 5] for i in range(c.prompts)]
 
 
-@pytest.mark.parametrize("case", S.cases(), ids=repr)
+@pytest.mark.parametrize("case", S.cases() + S.cases_of_pages(), ids=repr)
 def test_each_path(gpu, case):
     """Lengths of none, counts of none and too many, pages that are missing, unused slots of NaN; the same bits twice."""
     rng = np.random.default_rng(case.dim + case.batch)
@@ -47,10 +47,18 @@ def test_each_path(gpu, case):
     assert all(torch.equal(a, b) for a, b in zip(first, _run(gpu, args), strict=True))
     counts = torch.from_numpy(rng.integers(-1, case.queries + 3, case.batch).astype(np.int32))
     table, prefix = table.clone(), prefix.clone()
-    prefix[0, [1, 2]] = torch.tensor([-1, 99999], dtype=torch.int32)
+    prefix[0, :2] = torch.tensor([-1, 99999], dtype=torch.int32)[:prefix.shape[1]]
     table[0, 0] = -1
     table[-1] = 99999
     _both(gpu, (q, k, v, prefix, begins, table, own), counts=counts)
+
+
+@pytest.mark.parametrize("case", S.cases_of_many_rows(), ids=repr)
+def test_the_most_rows(gpu, case):
+    rng = np.random.default_rng(case.batch)
+    args = _args(case, rng, [1300, 700][:case.batch], [70])
+    _both(gpu, args)
+    _both(gpu, args, counts=torch.tensor([1023, 5][:case.batch], dtype=torch.int32))
 
 
 @pytest.mark.parametrize("case", [c for c in S.cases() if c.dim in (64, 192)], ids=repr)
@@ -70,9 +78,9 @@ def test_each_path_with_values_that_are_not_finite(gpu, case):
     rng = np.random.default_rng(c.dim)
     lens = [c.queries + 20] * c.batch
     lens[1 % c.batch] = 1  # its first queries see the prefix alone
-    if c.own_pages * S.PAGE < lens[0]:
-        lens = [min(n, c.own_pages * S.PAGE) for n in lens]
-    args = _args(c, rng, lens, [min(100, c.prefix_pages * S.PAGE)] * c.prompts)
+    if c.own_pages * c.page < lens[0]:
+        lens = [min(n, c.own_pages * c.page) for n in lens]
+    args = _args(c, rng, lens, [min(100, c.prefix_pages * c.page)] * c.prompts)
     q, k, v, prefix, begins, table, own = args
     bad = torch.zeros(q.shape, dtype=torch.bool)
     per = c.batch // c.prompts
