@@ -350,7 +350,8 @@ int tallax_kv_append(const tallax_kv_cache* cache, const int32_t* lens, const in
  *   x_j = scale * q.k_j, lse = log sum_j exp(x_j), w_j = exp(x_j - lse),
  *   out = sum_j w_j v_j.
  * A query that sees no slot, or whose every x_j is -inf, has out 0 and lse
- * -inf.  out_lse [batch, queries, heads] f32 (optional).  scores, out_scores
+ * -inf.  With a bf16 cache the weights are rounded to bf16 for their product
+ * with the values alone.  out_lse [batch, queries, heads] f32 (optional).  scores, out_scores
  * [batch, kv_heads, table_width * page_size] f32 (both or neither, may be the
  * same buffer): out_scores = scores + the sum of w_j over the queries and the heads of
  * a kv head; other slots are copied.  lens above max_len are taken as max_len

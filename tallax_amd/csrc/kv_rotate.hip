@@ -12,7 +12,7 @@
 //
 // Bound by memory: 4 x 4096 tokens of 32 + 2 x 8 heads of 128, bfloat16, 403 MB,
 // 76 us (5.3 TB/s; a copy of 4 GiB reaches 4.8); 3 x 2501 tokens of 12 + 2 x 12 heads
-// of 80, float32, three axes, 173 MB, 30 us by itself and 42 among other calls, whose
+// of 80, float32, three axes, 173 MB, 31 us by itself and 45 among other calls, whose
 // data then are in the caches.  A token each of 64 sequences takes 4.6 us, the launch
 // and a chain of loads (length, table, tokens); 65 pairs of 192 elements, partners
 // off the vectors' alignment, 395 MB in 101 us (3.9 TB/s).

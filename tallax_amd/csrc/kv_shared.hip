@@ -730,6 +730,11 @@ static void plan_shared(const tallax_kv_cache* c, int64_t prefixes, int64_t quer
   // the outputs, which spares the join and their parts' way.  So where the prefix is short next to its rows (128 sequences
   // behind 512: 49.6 and 56.0), or the decode kernel needs the registers that tiles leave it less of: two sixteens of
   // rows (128 x 5 queries behind 4099: 137 and 162), float32 (50 x 8 heads, one a kv head, behind 1024: 55 and 65).
+  // Both sides were measured with own slots of up to some 1000.  Longer ones that are alike in length fill the card as
+  // well (32 x 5 queries, 32 / 8 heads, lengths of 65536 down to a quarter: 1182 us, where their bytes take 1151; float32,
+  // one query, 16384: 828 and 578).  One long sequence among short ones is what this plan is slow for: its one chunk is what
+  // the call takes (of 31 x 500 slots and one of 4096 90 us, of 16384 242, of 65536 997, where kv_decode's chunks take 33, 59
+  // and 199 for the own slots).
   p->last = p->rg && max_len > 0 && c->batch * c->kv_heads * p->own.row_groups >= 256 &&
             (f32 || p->own.mt == 2 || max_prefix < 4 * all);
   if (p->last) {

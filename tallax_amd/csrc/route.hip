@@ -8,9 +8,12 @@
 // tokens whose 32-bit keys leave a choice open (route_exactly).  A row of logits is
 // read once or twice, the second time from the cache, and little else: 16384 tokens
 // of 256 float32 experts in 8 groups, sigmoid with a bias, the two largest, 17.8 MB,
-// take 13.1 us, where reading them takes 3.7.  What bounds it is its instructions:
-// some 10 us are a wave's way through the code, new to the CU, and 2.3 the few waves
-// with a comparison in 64 bits.  130 tokens take 6.8 us, one of 64 experts 3.1.
+// take 13.2 us, where reading them takes 3.7.  What bounds it is its instructions: 1151
+// vector ones a wave, four waves to a SIMD, whose vector unit they keep busy 85 % of the
+// time that they are there; 2.3 us are the few waves with a comparison in 64 bits.  130
+// tokens take 6.5 us, one of 64 experts 3.  A softmax with a bias takes 15.7 us (its sum,
+// and more comparisons in 64 bits, since that sum is of 32), unnormalised 12.0 (10.2 with a
+// sum of 32 bits), bfloat16 without either 7.9.
 #include <math.h>
 
 #include "tx_common.h"
@@ -305,10 +308,9 @@ __device__ __forceinline__ double reciprocal(double x) {
 // without a bias have room for the whole expert's number in the key, which then is
 // exact.
 //
-// Every wave runs through here once, and what it waits for is its instructions, at
-// some 16 cycles each when they are new to the CU: hence the loops, which hold
-// little code (16384 tokens of 256 experts in 8 groups took 17.2 us with everything
-// unrolled).
+// Every wave runs through here once, and what it waits for is its instructions, some
+// 16 cycles each with four waves to a SIMD.  Loops hold little code (16384 tokens of 256
+// experts in 8 groups took 17.2 us with everything unrolled).
 template <bool BF16, int L, int NJ>
 __global__ __launch_bounds__(kRouteWaves * kWave) void route_kernel(RouteArgs a) {
   extern __shared__ double lds[];  // [waves][experts], where there are groups

@@ -31,7 +31,8 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.T
     the lowest id (without a bias by the logits themselves, which no rounding
     of the scores ties).  Comparisons are of 64-bit values.  Their weights are
     the scores, divided by their sum if renormalise (0 where it is 0), times
-    scale.
+    scale, in 64 bits until they are rounded; a token's are the same whatever
+    tokens are beside it.
 
     Experts whose logit is -inf or NaN, or whose bias is NaN, are not there:
     they score 0, add nothing to their group, and are chosen after all others

@@ -88,7 +88,10 @@ def decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_
     default: queries) sees slots below lens[b] - counts[b] + t + 1, queries
     from counts[b] on see none.  Returns (out [batch, queries, heads, dim], lse
     [batch, queries, heads] float32 = log of the sum of exp(scale q.k)); a
-    query that sees nothing gives 0 and -inf.
+    query that sees nothing gives 0 and -inf.  Scores, sums and outputs are
+    float32 until out is rounded; with a bfloat16 cache the weights are rounded
+    to bfloat16 (by 2^-8 of each at most) for their product with the values,
+    not for lse, the division or new_scores.
 
     With scores, returns (out, lse, new_scores): scores plus the weights that
     each slot got, summed over the queries and the heads of its kv head.
@@ -123,11 +126,11 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     Query t of counts[b] sees its whole prefix and the slots that decode would
     show it of its own; queries from counts[b] on see nothing.  A sequence may
     have none of its own (lens 0, or a block_table of width 0).  Returns (out,
-    lse) as decode does, over both parts as one softmax.
+    lse) as decode does, over both parts as one softmax, rounded as decode's.
 
     max_prefix and max_len bound prefix_lens and lens (default: what the tables
     can hold); larger lengths are taken as them, and both parts are split by
-    them.  workspace: as decode's.
+    them.  batch * queries * heads is below 2^24.  workspace: as decode's.
     """
     return _lib.SERVING.decode_shared(q, k_pages, v_pages, prefix_table, prefix_lens, block_table, lens, scale, counts,
                                       max_prefix, max_len, workspace)
