@@ -103,6 +103,21 @@ def cases_of_pages():
     return r
 
 
+def cases_of_dims():
+    """Dims from the smallest on that leave most of a kernel's instance empty, or all but eight elements of it full."""
+    r = []
+    for dtype in (torch.bfloat16, torch.float32):
+        for dim in (8, 24, 56, 72, 104, 136, 248):
+            f32 = dtype == torch.float32
+            mt, narrow = (2 if f32 or dim <= 128 else 1), (4 if f32 and dim > 128 else 2)
+            r.append(Case(ROWS, 0, 1, dtype, dim, 4, 2, 3, 2, 2, 140, 60))
+            r.append(Case(BOTH, 4, 1, dtype, dim, 24, 1, 3, 5, 2, 200, 60))
+            r.append(Case(BOTH, narrow, 1, dtype, dim, 39, 3, 1, 3, 2, 200, 60))
+            r.append(Case(LAST, 4, mt, dtype, dim, 132, 1, 5, 4, 2, 200, 10))
+            r.append(Case(APART, narrow, 1, dtype, dim, 60, 10, 1, 6, 4, 60000, 60))
+    return r
+
+
 def cases_of_many_rows():
     """The most rows of a sequence's kv head."""
     r = []

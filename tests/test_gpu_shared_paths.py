@@ -37,7 +37,7 @@ def _begins(c, most=333):
     return [(min(most, c.prefix_pages * c.page), 70, 0, 1, 129)[i % 5] for i in range(c.prompts)]
 
 
-@pytest.mark.parametrize("case", S.cases() + S.cases_of_pages(), ids=repr)
+@pytest.mark.parametrize("case", S.cases() + S.cases_of_pages() + S.cases_of_dims(), ids=repr)
 def test_each_path(gpu, case):
     """Lengths of none, counts of none and too many, pages that are missing, unused slots of NaN; the same bits twice."""
     rng = np.random.default_rng(case.dim + case.batch)

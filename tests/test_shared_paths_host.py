@@ -16,7 +16,7 @@ def test_each_case_takes_its_path():
         dims = 64 if c.dim <= 64 else 128 if c.dim <= 128 else 256
         reached.add((path, rg, mt, c.dtype, dims, c.queries > 1 or path == S.BOTH))
         reached.add((path, c.dtype, dims, own_chunks > 1))
-    for c in S.cases_of_pages() + S.cases_of_many_rows():
+    for c in S.cases_of_pages() + S.cases_of_dims() + S.cases_of_many_rows():
         assert c.plan()[:3] == [c.path, c.rg, c.mt], (c, c.plan())
     for dtype in (torch.bfloat16, torch.float32):
         for dims in (64, 128, 256):
